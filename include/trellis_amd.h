@@ -37,7 +37,9 @@ enum trellis_codebook {
   TRELLIS_CB_1MAD = 2   /* x*34038481+76625530, byte sum, (y-510)/147.800537109375 (qtip.py:32-37) */
 };
 
-enum trellis_dtype { TRELLIS_F32 = 0, TRELLIS_F16 = 1 };
+/* TRELLIS_BF16: the operators between the packed linears only (residual norm, cache,
+ * attention); the packed linears take the other two. */
+enum trellis_dtype { TRELLIS_F32 = 0, TRELLIS_F16 = 1, TRELLIS_BF16 = 2 };
 
 typedef enum trellis_status {
   TRELLIS_OK = 0,
@@ -57,7 +59,12 @@ typedef enum trellis_status {
   TRELLIS_ERR_GROUP = 14,      /* group of 0 or more than 8 linears, or mixed K / V / codebook */
   TRELLIS_ERR_FLAGS = 15,      /* unknown bits in the flags of an _ex call */
   TRELLIS_ERR_SCRATCH = 16,    /* a _noalloc call needs more than TRELLIS_NOALLOC_SCRATCH_BYTES */
-  TRELLIS_ERR_CAPTURE = 17     /* the first _noalloc call on a device made under stream capture */
+  TRELLIS_ERR_CAPTURE = 17,    /* the first _noalloc call on a device made under stream capture */
+  TRELLIS_ERR_WIDTH = 18,      /* norm width outside 1 .. TRELLIS_NORM_MAX_WIDTH */
+  TRELLIS_ERR_HEADS = 19,      /* head dim not a multiple of 8 in [8,256], query heads not a positive
+                                * multiple of the cache's, or rotary dims not a multiple of 16 in [16,dim] */
+  TRELLIS_ERR_PAGE = 20,       /* page size not a power of 2 in [16,1024], or an empty table or pool */
+  TRELLIS_ERR_KEEP = 21        /* eviction: keep < 1, or recent outside 0 .. keep */
 } trellis_status;
 
 /* Flags of trellis_packed_linear_ex / trellis_packed_linear_group_ex. */
@@ -195,6 +202,91 @@ int trellis_embed_rows(const trellis_desc *W, const int32_t *tokens, int ntok, v
 int trellis_encode_workspace_bytes(int K, uint32_t ntiles, size_t *bytes);
 int trellis_encode_tiles(const float *w, uint32_t ntiles, int K, int codebook, uint32_t *bits,
                          float *dq, void *workspace, size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------- between the packed linears
+ * What a decoder block runs between its linears (the reference's RMSNORM, QKNORM, ROPE, ATTN and
+ * ADD dispatches around a contiguous cache, web/model.js:77-102), for serving: norms around a block
+ * with the residual, a paged key-value cache with its append, attention of one new token per row,
+ * and eviction from the cache. All arithmetic is fp32 with one rounding per output. Rows, tokens
+ * and lengths of 0 are no error. */
+
+/* The norms around a block, for each of `rows` rows of `width` elements:
+ *   b = x, or x * rsqrt(mean(x^2) + eps) * post_weight   (post_weight not NULL)
+ *   h = residual + scale * gate * b                      (residual, gate: NULL leaves them out)
+ *   y = h * rsqrt(mean(h^2) + eps) * weight              (of h before its rounding)
+ *   x: x_dtype, row stride ldx elements; gate: x_dtype, row stride ldg (0: one row for all),
+ *   gate_inner 1, or 0 for one value per row; residual and h: r_dtype; y: y_dtype
+ *   weight, post_weight: f32 [width]
+ * h may be NULL (not wanted) or the residual itself; no other output may overlap an input. */
+#define TRELLIS_NORM_MAX_WIDTH 32768
+int trellis_residual_norm(const void *x, int64_t ldx, int x_dtype, const void *residual,
+                          int64_t ldr, int r_dtype, const void *gate, int64_t ldg, int gate_inner,
+                          const float *post_weight, const float *weight, float scale, float eps,
+                          void *h, int64_t ldh, void *y, int64_t ldy, int y_dtype, int64_t rows,
+                          int width, void *stream);
+
+/* A paged key-value cache of one layer, as one call sees it. Token j of row b is slot
+ * j % page_size of page table[b][j / page_size]. A page id outside [0, pages) is no page: nothing
+ * is written there and its tokens count as absent. A call sees the first max_len tokens of a row. */
+typedef struct trellis_kv_cache {
+  void *k, *v;               /* [pages][heads][page_size][head_dim] of `dtype`, 16-byte aligned */
+  float *scores;             /* accumulated attention weight [pages][heads][page_size], or NULL */
+  int32_t *pos;              /* token positions [pages][heads][page_size], or NULL */
+  const int32_t *table;      /* [rows][width] page ids, row stride table_stride */
+  const int32_t *lens;       /* [rows] tokens per row */
+  int64_t page_stride, head_stride, slot_stride;  /* of k and v, elements, multiples of 8 */
+  int64_t table_stride;
+  int32_t pages, heads, page_size, head_dim;
+  int32_t dtype;             /* TRELLIS_F16 or TRELLIS_BF16 */
+  int32_t rows, width, max_len;
+} trellis_kv_cache;
+
+/* New tokens into the cache: per token, q' = rot(norm(q)) out, rot(norm(k)) and v into the token's
+ * slot, score 0 and its position into the planes (where the cache has them).
+ *   q: [tokens][q_heads][head_dim], k, v: [tokens][heads][head_dim], all x_dtype, token and head
+ *   strides in elements; q_out: [tokens][q_heads][head_dim] contiguous, q_dtype, 16-byte aligned
+ *   starts: [rows + 1], tokens starts[b] .. starts[b+1]-1 belong to row b; NULL: token t is row t's
+ *   lens counts these tokens already: the i-th of row b's n has slot lens[b] - n + i
+ *   positions: [tokens], or NULL: the slots
+ *   q_weight, k_weight: f32 [head_dim], both or neither: norm(x) = x * rsqrt(mean(x^2) + eps) * w
+ *   cos, sin: f32 [n_positions][rot / 2], both or neither: pairs (i, i + rot/2) of the first rot
+ *   dims are turned; a position outside the table makes them NaN
+ * A token of no row, or whose slot the table does not hold, is not stored and its q' is 0. */
+int trellis_kv_append(const trellis_kv_cache *cache, const void *q, int64_t q_token_stride,
+                      int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                      int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                      int64_t v_head_stride, int x_dtype, int tokens, int q_heads,
+                      const int32_t *starts, const int32_t *positions, const float *q_weight,
+                      const float *k_weight, float eps, const float *cos, const float *sin, int rot,
+                      int n_positions, void *q_out, int q_dtype, void *stream);
+
+/* Attention of one new token per row: out[b][i] = sum_j p_j v_j, p = softmax over the row's tokens
+ * of scale * q[b][i] . k_j, with key-value head i / (q_heads / heads). A row without tokens gives 0.
+ *   q: [rows][q_heads][head_dim] of q_dtype, row and head strides in elements
+ *   out: [rows][q_heads][head_dim] contiguous of out_dtype
+ *   accumulate: also scores[token][heads] += the sum of p over the query heads of the key-value
+ *   head (no page may then be in two rows' tables)
+ * The workspace (trellis_attention_workspace_bytes, 256-byte aligned) needs no initialisation; it
+ * may be NULL where the size is 0. */
+int trellis_attention_workspace_bytes(const trellis_kv_cache *cache, int q_heads, int accumulate,
+                                      size_t *bytes);
+int trellis_paged_attention(const trellis_kv_cache *cache, const void *q, int64_t q_row_stride,
+                            int64_t q_head_stride, int q_dtype, int q_heads, float scale,
+                            int accumulate, void *out, int out_dtype, void *workspace,
+                            size_t ws_bytes, void *stream);
+
+/* Eviction: of a row's tokens, per key-value head, `keep` stay: those of the last `recent`
+ * positions (pos >= next_pos[b] - recent; next_pos NULL: the row's length), then those of the
+ * largest score, equal scores by the lowest slot. Kept tokens below slot `keep` stay in their
+ * slots; the others' slots take the kept tokens from above, both in ascending order. Key, value,
+ * score and position move together. out_table NULL: in place (no page may be in two rows' tables).
+ * Otherwise every kept token is copied to its slot of out_table's pages, which must not be among
+ * the table's. new_lens[b] = min(length, keep); it must not be the cache's lens.
+ * Workspace as for the attention. */
+int trellis_evict_workspace_bytes(const trellis_kv_cache *cache, int keep, size_t *bytes);
+int trellis_kv_evict(const trellis_kv_cache *cache, int keep, int recent, const int32_t *next_pos,
+                     const int32_t *out_table, int64_t out_table_stride, int out_width,
+                     int32_t *new_lens, void *workspace, size_t ws_bytes, void *stream);
 
 /* Human-readable name of a status code. */
 const char *trellis_strerror(int status);

@@ -13,7 +13,8 @@ from .format import PackedRecord, fit_block, read_packed, write_packed
 
 __all__ = ["PackedRecord", "read_packed", "write_packed", "fit_block", "TrellisError",
            "TrellisLibraryMissing", "PackedLinear", "PackedGroup", "PackedOps", "load_packed",
-           "encode_tiles", "library", "TrellisLinear", "TrellisGroupLinear", "swap_linears"]
+           "encode_tiles", "library", "TrellisLinear", "TrellisGroupLinear", "swap_linears",
+           "rms_norm", "residual_norm", "append_kv", "paged_attention", "evict_kv", "PagedKVCache"]
 
 
 def library():
@@ -29,4 +30,10 @@ def __getattr__(name):
     if name in ("TrellisLinear", "TrellisGroupLinear", "swap_linears"):
         from . import modules
         return getattr(modules, name)
+    if name in ("rms_norm", "residual_norm"):
+        from . import norms
+        return getattr(norms, name)
+    if name in ("append_kv", "paged_attention", "evict_kv", "PagedKVCache"):
+        from . import kv_cache
+        return getattr(kv_cache, name)
     raise AttributeError(name)

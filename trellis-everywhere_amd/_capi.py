@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("TRELLIS_AMD_LIB") or os.path.join(HERE, "libtrellis_a
 
 # enum trellis_codebook / trellis_dtype (include/trellis_amd.h)
 CB_IDS = {"mcg": 0, "3inst": 1, "1mad": 2}
-DT_F32, DT_F16 = 0, 1
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 STATUS_NAMES = {
     0: "TRELLIS_OK", 1: "TRELLIS_ERR_NULL", 2: "TRELLIS_ERR_SHAPE", 3: "TRELLIS_ERR_BLOCK",
@@ -23,7 +23,8 @@ STATUS_NAMES = {
     8: "TRELLIS_ERR_ALIGN", 9: "TRELLIS_ERR_DTYPE", 10: "TRELLIS_ERR_WORKSPACE",
     11: "TRELLIS_ERR_BATCH", 12: "TRELLIS_ERR_RANGE", 13: "TRELLIS_ERR_LAUNCH",
     14: "TRELLIS_ERR_GROUP", 15: "TRELLIS_ERR_FLAGS", 16: "TRELLIS_ERR_SCRATCH",
-    17: "TRELLIS_ERR_CAPTURE",
+    17: "TRELLIS_ERR_CAPTURE", 18: "TRELLIS_ERR_WIDTH", 19: "TRELLIS_ERR_HEADS",
+    20: "TRELLIS_ERR_PAGE", 21: "TRELLIS_ERR_KEEP",
 }
 
 # TRELLIS_NOALLOC_SCRATCH_BYTES: the static workspace of trellis_packed_linear_group_noalloc
@@ -39,7 +40,9 @@ EXPORTED = ("trellis_workspace_bytes", "trellis_packed_linear", "trellis_decode_
             "trellis_packed_linear_group", "trellis_embed_rows",
             "trellis_encode_workspace_bytes", "trellis_encode_tiles",
             "trellis_packed_linear_ex", "trellis_packed_linear_group_ex",
-            "trellis_packed_linear_group_noalloc")
+            "trellis_packed_linear_group_noalloc", "trellis_residual_norm", "trellis_kv_append",
+            "trellis_attention_workspace_bytes", "trellis_paged_attention",
+            "trellis_evict_workspace_bytes", "trellis_kv_evict")
 
 
 class TrellisLibraryMissing(RuntimeError):
@@ -68,6 +71,30 @@ class TrellisDesc(ctypes.Structure):
         ("block_in", ctypes.c_int32),
         ("block_out", ctypes.c_int32),
         ("nwords", ctypes.c_int32),
+    ]
+
+
+class TrellisKVCache(ctypes.Structure):
+    """struct trellis_kv_cache (include/trellis_amd.h)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("scores", ctypes.c_void_p),
+        ("pos", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("pages", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
     ]
 
 
@@ -129,6 +156,17 @@ def load(path: str | None = None):
                                          ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
                                          ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
     lib.trellis_encode_tiles.restype = ctypes.c_int
+    P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+    C, SZ = ctypes.POINTER(TrellisKVCache), ctypes.c_size_t
+    for name, args in (
+            ("trellis_residual_norm", [P, L, I, P, L, I, P, L, I, P, P, F, F, P, L, P, L, I, L, I, P]),
+            ("trellis_kv_append", [C, P, L, L, P, L, L, P, L, L, I, I, I, P, P, P, P, F, P, P, I, I, P, I, P]),
+            ("trellis_attention_workspace_bytes", [C, I, I, ctypes.POINTER(SZ)]),
+            ("trellis_paged_attention", [C, P, L, L, I, I, F, I, P, I, P, SZ, P]),
+            ("trellis_evict_workspace_bytes", [C, I, ctypes.POINTER(SZ)]),
+            ("trellis_kv_evict", [C, I, I, P, P, L, I, P, P, SZ, P])):
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, ctypes.c_int
     lib.trellis_strerror.argtypes = [ctypes.c_int]
     lib.trellis_strerror.restype = ctypes.c_char_p
     lib.trellis_version.argtypes = []

@@ -1,0 +1,418 @@
+// serve.hip — C ABI of the operators between the packed linears (include/trellis_amd.h): validation,
+// launch planning and the dispatch to norm.h, append.h, attend.h and evict.h.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstring>
+
+#include "trellis_amd.h"
+#include "append.h"
+#include "attend.h"
+#include "evict.h"
+#include "norm.h"
+
+using namespace trellis;
+
+namespace {
+
+bool known_dtype(int dt) { return dt == TRELLIS_F32 || dt == TRELLIS_F16 || dt == TRELLIS_BF16; }
+int dtype_size(int dt) { return dt == TRELLIS_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int launched() { return hipGetLastError() == hipSuccess ? TRELLIS_OK : TRELLIS_ERR_LAUNCH; }
+int log2_of(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+// Workgroups of a launch: HIP counts threads in 32 bits per dimension.
+bool grid_fits(int64_t blocks, int threads) { return blocks * threads < (int64_t(1) << 32) && blocks < (int64_t(1) << 31); }
+
+int device_cus() {
+  static const int cus = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+      return 256;
+    return n;
+  }();
+  return cus;
+}
+
+// ---------------------------------------------------------------- residual norm
+
+template <class TX, class TR>
+void launch_norm(const NormArgs& a, bool vec, int64_t rows, hipStream_t st) {
+  // up to 8192 elements one chunk of 8 a thread, above four
+  const int chunks = a.width <= 8192 ? 1 : 4;
+  const int threads = ((a.width + 8 * chunks - 1) / (8 * chunks) + 63) / 64 * 64;
+  const dim3 grid(static_cast<unsigned>(rows)), block(threads);
+  if (vec && chunks == 1) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 1>), grid, block, 0, st, a);
+  else if (vec) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 4>), grid, block, 0, st, a);
+  else if (chunks == 1) hipLaunchKernelGGL((norm_kernel<TX, TR, false, 1>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((norm_kernel<TX, TR, false, 4>), grid, block, 0, st, a);
+}
+
+template <class TX>
+void launch_norm_r(const NormArgs& a, int r_dtype, bool vec, int64_t rows, hipStream_t st) {
+  if (r_dtype == TRELLIS_F32) launch_norm<TX, float>(a, vec, rows, st);
+  else if (r_dtype == TRELLIS_F16) launch_norm<TX, _Float16>(a, vec, rows, st);
+  else launch_norm<TX, bf16_t>(a, vec, rows, st);
+}
+
+// ---------------------------------------------------------------- cache
+
+int validate_cache(const trellis_kv_cache* c) {
+  if (!c || !c->k || !c->v || (c->rows != 0 && (!c->table || !c->lens))) return TRELLIS_ERR_NULL;
+  if (c->dtype != TRELLIS_F16 && c->dtype != TRELLIS_BF16) return TRELLIS_ERR_DTYPE;
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 || c->heads < 1) return TRELLIS_ERR_HEADS;
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) || c->pages < 1 || c->width < 1)
+    return TRELLIS_ERR_PAGE;
+  if (c->rows < 0 || c->max_len < 0) return TRELLIS_ERR_BATCH;
+  // 16-byte rows, and byte offsets within a page that fit 32 bits
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % 8 || c->head_stride % 8 || c->slot_stride % 8 ||
+      c->page_stride < 0 || c->head_stride < 0 || c->slot_stride < c->head_dim ||
+      c->slot_stride >= (int64_t(1) << 30) / c->page_size || c->table_stride < 0)
+    return TRELLIS_ERR_ALIGN;
+  return TRELLIS_OK;
+}
+
+Cache cache_of(const trellis_kv_cache* c) {
+  Cache r;
+  r.k = c->k;
+  r.v = c->v;
+  r.scores = c->scores;
+  r.pos = c->pos;
+  r.table = c->table;
+  r.lens = c->lens;
+  r.page_stride = c->page_stride;
+  r.head_stride = c->head_stride;
+  r.slot_stride = c->slot_stride;
+  r.table_stride = c->table_stride;
+  r.pages = c->pages;
+  r.heads = c->heads;
+  r.page_shift = log2_of(c->page_size);
+  r.d = c->head_dim;
+  r.rows = c->rows;
+  r.width = c->width;
+  r.max_len = c->max_len;
+  return r;
+}
+
+// The tokens of a row that a call can see.
+int longest(const trellis_kv_cache* c) {
+  const int64_t cap = static_cast<int64_t>(c->width) * c->page_size;
+  return static_cast<int>(c->max_len < cap ? c->max_len : cap);
+}
+
+int lanes_per_row(int d) { return 1 << log2_of((d + 7) / 8); }
+
+template <class TX, class TC>
+void launch_append(const AppendArgs& a, bool vec, int lpr, unsigned grid, hipStream_t st) {
+  if (vec) hipLaunchKernelGGL((append_kernel<TX, TC, true>), dim3(grid), dim3(256), 0, st, a, lpr);
+  else hipLaunchKernelGGL((append_kernel<TX, TC, false>), dim3(grid), dim3(256), 0, st, a, lpr);
+}
+
+// ---------------------------------------------------------------- attention
+
+struct AttendPlan {
+  int splits, row_blocks;
+  int64_t logit_stride;
+  size_t off_ml, off_total, off_logits, ws;
+};
+
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
+
+AttendPlan attend_plan(const trellis_kv_cache* c, int q_heads, bool accumulate) {
+  AttendPlan p;
+  const int n = longest(c), group = q_heads / c->heads;
+  p.row_blocks = (group + 15) / 16;
+  const int64_t one = static_cast<int64_t>(c->rows) * c->heads * p.row_blocks;
+  // chunks of at least ATT_CHUNK_MIN tokens, enough of them for four workgroups per CU
+  const int64_t most = (n + ATT_CHUNK_MIN - 1) / ATT_CHUNK_MIN;
+  const int64_t want = one > 0 ? (4LL * device_cus() + one - 1) / one : 1;
+  p.splits = static_cast<int>(want < most ? want : most);
+  if (p.splits < 1) p.splits = 1;
+  const size_t bh = static_cast<size_t>(c->rows) * q_heads;
+  p.logit_stride = (static_cast<int64_t>(n) + 31) / 32 * 32;
+  size_t ws = p.splits > 1 ? up256(bh * p.splits * c->head_dim * 4) : 0;
+  p.off_ml = ws;
+  if (p.splits > 1) ws += up256(bh * p.splits * 8);
+  p.off_total = ws;
+  if (accumulate) ws += up256(bh * 8);
+  p.off_logits = ws;
+  if (accumulate) ws += up256(bh * p.logit_stride * 4);
+  p.ws = ws;
+  return p;
+}
+
+template <class T, int DP>
+void launch_attend(const AttendArgs& a, bool exact, unsigned grid, hipStream_t st) {
+  const bool full = a.c.d == DP;
+  const dim3 block(64 * ATT_WAVES);
+  if (full && exact) hipLaunchKernelGGL((attend_kernel<T, DP, true, true>), dim3(grid), block, 0, st, a);
+  else if (full) hipLaunchKernelGGL((attend_kernel<T, DP, true, false>), dim3(grid), block, 0, st, a);
+  else if (exact) hipLaunchKernelGGL((attend_kernel<T, DP, false, true>), dim3(grid), block, 0, st, a);
+  else hipLaunchKernelGGL((attend_kernel<T, DP, false, false>), dim3(grid), block, 0, st, a);
+}
+
+template <class T>
+void launch_attend_d(const AttendArgs& a, bool exact, unsigned grid, hipStream_t st) {
+  if (a.c.d <= 64) launch_attend<T, 64>(a, exact, grid, st);
+  else if (a.c.d <= 128) launch_attend<T, 128>(a, exact, grid, st);
+  else launch_attend<T, 256>(a, exact, grid, st);
+}
+
+int validate_attention(const trellis_kv_cache* c, int q_heads, int accumulate) {
+  const int v = validate_cache(c);
+  if (v) return v;
+  if (q_heads < 1 || q_heads % c->heads) return TRELLIS_ERR_HEADS;
+  if (accumulate && !c->scores) return TRELLIS_ERR_NULL;
+  return TRELLIS_OK;
+}
+
+// ---------------------------------------------------------------- eviction
+
+int validate_evict(const trellis_kv_cache* c, int keep, int recent) {
+  const int v = validate_cache(c);
+  if (v) return v;
+  if (!c->scores || !c->pos) return TRELLIS_ERR_NULL;
+  if (keep < 1 || recent < 0 || recent > keep) return TRELLIS_ERR_KEEP;
+  return TRELLIS_OK;
+}
+
+struct EvictPlan {
+  size_t off_first, off_second, ws;
+};
+
+EvictPlan evict_plan(const trellis_kv_cache* c, int keep) {
+  EvictPlan p;
+  const size_t bh = static_cast<size_t>(c->rows) * c->heads;
+  p.off_first = up256(bh * 4);
+  p.off_second = p.off_first + up256(bh * keep * 4);
+  p.ws = p.off_second + up256(bh * keep * 4);
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int trellis_residual_norm(const void* x, int64_t ldx, int x_dtype, const void* residual, int64_t ldr,
+                          int r_dtype, const void* gate, int64_t ldg, int gate_inner,
+                          const float* post_weight, const float* weight, float scale, float eps, void* h,
+                          int64_t ldh, void* y, int64_t ldy, int y_dtype, int64_t rows, int width,
+                          void* stream) {
+  if (rows < 0) return TRELLIS_ERR_BATCH;
+  if (width < 1 || width > TRELLIS_NORM_MAX_WIDTH) return TRELLIS_ERR_WIDTH;
+  if (!known_dtype(x_dtype) || !known_dtype(r_dtype) || !known_dtype(y_dtype)) return TRELLIS_ERR_DTYPE;
+  if (rows == 0) return TRELLIS_OK;
+  if (!x || !weight || !y) return TRELLIS_ERR_NULL;
+  if (!grid_fits(rows, 1024)) return TRELLIS_ERR_BATCH;
+  const int xs = dtype_size(x_dtype), rs = dtype_size(r_dtype), ys = dtype_size(y_dtype);
+  if (!aligned(x, xs) || !aligned(y, ys) || (residual && !aligned(residual, rs)) || (h && !aligned(h, rs)) ||
+      (gate && !aligned(gate, xs)) || !aligned(weight, 4) || (post_weight && !aligned(post_weight, 4)) ||
+      (gate_inner != 0 && gate_inner != 1) || (rows > 1 && (ldy < width || (h && ldh < width))))
+    return TRELLIS_ERR_ALIGN;
+  // whole 16-byte accesses everywhere, or none
+  const auto vec16 = [&](const void* p, int64_t ld, int size) { return !p || (aligned(p, 16) && (rows == 1 || ld * size % 16 == 0)); };
+  const bool vec = width % 8 == 0 && vec16(x, ldx, xs) && vec16(residual, ldr, rs) && vec16(h, ldh, rs) &&
+                   vec16(y, ldy, ys) && (gate_inner == 0 || vec16(gate, ldg, xs)) && vec16(weight, 0, 4) &&
+                   vec16(post_weight, 0, 4);
+  NormArgs a;
+  a.x = x;
+  a.residual = residual;
+  a.gate = gate;
+  a.post_w = post_weight;
+  a.w = weight;
+  a.h = h;
+  a.y = y;
+  a.ldx = ldx;
+  a.ldr = ldr;
+  a.ldg = ldg;
+  a.ldh = ldh;
+  a.ldy = ldy;
+  a.width = width;
+  a.gate_inner = gate_inner;
+  a.y_dt = y_dtype;
+  a.scale = scale;
+  a.eps = eps;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (x_dtype == TRELLIS_F32) launch_norm_r<float>(a, r_dtype, vec, rows, st);
+  else if (x_dtype == TRELLIS_F16) launch_norm_r<_Float16>(a, r_dtype, vec, rows, st);
+  else launch_norm_r<bf16_t>(a, r_dtype, vec, rows, st);
+  return launched();
+}
+
+int trellis_kv_append(const trellis_kv_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                      const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                      int64_t v_token_stride, int64_t v_head_stride, int x_dtype, int tokens, int q_heads,
+                      const int32_t* starts, const int32_t* positions, const float* q_weight, const float* k_weight,
+                      float eps, const float* cos, const float* sin, int rot, int n_positions, void* q_out,
+                      int q_dtype, void* stream) {
+  const int bad = validate_cache(cache);
+  if (bad) return bad;
+  if (!known_dtype(x_dtype) || !known_dtype(q_dtype)) return TRELLIS_ERR_DTYPE;
+  if (q_heads < 1 || q_heads % cache->heads) return TRELLIS_ERR_HEADS;
+  if (tokens < 0 || (!starts && tokens != cache->rows)) return TRELLIS_ERR_BATCH;
+  if ((cos != nullptr) != (sin != nullptr) || (q_weight != nullptr) != (k_weight != nullptr)) return TRELLIS_ERR_NULL;
+  if (cos && (rot < 16 || rot % 16 || rot > cache->head_dim)) return TRELLIS_ERR_HEADS;
+  if (cos && n_positions < 1) return TRELLIS_ERR_RANGE;
+  if (tokens == 0) return TRELLIS_OK;
+  if (!q || !k || !v || !q_out) return TRELLIS_ERR_NULL;
+  if (cache->rows < 1) return TRELLIS_ERR_BATCH;
+  const int xs = dtype_size(x_dtype);
+  if (!aligned(q, xs) || !aligned(k, xs) || !aligned(v, xs) || !aligned(q_out, 16)) return TRELLIS_ERR_ALIGN;
+  AppendArgs a;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_t = q_token_stride;
+  a.q_h = q_head_stride;
+  a.k_t = k_token_stride;
+  a.k_h = k_head_stride;
+  a.v_t = v_token_stride;
+  a.v_h = v_head_stride;
+  a.q_out = q_out;
+  a.q_w = q_weight;
+  a.k_w = k_weight;
+  a.cos = cos;
+  a.sin = sin;
+  a.starts = starts;
+  a.positions = positions;
+  a.tokens = tokens;
+  a.hq = q_heads;
+  a.q_dt = q_dtype;
+  a.rot = rot;
+  a.n_positions = n_positions;
+  a.eps = eps;
+  a.c = cache_of(cache);
+  const int per = 16 / xs;
+  const bool vec = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && q_token_stride % per == 0 &&
+                   q_head_stride % per == 0 && k_token_stride % per == 0 && k_head_stride % per == 0 &&
+                   v_token_stride % per == 0 && v_head_stride % per == 0;
+  const int lpr = lanes_per_row(cache->head_dim);
+  const int64_t items = static_cast<int64_t>(tokens) * (q_heads + 2 * static_cast<int64_t>(cache->heads));
+  const int64_t blocks = (items + 256 / lpr - 1) / (256 / lpr);
+  if (!grid_fits(blocks, 256)) return TRELLIS_ERR_BATCH;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool f16 = cache->dtype == TRELLIS_F16;
+  if (x_dtype == TRELLIS_F32) {
+    if (f16) launch_append<float, _Float16>(a, vec, lpr, grid, st);
+    else launch_append<float, bf16_t>(a, vec, lpr, grid, st);
+  } else if (x_dtype == TRELLIS_F16) {
+    if (f16) launch_append<_Float16, _Float16>(a, vec, lpr, grid, st);
+    else launch_append<_Float16, bf16_t>(a, vec, lpr, grid, st);
+  } else {
+    if (f16) launch_append<bf16_t, _Float16>(a, vec, lpr, grid, st);
+    else launch_append<bf16_t, bf16_t>(a, vec, lpr, grid, st);
+  }
+  return launched();
+}
+
+int trellis_attention_workspace_bytes(const trellis_kv_cache* cache, int q_heads, int accumulate, size_t* bytes) {
+  if (!bytes) return TRELLIS_ERR_NULL;
+  const int v = validate_attention(cache, q_heads, accumulate);
+  if (v) return v;
+  *bytes = attend_plan(cache, q_heads, accumulate != 0).ws;
+  return TRELLIS_OK;
+}
+
+int trellis_paged_attention(const trellis_kv_cache* cache, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                            int q_dtype, int q_heads, float scale, int accumulate, void* out, int out_dtype,
+                            void* workspace, size_t ws_bytes, void* stream) {
+  const int v = validate_attention(cache, q_heads, accumulate);
+  if (v) return v;
+  if (!known_dtype(q_dtype) || !known_dtype(out_dtype)) return TRELLIS_ERR_DTYPE;
+  if (cache->rows == 0) return TRELLIS_OK;
+  if (!q || !out) return TRELLIS_ERR_NULL;
+  const int qs = dtype_size(q_dtype);
+  if (!aligned(q, qs) || !aligned(out, dtype_size(out_dtype))) return TRELLIS_ERR_ALIGN;
+  const AttendPlan p = attend_plan(cache, q_heads, accumulate != 0);
+  if (p.ws && (!workspace || ws_bytes < p.ws)) return TRELLIS_ERR_WORKSPACE;
+  if (p.ws && !aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
+  char* ws = static_cast<char*>(workspace);
+  AttendArgs a;
+  a.q = q;
+  a.q_b = q_row_stride;
+  a.q_h = q_head_stride;
+  a.q_dt = q_dtype;
+  a.q_vec = aligned(q, 16) && q_row_stride * qs % 16 == 0 && q_head_stride * qs % 16 == 0;
+  a.out = out;
+  a.out_dt = out_dtype;
+  a.hq = q_heads;
+  a.group = q_heads / cache->heads;
+  a.row_blocks = p.row_blocks;
+  a.splits = p.splits;
+  a.scale = scale * 1.44269504088896340736f;
+  a.part = reinterpret_cast<float*>(ws);
+  a.ml = reinterpret_cast<float*>(ws + p.off_ml);
+  a.total = accumulate ? reinterpret_cast<float*>(ws + p.off_total) : nullptr;
+  a.logits = accumulate ? reinterpret_cast<float*>(ws + p.off_logits) : nullptr;
+  a.logit_stride = p.logit_stride;
+  a.c = cache_of(cache);
+  const int64_t one = static_cast<int64_t>(cache->rows) * cache->heads;
+  const int64_t blocks = one * p.row_blocks * p.splits, bh = static_cast<int64_t>(cache->rows) * q_heads;
+  const int64_t score_blocks = one * ((static_cast<int64_t>(cache->max_len) + 255) / 256);
+  if (!grid_fits(blocks, 64 * ATT_WAVES) || !grid_fits(bh, 256) || (accumulate && !grid_fits(score_blocks, 256)))
+    return TRELLIS_ERR_BATCH;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool exact = q_dtype != cache->dtype || out_dtype == TRELLIS_F32;
+  if (cache->dtype == TRELLIS_F16) launch_attend_d<_Float16>(a, exact, static_cast<unsigned>(blocks), st);
+  else launch_attend_d<bf16_t>(a, exact, static_cast<unsigned>(blocks), st);
+  if (p.splits > 1) hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>(bh)), dim3(256), 0, st, a);
+  if (accumulate && score_blocks > 0)
+    hipLaunchKernelGGL(attend_score_kernel, dim3(static_cast<unsigned>(score_blocks)), dim3(256), 0, st, a);
+  return launched();
+}
+
+int trellis_evict_workspace_bytes(const trellis_kv_cache* cache, int keep, size_t* bytes) {
+  if (!bytes) return TRELLIS_ERR_NULL;
+  const int v = validate_evict(cache, keep, 0);
+  if (v) return v;
+  *bytes = evict_plan(cache, keep).ws;
+  return TRELLIS_OK;
+}
+
+int trellis_kv_evict(const trellis_kv_cache* cache, int keep, int recent, const int32_t* next_pos,
+                     const int32_t* out_table, int64_t out_table_stride, int out_width, int32_t* new_lens,
+                     void* workspace, size_t ws_bytes, void* stream) {
+  const int v = validate_evict(cache, keep, recent);
+  if (v) return v;
+  if (out_table && (out_width < 1 || out_table_stride < 0)) return TRELLIS_ERR_PAGE;
+  if (cache->rows == 0) return TRELLIS_OK;
+  if (!new_lens) return TRELLIS_ERR_NULL;
+  if (new_lens == cache->lens) return TRELLIS_ERR_RANGE;
+  const EvictPlan p = evict_plan(cache, keep);
+  if (!workspace || ws_bytes < p.ws) return TRELLIS_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
+  char* ws = static_cast<char*>(workspace);
+  EvictArgs a;
+  a.c = cache_of(cache);
+  a.next_pos = next_pos;
+  a.out_table = out_table;
+  a.out_stride = out_table_stride;
+  a.out_width = out_width;
+  a.keep = keep;
+  a.recent = recent;
+  a.new_lens = new_lens;
+  a.count = reinterpret_cast<int32_t*>(ws);
+  a.first = reinterpret_cast<int32_t*>(ws + p.off_first);
+  a.second = reinterpret_cast<int32_t*>(ws + p.off_second);
+  const int64_t bh = static_cast<int64_t>(cache->rows) * cache->heads;
+  // the most moves a head can make, in groups of the rows one workgroup moves, up to 64 workgroups a head
+  const int n = longest(cache);
+  const int most = out_table ? (keep < n ? keep : n) : n - keep < keep ? n - keep : keep;
+  const int lpr = lanes_per_row(cache->head_dim);
+  int blocks = most > 0 ? (most + 256 / lpr - 1) / (256 / lpr) : 0;
+  if (blocks > 64) blocks = 64;
+  if (!grid_fits(bh, EV_THREADS) || !grid_fits(bh * blocks, 256)) return TRELLIS_ERR_BATCH;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(bh)), dim3(EV_THREADS), 0, st, a);
+  if (blocks > 0)
+    hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(bh * blocks)), dim3(256), 0, st, a, lpr, blocks);
+  return launched();
+}
+
+}  // extern "C"

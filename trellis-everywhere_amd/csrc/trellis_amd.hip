@@ -620,8 +620,8 @@ const char* trellis_strerror(int status) {
     case TRELLIS_ERR_V: return "V (weights per trellis step) must be 1 or 2";
     case TRELLIS_ERR_CODEBOOK: return "unknown codebook id";
     case TRELLIS_ERR_NWORDS: return "nwords must equal 256*K/32";
-    case TRELLIS_ERR_ALIGN: return "bits must be 16-byte aligned and strides must cover a row";
-    case TRELLIS_ERR_DTYPE: return "x/y dtype must be TRELLIS_F32 or TRELLIS_F16";
+    case TRELLIS_ERR_ALIGN: return "a pointer is not aligned as its kernel reads it (bits, cache: 16 bytes), or a stride does not fit";
+    case TRELLIS_ERR_DTYPE: return "unsupported dtype (a packed linear's x/y: TRELLIS_F32 or TRELLIS_F16)";
     case TRELLIS_ERR_WORKSPACE: return "workspace missing or too small";
     case TRELLIS_ERR_BATCH: return "batch must be >= 1";
     case TRELLIS_ERR_RANGE: return "tile range outside the matrix";
@@ -634,6 +634,12 @@ const char* trellis_strerror(int status) {
     case TRELLIS_ERR_CAPTURE:
       return "the first no-allocation call on a device must not be made under stream capture "
              "(it looks up the device's scratch address)";
+    case TRELLIS_ERR_WIDTH: return "norm width must be in 1 .. TRELLIS_NORM_MAX_WIDTH";
+    case TRELLIS_ERR_HEADS:
+      return "head dim must be a multiple of 8 in [8,256], query heads a positive multiple of the "
+             "cache's heads, rotary dims a multiple of 16 up to the head dim";
+    case TRELLIS_ERR_PAGE: return "page size must be a power of 2 in [16,1024], pool and table not empty";
+    case TRELLIS_ERR_KEEP: return "eviction needs keep >= 1 and 0 <= recent <= keep";
     default: return "unknown trellis status";
   }
 }

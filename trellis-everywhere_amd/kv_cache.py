@@ -1,0 +1,325 @@
+"""A paged key-value cache and the attention that decodes from it (trellis_kv_append,
+trellis_paged_attention, trellis_kv_evict): what a decoder block runs between its q/k/v and its o linear
+(the reference's QKNORM, ROPE, cache copy and ATTN dispatches over one contiguous sequence,
+web/model.js:83-95). For serving: forward only.
+
+append_kv, paged_attention and evict_kv work on tensors that the caller owns; PagedKVCache owns them.
+
+  k_pages, v_pages: [pages, heads, page_size, head_dim] float16 or bfloat16; alike in strides, unit last
+  table: int32 [rows, width], row b's token j in slot j % page_size of page table[b, j // page_size]; an
+         id outside the pool is no page (nothing is written, its tokens count as absent)
+  lens:  int32 [rows], tokens per row
+  scores: float32 and pos: int32, [pages, heads, page_size]: each token's accumulated attention weight
+          and its position
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _capi
+from .norms import _DT, refuse_grad
+from .packed_linear import _stream
+
+
+def _cache(k_pages, v_pages, scores, pos, table, lens, max_len):
+    """The C view of a cache (struct trellis_kv_cache), its arguments checked."""
+    dev, shape, strides = k_pages.device, k_pages.shape, k_pages.stride()
+    if dev.type != "cuda":
+        raise ValueError(f"the cache lives on a GPU, not {dev}")
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != strides or v_pages.dtype != k_pages.dtype:
+        raise ValueError("k_pages and v_pages must be [pages, heads, page_size, head_dim], alike in dtype and strides")
+    dt = _DT.get(k_pages.dtype)
+    if dt is None or dt == _capi.DT_F32:
+        raise ValueError(f"cache dtype {k_pages.dtype} must be float16 or bfloat16")
+    if strides[3] != 1:
+        raise ValueError("k_pages and v_pages must have unit stride over head_dim")
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] != 1):
+        raise ValueError("table must be int32 [rows, width] with unit column stride")
+    rows, width = table.shape
+    if lens.dtype != torch.int32 or lens.shape != (rows,) or not lens.is_contiguous():
+        raise ValueError(f"lens must be a contiguous int32 [{rows}] tensor")
+    s_ptr = p_ptr = None
+    if scores is not None:
+        if scores.dtype != torch.float32 or scores.shape != shape[:3] or not scores.is_contiguous() or scores.device != dev:
+            raise ValueError(f"scores must be a contiguous float32 {list(shape[:3])} tensor on {dev}")
+        s_ptr = scores.data_ptr()
+    if pos is not None:
+        if pos.dtype != torch.int32 or pos.shape != shape[:3] or not pos.is_contiguous() or pos.device != dev:
+            raise ValueError(f"pos must be a contiguous int32 {list(shape[:3])} tensor on {dev}")
+        p_ptr = pos.data_ptr()
+    if v_pages.device != dev or table.device != dev or lens.device != dev:
+        raise ValueError(f"v_pages, table and lens must be on {dev}")
+    pages, heads, page_size, d = shape
+    if max_len is None:
+        max_len = min(width * page_size, 0x7FFFFFFF)
+    return _capi.TrellisKVCache(k_pages.data_ptr(), v_pages.data_ptr(), s_ptr, p_ptr, table.data_ptr(), lens.data_ptr(),
+                                strides[0], strides[1], strides[2], table.stride(0), pages, heads, page_size, d, dt,
+                                rows, width, max_len)
+
+
+def _dtype(name, dtype):
+    dt = _DT.get(dtype)
+    if dt is None:
+        raise ValueError(f"{name} dtype {dtype} must be float32, float16 or bfloat16")
+    return dt
+
+
+def _ints(name, t, shape, dev):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on {dev}")
+    return t.data_ptr()
+
+
+def _workspace(given, need, dev):
+    """The call's scratch: the caller's, or a block of torch's allocator, which hands it on in stream order."""
+    if given is not None:
+        if given.device != dev or not given.is_contiguous():
+            raise ValueError(f"workspace must be contiguous on {dev}")
+        return given, given.data_ptr(), given.numel() * given.element_size()
+    if need == 0:
+        return None, None, 0
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr(), need
+
+
+def append_kv(q, k, v, k_pages, v_pages, table, lens, *, starts=None, positions=None, q_norm=None, k_norm=None,
+              eps: float = 1e-6, cos=None, sin=None, scores=None, pos=None, q_dtype=None):
+    """New tokens into the cache; returns the queries that attend to it.
+
+    q [tokens, q_heads, d], k and v [tokens, heads, d] (one dtype, any token and head strides):
+        q' = rot(norm(q)) returned as q_dtype (q's if None); rot(norm(k)) and v into the token's slot
+    norm: x * rsqrt(mean(x^2) + eps) * w per head, with float32 q_norm and k_norm [d] (both or neither)
+    rot:  pairs (x_i, x_{i + r/2}), i < r/2, turned by float32 cos and sin [positions, r/2] at the token's
+          position (both or neither; dims from r on stay; a position outside the table gives NaN)
+    lens counts these tokens already: the i-th of a row's n goes to slot lens[b] - n + i.
+    starts: int32 [rows + 1], tokens starts[b] .. starts[b+1]-1 are row b's; None: one token for each row.
+    positions: int32 [tokens]; None: the slots (as long as nothing has been evicted).
+    scores, pos: the new tokens' entries are set to 0 and to their positions.
+    A token of no row, or whose slot the table does not hold (padding), is not stored and its q' is 0."""
+    refuse_grad(q, k, v, q_norm, k_norm)
+    c = _cache(k_pages, v_pages, scores, pos, table, lens, None)
+    dev, d = k_pages.device, c.head_dim
+    if q.dim() != 3 or q.shape[2] != d:
+        raise ValueError(f"q must be [tokens, q_heads, {d}]")
+    tokens, hq = q.shape[0], q.shape[1]
+    if k.shape != (tokens, c.heads, d) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [{tokens}, {c.heads}, {d}]")
+    if k.dtype != q.dtype or v.dtype != q.dtype or q.device != dev or k.device != dev or v.device != dev:
+        raise ValueError(f"q, k and v must share a dtype on {dev}")
+    xdt = _dtype("q", q.dtype)
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    if (q_norm is None) != (k_norm is None) or (cos is None) != (sin is None):
+        raise ValueError("q_norm and k_norm, and cos and sin, go together")
+    qw = kw = cp = sp = None
+    rot = n_pos = 0
+    if q_norm is not None:
+        for w in (q_norm, k_norm):
+            if w.dtype != torch.float32 or w.shape != (d,) or w.device != dev or not w.is_contiguous():
+                raise ValueError(f"q_norm and k_norm must be contiguous float32 [{d}] tensors on {dev}")
+        qw, kw = q_norm.data_ptr(), k_norm.data_ptr()
+    if cos is not None:
+        if cos.dim() != 2 or sin.shape != cos.shape:
+            raise ValueError("cos and sin must be [positions, rotary dims / 2]")
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"cos and sin must be contiguous float32 tensors on {dev}")
+        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
+        cp, sp = cos.data_ptr(), sin.data_ptr()
+    s_ptr = _ints("starts", starts, (c.rows + 1,), dev)
+    p_ptr = _ints("positions", positions, (tokens,), dev)
+    odt = q.dtype if q_dtype is None else q_dtype
+    out = torch.empty((tokens, hq, d), dtype=odt, device=dev)
+    st = _capi.load().trellis_kv_append(
+        c, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+        v.stride(1), xdt, tokens, hq, s_ptr, p_ptr, qw, kw, eps, cp, sp, rot, n_pos, out.data_ptr(),
+        _dtype("q'", odt), _stream(dev))
+    if st:
+        _capi.check(st)
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = None, max_len: int | None = None,
+                    scores=None, out=None, out_dtype=None, workspace=None):
+    """Attention of one new token per row over the cache: q [rows, q_heads, d] (any row and head strides),
+    query head i over key-value head i // (q_heads // heads); softmax(scale * q.k) v over the row's
+    tokens, scale d**-0.5 if None. A row without tokens gives zeros. Returns [rows, q_heads, d] of
+    out_dtype (q's if None), or fills a contiguous `out`.
+
+    max_len: the longest row the call has to expect; it plans the split over the length, and tokens past
+        it are not seen. None: all that the table can hold. Give the batch's own bound where one is known.
+    scores: each token's entry grows by the sum of its weights over the query heads of its head.
+    workspace: scratch for callers that keep it (a contiguous tensor of attention_workspace_bytes); None:
+        allocated for the call."""
+    refuse_grad(q)
+    c = _cache(k_pages, v_pages, scores, None, table, lens, max_len)
+    dev, d = k_pages.device, c.head_dim
+    if q.dim() != 3 or q.shape[0] != c.rows or q.shape[2] != d or q.device != dev:
+        raise ValueError(f"q must be [{c.rows}, q_heads, {d}] on {dev}")
+    qdt = _dtype("q", q.dtype)
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    hq = q.shape[1]
+    if out is None:
+        out = torch.empty((c.rows, hq, d), dtype=q.dtype if out_dtype is None else out_dtype, device=dev)
+    elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous {list(q.shape)} tensor on {dev}")
+    lib, need = _capi.load(), ctypes.c_size_t(0)
+    acc = 0 if scores is None else 1
+    st = lib.trellis_attention_workspace_bytes(c, hq, acc, need)
+    if st:
+        _capi.check(st)
+    ws, ws_ptr, ws_bytes = _workspace(workspace, need.value, dev)
+    st = lib.trellis_paged_attention(c, q.data_ptr(), q.stride(0), q.stride(1), qdt, hq,
+                                     d ** -0.5 if scale is None else scale, acc, out.data_ptr(),
+                                     _dtype("out", out.dtype), ws_ptr, ws_bytes, _stream(dev))
+    if st:
+        _capi.check(st)
+    return out
+
+
+def evict_kv(k_pages, v_pages, scores, pos, table, lens, keep: int, recent: int, *, next_pos=None, out_table=None,
+             max_len: int | None = None, workspace=None):
+    """Evict by accumulated attention weight: of each row's tokens, per key-value head, `keep` stay: those of
+    the last `recent` positions (pos >= next_pos[b] - recent), then those of the largest scores, equal
+    scores by the lowest slot. A kept token below slot `keep` stays in its slot; the freed slots below take
+    the kept tokens from above, both in ascending order. Key, value, score and position move together.
+
+    next_pos: int32 [rows], positions each row has seen; None: its length (nothing evicted before).
+    out_table: int32 [rows, width]: the kept tokens are copied to these pages instead (none of them in
+        `table`), whose own stay as they are; None: in place, where no page may be in two rows' tables.
+    Returns the new lengths min(lens, keep) as a new tensor; `lens` itself stays, for a model's other
+    layers. Rows of up to `keep` tokens stay as they are."""
+    c = _cache(k_pages, v_pages, scores, pos, table, lens, max_len)
+    if scores is None or pos is None:
+        raise ValueError("eviction goes by scores and pos")
+    dev = k_pages.device
+    n_ptr = _ints("next_pos", next_pos, (c.rows,), dev)
+    o_ptr, o_stride, o_width = None, 0, 0
+    if out_table is not None:
+        if out_table.dtype != torch.int32 or out_table.dim() != 2 or out_table.shape[0] != c.rows or \
+                (out_table.stride(1) != 1 and out_table.shape[1] != 1) or out_table.device != dev:
+            raise ValueError(f"out_table must be int32 [{c.rows}, width] with unit column stride on {dev}")
+        o_ptr, o_stride, o_width = out_table.data_ptr(), out_table.stride(0), out_table.shape[1]
+    lib, need = _capi.load(), ctypes.c_size_t(0)
+    st = lib.trellis_evict_workspace_bytes(c, keep, need)
+    if st:
+        _capi.check(st)
+    new_lens = torch.empty_like(lens)
+    ws, ws_ptr, ws_bytes = _workspace(workspace, need.value, dev)
+    st = lib.trellis_kv_evict(c, keep, recent, n_ptr, o_ptr, o_stride, o_width, new_lens.data_ptr(), ws_ptr, ws_bytes,
+                              _stream(dev))
+    if st:
+        _capi.check(st)
+    return new_lens
+
+
+class PagedKVCache:
+    """The key-value cache of a model's layers for up to `rows` sequences of up to `max_len` cached tokens,
+    in pages that the rows take from one pool as they grow.
+
+    A step calls grow() once, then append() and attend() for each layer; evict() once after a step keeps
+    the rows within a budget. The page tables, lengths and positions are shared by the layers. Calls are
+    ordered on the current stream; use the cache on one stream at a time."""
+
+    def __init__(self, layers: int, heads: int, head_dim: int, *, rows: int, max_len: int, pages: int | None = None,
+                 page_size: int = 64, dtype: torch.dtype = torch.float16, device="cuda", evictable: bool = False):
+        width = -(-max_len // page_size)
+        pages = rows * width if pages is None else pages
+        if min(layers, heads, rows, max_len, pages) < 1:
+            raise ValueError("layers, heads, rows, max_len and pages must be positive")
+        shape = (pages, heads, page_size, head_dim)
+        self.page_size, self.max_len, self.device = page_size, max_len, torch.device(device)
+        # idle slots are never read as values: no fill
+        self.k = [torch.empty(shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.v = [torch.empty(shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.scores = [torch.zeros(shape[:3], dtype=torch.float32, device=device) if evictable else None for _ in range(layers)]
+        self.pos = [torch.zeros(shape[:3], dtype=torch.int32, device=device) if evictable else None for _ in range(layers)]
+        self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.next_pos = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.lengths, self.seen = [0] * rows, [0] * rows     # the host's copies of lens and next_pos
+        self._free = list(range(pages - 1, -1, -1))
+        self._owned: list[list[int]] = [[] for _ in range(rows)]
+        self._starts = self._positions = None
+
+    def _upload(self, dst: torch.Tensor, values) -> None:
+        dst.copy_(torch.tensor(values, dtype=torch.int32))
+
+    def _upload_table(self) -> None:
+        width = self.table.shape[1]
+        self._upload(self.table, [own + [-1] * (width - len(own)) for own in self._owned])
+
+    def grow(self, counts) -> None:
+        """Room for counts[b] new tokens in each row b (an int: in every row); the next append() calls fill it.
+        Raises ValueError, and changes nothing, where a row would pass max_len or the pool has too few pages."""
+        rows = len(self.lengths)
+        counts = [counts] * rows if isinstance(counts, int) else list(counts)
+        if len(counts) != rows or min(counts) < 0:
+            raise ValueError(f"counts must be {rows} numbers >= 0")
+        lengths = [n + c for n, c in zip(self.lengths, counts)]
+        if max(lengths) > self.max_len:
+            raise ValueError(f"a row of {max(lengths)} tokens passes max_len={self.max_len}")
+        need = [-(-n // self.page_size) - len(own) for n, own in zip(lengths, self._owned)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"{sum(need)} pages needed, {len(self._free)} free")
+        for own, k in zip(self._owned, need):
+            own.extend(self._free.pop() for _ in range(k))
+        if any(need):
+            self._upload_table()
+        self.lengths = lengths
+        self.seen = [p + c for p, c in zip(self.seen, counts)]
+        self._upload(self.lens, self.lengths)
+        self._upload(self.next_pos, self.seen)
+        if all(c == 1 for c in counts):
+            self._starts, self._positions = None, self.next_pos - 1
+        else:
+            starts = [0]
+            for c in counts:
+                starts.append(starts[-1] + c)
+            where = [i for p, c in zip(self.seen, counts) for i in range(p - c, p)]
+            self._starts = torch.tensor(starts, dtype=torch.int32).to(self.device)
+            self._positions = torch.tensor(where, dtype=torch.int32).to(self.device)
+
+    def append(self, layer: int, q, k, v, **rotary):
+        """append_kv of the tokens that grow() made room for (row by row), at their positions in the sequences."""
+        if self._positions is None:
+            raise ValueError("grow() first")
+        return append_kv(q, k, v, self.k[layer], self.v[layer], self.table, self.lens, starts=self._starts,
+                         positions=self._positions, scores=self.scores[layer], pos=self.pos[layer], **rotary)
+
+    def attend(self, layer: int, q, *, scale: float | None = None, out_dtype=None):
+        """paged_attention of one query token per row (a row without tokens gives zeros)."""
+        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, scale=scale,
+                               max_len=max(self.lengths), scores=self.scores[layer], out_dtype=out_dtype)
+
+    def evict(self, keep: int, recent: int) -> None:
+        """evict_kv of every layer, in place; the pages that the rows no longer fill go back to the pool."""
+        if self.scores[0] is None:
+            raise ValueError("the cache was not made evictable")
+        new_lens = None
+        for k, v, scores, pos in zip(self.k, self.v, self.scores, self.pos):
+            new_lens = evict_kv(k, v, scores, pos, self.table, self.lens, keep, recent, next_pos=self.next_pos,
+                                max_len=max(self.lengths))
+        self.lens.copy_(new_lens)
+        self._set_lengths([min(n, keep) for n in self.lengths])
+
+    def release(self, row: int) -> None:
+        """The row's sequence has ended: its pages go back to the pool, the row is empty."""
+        self.seen[row] = 0
+        self._upload(self.next_pos, self.seen)
+        self._set_lengths([0 if b == row else n for b, n in enumerate(self.lengths)])
+        self._upload(self.lens, self.lengths)
+
+    def _set_lengths(self, lengths) -> None:
+        self._starts = self._positions = None
+        self.lengths, freed = lengths, False
+        for own, n in zip(self._owned, lengths):
+            while len(own) > -(-n // self.page_size):
+                self._free.append(own.pop())
+                freed = True
+        if freed:
+            self._upload_table()
