@@ -27,92 +27,97 @@ struct AppendArgs {
   Cache c;
 };
 
-// LPR lanes (a power of 2, 8 dims each) per (token, head) row; heads in the order q, k, v.
-// VEC: every row of q, k and v is 16-byte aligned.
+// A workgroup takes one token and `rounds` times 256 / lpr of its heads (q, k, v in that order), lpr lanes (a
+// power of 2) a head, so the token's row, slot, page and angles are found once. A lane holds 8 dims of its
+// head: the rotary dims as 4 of the first half and their 4 partners of the second (nothing to exchange), the
+// others 8 in a row. VEC: every row of q, k and v is 16-byte aligned.
+// Bound: APPEND_FIGURES.
 template <class TX, class TC, bool VEC>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int lpr) {
-  const int lane = threadIdx.x & 63, sub = threadIdx.x & (lpr - 1);
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int lpr, int rounds, int parts) {
+  const int lane = threadIdx.x & 63, sub = threadIdx.x & (lpr - 1), group = threadIdx.x / lpr, groups = 256 / lpr;
   const int heads = a.hq + 2 * a.c.heads, d = a.c.d;
-  const long long item = static_cast<long long>(blockIdx.x) * (256 / lpr) + threadIdx.x / lpr;
-  // rows past the last go through the lane exchanges with the others
-  const bool in = item < static_cast<long long>(a.tokens) * heads;
-  const int t = in ? static_cast<int>(item / heads) : 0, hh = in ? static_cast<int>(item - static_cast<long long>(t) * heads) : 0;
-  const int kind = hh < a.hq ? 0 : hh < a.hq + a.c.heads ? 1 : 2;   // q, k, v
-  const int head = kind == 0 ? hh : kind == 1 ? hh - a.hq : hh - a.hq - a.c.heads;
+  const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;
 
   // the token's row b and slot: lens counts the call's tokens already
-  int b = t, slot;
-  bool live = in;
+  int b = t, slot = -1;
+  bool live = true;
   if (a.starts) {
-    int lo = 0, hi = a.c.rows;   // the last row whose first token is at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.starts[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-    const int first = a.starts[b], end = a.starts[b + 1];
-    live = live && t >= first && t < end;
-    slot = a.c.lens[b] - (end - t);
+    // the row is the number of rows that end at or before t
+    b = 0;
+    for (int i = 0; i < a.c.rows; i += 64) b += __popcll(__ballot(i + lane < a.c.rows && a.starts[i + lane + 1] <= t));
+    live = b < a.c.rows && a.starts[0] <= t;
+    if (live) slot = a.c.lens[b] - (a.starts[b + 1] - t);
   } else {
     slot = a.c.lens[b] - 1;
   }
   live = live && slot >= 0 && slot < (static_cast<long long>(a.c.width) << a.c.page_shift);
   const int page = live ? a.c.page_of(b, slot) : -1;
   live = live && page >= 0;
+  const int position = a.positions ? a.positions[t] : slot;
 
-  const bool own = in && sub * 8 < d;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const TX* src = kind == 0 ? static_cast<const TX*>(a.q) + t * a.q_t + head * a.q_h
-                  : kind == 1 ? static_cast<const TX*>(a.k) + t * a.k_t + head * a.k_h
-                              : static_cast<const TX*>(a.v) + t * a.v_t + head * a.v_h;
-  if (own) load8<TX, VEC>(src + sub * 8, x);
-  const float* w = kind == 0 ? a.q_w : a.k_w;
-  const bool normed = kind != 2 && w;
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-  ss = group_sum(ss, lpr, lane);
-  if (normed && own) {
-    const float f = 1.0f / __builtin_sqrtf(ss * (1.0f / static_cast<float>(d)) + a.eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * f * w[sub * 8 + i];
-  }
-  const int position = a.positions ? (in ? a.positions[t] : 0) : slot;
-  if (a.cos) {
-    // the partner dims sit rot / 16 lanes up (first half) or down (second half)
-    const int hl = a.rot / 16;
-    const bool first = sub < hl, turn = sub < 2 * hl && kind != 2;
-    const int from = (lane & ~(lpr - 1)) + (first ? sub + hl : turn ? sub - hl : sub);
-    const int i0 = (first ? sub : sub - hl) * 8;
-    const bool known = position >= 0 && position < a.n_positions;
-    const long long row = static_cast<long long>(known ? position : 0) * (a.rot / 2) + i0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl(x[i], from);
-      if (turn && own) {
-        // a position that the table does not hold has no angle: NaN
-        const float c = known ? a.cos[row + i] : __builtin_nanf(""), s = known ? a.sin[row + i] : __builtin_nanf("");
-        x[i] = first ? x[i] * c - other * s : x[i] * c + other * s;
-      }
+  // the lane's dims: d0 .. d0 + 3 and d1 .. d1 + 3
+  const int turned = a.cos ? a.rot / 8 : 0;
+  const bool turn = sub < turned, own = sub * 8 < d;
+  const int d0 = turn ? 4 * sub : 8 * sub, d1 = turn ? a.rot / 2 + 4 * sub : 8 * sub + 4;
+  float4_t c = float4_t{1.f, 1.f, 1.f, 1.f}, s = float4_t{0.f, 0.f, 0.f, 0.f};
+  if (turn) {
+    if (position >= 0 && position < a.n_positions) {
+      const long long at = static_cast<long long>(position) * (a.rot / 2) + d0;
+      c = *reinterpret_cast<const float4_t*>(a.cos + at);
+      s = *reinterpret_cast<const float4_t*>(a.sin + at);
+    } else {
+      // a position that the table does not hold has no angle
+      const float nan = __builtin_nanf("");
+      c = s = float4_t{nan, nan, nan, nan};
     }
   }
-  if (!own) return;
-  if (kind == 0) {
-    // a token without a slot (padding) gets zeros
-    if (!live)
+  for (int r = 0; r < rounds; ++r) {
+    const int hh = (part * rounds + r) * groups + group;
+    const bool in = hh < heads;
+    const int kind = hh < a.hq ? 0 : hh < a.hq + a.c.heads ? 1 : 2;   // q, k, v
+    const int head = kind == 0 ? hh : kind == 1 ? hh - a.hq : hh - a.hq - a.c.heads;
+    float4_t x = float4_t{0.f, 0.f, 0.f, 0.f}, y = x;
+    if (in && own) {
+      const TX* src = kind == 0 ? static_cast<const TX*>(a.q) + t * a.q_t + head * a.q_h
+                      : kind == 1 ? static_cast<const TX*>(a.k) + t * a.k_t + head * a.k_h
+                                  : static_cast<const TX*>(a.v) + t * a.v_t + head * a.v_h;
+      x = load4<TX, VEC>(src + d0);
+      y = load4<TX, VEC>(src + d1);
+    }
+    const float* w = kind == 0 ? a.q_w : a.k_w;
+    if (w) {
+      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    store8_dt<true>(a.q_out, (static_cast<long long>(t) * a.hq + head) * d + sub * 8, a.q_dt, x);
-    return;
-  }
-  if (!live) return;
-  TC* dst = static_cast<TC*>(kind == 1 ? a.c.k : a.c.v) + a.c.row_at(page, head, slot) + sub * 8;
-  store8<TC, true>(dst, x);
-  if (kind == 1 && sub == 0) {
-    const long long p = a.c.slot_at(page, head, slot);
-    if (a.c.scores) a.c.scores[p] = 0.f;
-    if (a.c.pos) a.c.pos[p] = position;
+      for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(x[i], x[i], __builtin_fmaf(y[i], y[i], ss));
+      ss = group_sum(ss, lpr, lane);
+      if (kind != 2 && own) {
+        const float f = 1.0f / __builtin_sqrtf(ss * (1.0f / static_cast<float>(d)) + a.eps);
+        x = x * f * *reinterpret_cast<const float4_t*>(w + d0);
+        y = y * f * *reinterpret_cast<const float4_t*>(w + d1);
+      }
+    }
+    if (turn && kind != 2) {
+      const float4_t u = x * c - y * s;
+      y = y * c + x * s;
+      x = u;
+    }
+    if (!in || !own) continue;
+    if (kind == 0) {
+      // a token without a slot (padding) gets zeros
+      if (!live) x = y = float4_t{0.f, 0.f, 0.f, 0.f};
+      const long long at = (static_cast<long long>(t) * a.hq + head) * d;
+      store4_dt(a.q_out, at + d0, a.q_dt, x);
+      store4_dt(a.q_out, at + d1, a.q_dt, y);
+    } else if (live) {
+      TC* dst = static_cast<TC*>(kind == 1 ? a.c.k : a.c.v) + a.c.row_at(page, head, slot);
+      store4(dst + d0, x);
+      store4(dst + d1, y);
+      if (kind == 1 && sub == 0) {
+        const long long p = a.c.slot_at(page, head, slot);
+        if (a.c.scores) a.c.scores[p] = 0.f;
+        if (a.c.pos) a.c.pos[p] = position;
+      }
+    }
   }
 }
 

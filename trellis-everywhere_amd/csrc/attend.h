@@ -32,6 +32,7 @@ namespace trellis {
 constexpr int ATT_WAVES = 4;
 constexpr int ATT_TILE = 32;                          // tokens per tile
 constexpr int ATT_CHUNK_MIN = ATT_TILE * ATT_WAVES;   // the shortest chunk: a tile per wave
+constexpr int ATT_SPLITS = 1024;                      // the most chunks of a row
 constexpr float ATT_LOW = -3.0e38f;                   // below every logit that counts
 constexpr float ATT_TOP = 11.f;                       // log2 of the weight at the maximum when it is set
 constexpr float ATT_SLACK = 4.f;                      // how far (log2) a logit may pass it
@@ -352,23 +353,57 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 }
 
 // The chunks of one (row, query head) joined: out = sum_c f_c part_c / sum_c f_c sum_c, f_c = 2^(m_c - max).
+// A workgroup's threads take the chunks' maxima and sums side by side, then the partial sums as (chunk group,
+// 4 dims), so that all of a round's loads are in flight together; one thread per dim that walked the chunks
+// one after another took 48 us for 64 chunks of 32 heads, this takes 4.
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-  const int tid = threadIdx.x;
+  __shared__ float s_f[ATT_SPLITS], s_red[2][4];
+  __shared__ float4_t s_acc[256];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const long long bh = blockIdx.x;
   const int b = static_cast<int>(bh / a.hq), d = a.c.d;
   const int n = a.c.length(b), chunk = att_chunk(n, a.splits);
   const int used = max((n + chunk - 1) / chunk, 1);
-  const float* ml = a.ml + 2 * bh * a.splits;
-  float mx = ATT_LOW;
-  for (int c = 0; c < used; ++c) mx = fmaxf(mx, ml[2 * c]);
+  const float2* ml = reinterpret_cast<const float2*>(a.ml) + bh * a.splits;
+  float m[ATT_SPLITS / 256], l[ATT_SPLITS / 256], mx = ATT_LOW;
+#pragma unroll
+  for (int i = 0; i < ATT_SPLITS / 256; ++i) {
+    const int c = tid + 256 * i;
+    const float2 v = c < used ? ml[c] : make_float2(ATT_LOW, 0.f);
+    m[i] = v.x;
+    l[i] = v.y;
+    mx = fmaxf(mx, v.x);
+  }
+  mx = wave_max(mx, lane);
+  if (lane == 0) s_red[0][wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
   float sum = 0.f;
-  for (int c = 0; c < used; ++c) sum = __builtin_fmaf(ml[2 * c + 1], exp2f(ml[2 * c] - mx), sum);
+#pragma unroll
+  for (int i = 0; i < ATT_SPLITS / 256; ++i) {
+    const float f = exp2f(m[i] - mx);
+    if (tid + 256 * i < used) s_f[tid + 256 * i] = f;
+    sum = __builtin_fmaf(l[i], f, sum);
+  }
+  sum = wave_sum(sum, lane);
+  if (lane == 0) s_red[1][wave] = sum;
+  __syncthreads();
+  sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // no token (or none on a page that exists)
-  for (int dim = tid; dim < d; dim += 256) {
-    float acc = 0.f;
-    for (int c = 0; c < used; ++c)
-      acc = __builtin_fmaf(a.part[(bh * a.splits + c) * d + dim], exp2f(ml[2 * c] - mx), acc);
-    store_dt(a.out, bh * d + dim, a.out_dt, acc * inv);
+  const int quads = d / 4, groups = 256 / quads;
+  const int grp = tid / quads, dim = (tid - grp * quads) * 4;
+  float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
+  if (grp < groups) {
+#pragma unroll 8
+    for (int c = grp; c < used; c += groups)
+      acc += *reinterpret_cast<const float4_t*>(a.part + (bh * a.splits + c) * d + dim) * s_f[c];
+  }
+  s_acc[tid] = acc;
+  __syncthreads();
+  if (grp == 0) {
+    for (int i = 1; i < groups; ++i) acc += s_acc[i * quads + tid];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_dt(a.out, bh * d + dim + i, a.out_dt, acc[i] * inv);
   }
   if (a.total && tid == 0) {
     a.total[2 * bh] = mx;

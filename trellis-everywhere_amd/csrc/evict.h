@@ -7,17 +7,18 @@
 //         the moves of one head have no order among them.
 // In place only the moves are made; with an out table every kept token goes to its slot there.
 //
-// evict_select_kernel, one workgroup per (row, head): the keep-th largest key by 8-bit digits of the keys'
-// range (LDS histograms), then one pass in slot order that ranks holes and sources by ballots.
-// evict_move_kernel copies.
+// evict_select_kernel, one workgroup per (row, head): the keep-th largest key by 11-bit digits of the keys'
+// range (LDS histograms), then one scan in slot order that gives holes and sources their ranks: with c(j) the
+// kept tokens below slot j, a hole is the (j - c(j))-th, a source the (c(j) - c(keep))-th.
+// evict_move_kernel copies; a call whose rows can move EV_FUSED tokens at most copies in the first kernel.
+// Bound: the first kernel by its chain of dependent steps (page, position and score loads, three digits of
+// four barriers, the scan): EVICT_FIGURES.
 #pragma once
 
 #include "serve.h"
 
 namespace trellis {
 
-constexpr int EV_THREADS = 1024;
-constexpr int EV_WAVES = EV_THREADS / 64;
 constexpr uint32_t EV_RECENT = 0xFFFFFFFFu;   // key of a token kept for its position
 
 struct EvictArgs {
@@ -42,96 +43,264 @@ __device__ __forceinline__ uint32_t ev_key(float score) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ uint32_t ev_token_key(const EvictArgs& a, int b, int head, int j, int from) {
-  const int page = a.c.page_of(b, j);
-  if (page < 0) return 0;
-  const long long p = a.c.slot_at(page, head, j);
-  return a.c.pos[p] >= from ? EV_RECENT : ev_key(a.c.scores[p]);
+// Inclusive sum over the wave's lanes up to this one (DPP row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
+  return v;
 }
 
-// Exclusive rank of `flag` over the workgroup in thread order, and the total.
-__device__ __forceinline__ int block_rank(bool flag, int* totals, int& total) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const unsigned long long vote = __ballot(flag);
-  if (lane == 0) totals[wave] = __popcll(vote);
-  __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < EV_WAVES; ++w) {
-    const int t = totals[w];
-    before += w < wave ? t : 0;
-    total += t;
+__device__ __forceinline__ void ev_move(const EvictArgs& a, int b, int head, int from, int from_page, int to, int to_page,
+                                        int sub) {
+  if (from_page < 0 || to_page < 0) return;
+  const long long s = a.c.row_at(from_page, head, from), t = a.c.row_at(to_page, head, to);
+  if (sub * 8 < a.c.d) {
+    const u32x4_t k = *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.c.k) + 2 * s + 16 * sub);
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.c.v) + 2 * s + 16 * sub);
+    *reinterpret_cast<u32x4_t*>(static_cast<char*>(a.c.k) + 2 * t + 16 * sub) = k;
+    *reinterpret_cast<u32x4_t*>(static_cast<char*>(a.c.v) + 2 * t + 16 * sub) = v;
   }
-  __syncthreads();
-  return before + __popcll(vote & ((1ull << lane) - 1));
+  if (sub == 0) {
+    const long long p = a.c.slot_at(from_page, head, from), q = a.c.slot_at(to_page, head, to);
+    a.c.scores[q] = a.c.scores[p];
+    a.c.pos[q] = a.c.pos[p];
+  }
 }
 
-__global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[256], totals[EV_WAVES], s_digit, s_left;
-  const int tid = threadIdx.x;
+constexpr int EV_BINS = 2048;
+constexpr int EV_FUSED = 64;    // most moves of a row and head that the select kernel makes itself
+
+// A thread's keys stay in registers: G groups of 4 consecutive tokens (a page id, 16 bytes of positions and of
+// scores each), group i of a thread at token segment + 4 (i * THREADS + tid). Rows longer than a segment of
+// 4 G THREADS tokens go through in segments, read again for each step.
+template <int THREADS, int G, bool FUSED>
+__global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int lpr) {
+  constexpr int WAVES = THREADS / 64, SEG = 4 * G * THREADS;
+  constexpr int BPT = EV_BINS / THREADS;
+  __shared__ int hist[2][EV_BINS], totals[WAVES], counts[2][G * WAVES];
+  __shared__ int s_digit, s_left, s_equals, s_first[EV_FUSED], s_second[EV_FUSED];
+  __shared__ uint32_t s_lo[WAVES], s_hi[WAVES];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int head = blockIdx.x % a.c.heads, b = blockIdx.x / a.c.heads;
-  const int n = a.c.length(b);
+  const int n = a.c.length(b), keep = a.keep;
   const long long bh = blockIdx.x;
-  if (tid == 0 && head == 0) a.new_lens[b] = min(n, a.keep);
-  int32_t* first = a.first + bh * a.keep;
-  int32_t* second = a.second + bh * a.keep;
-  if (n <= a.keep) {
+  if (tid == 0 && head == 0) a.new_lens[b] = min(n, keep);
+  int32_t* first = a.first + bh * keep;
+  int32_t* second = a.second + bh * keep;
+  if (n <= keep) {
     // everything stays: nothing moves in place, all slots are copied to an out table
-    if (a.out_table)
-      for (int j = tid; j < n; j += EV_THREADS) first[j] = j;
-    if (tid == 0) a.count[bh] = a.out_table ? n : 0;
+    if constexpr (!FUSED) {
+      if (a.out_table)
+        for (int j = tid; j < n; j += THREADS) first[j] = j;
+      if (tid == 0) a.count[bh] = a.out_table ? n : 0;
+    }
     return;
   }
-  const int next = a.next_pos ? a.next_pos[b] : n;
-  const int from = next - a.recent;
+  const int from = (a.next_pos ? a.next_pos[b] : n) - a.recent;
+  const int segs = (n + SEG - 1) / SEG;
 
-  // ---- the key of the keep-th largest, digit by digit, and how many of its equals are kept
+  // the segment's keys: loads without branches (of the row's last group past its end, of page 0 for a missing
+  // page), so that a step's are all in flight together
+  uint32_t key[G][4];
+  const auto token = [&](int seg, int i) { return seg * SEG + 4 * (i * THREADS + tid); };
+  const auto load = [&](int seg) {
+    int page[G];
+    u32x4_t at[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) page[i] = a.c.page_of(b, min(token(seg, i), (n - 1) & ~3));
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const long long p = a.c.slot_at(max(page[i], 0), head, min(token(seg, i), (n - 1) & ~3));
+      at[i] = *reinterpret_cast<const u32x4_t*>(a.c.pos + p);
+      const u32x4_t s = *reinterpret_cast<const u32x4_t*>(a.c.scores + p);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) key[i][q] = s[q];
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        key[i][q] = page[i] < 0 ? 0u : static_cast<int>(at[i][q]) >= from ? EV_RECENT : ev_key(__builtin_bit_cast(float, key[i][q]));
+  };
+  // f(number among the thread's keys, token, key) for every token of the segment
+  const auto each = [&](int seg, auto f) {
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (token(seg, i) + q < n) f(4 * i + q, token(seg, i) + q, key[i][q]);
+  };
+
+  // ---- the keys' range
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
+  for (int seg = 0; seg < segs; ++seg) {
+    load(seg);
+    each(seg, [&](int, int, uint32_t k) {
+      lo = min(lo, k);
+      hi = max(hi, k);
+    });
+  }
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) {
+    lo = min(lo, static_cast<uint32_t>(__shfl_xor(static_cast<int>(lo), h)));
+    hi = max(hi, static_cast<uint32_t>(__shfl_xor(static_cast<int>(hi), h)));
+  }
+  if (lane == 0) {
+    s_lo[wave] = lo;
+    s_hi[wave] = hi;
+  }
+  for (int i = tid; i < EV_BINS; i += THREADS) hist[0][i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    lo = min(lo, s_lo[w]);
+    hi = max(hi, s_hi[w]);
+  }
+
+  // ---- the keep-th largest key less lo, digit by digit; `left` of the tokens equal to it are kept
   uint32_t prefix = 0;
-  int left = a.keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += EV_THREADS) {
-      const uint32_t key = ev_token_key(a, b, head, j, from);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+  int left = keep, equals = n, bits = hi > lo ? 32 - __builtin_clz(hi - lo) : 0;
+  for (int now = 0; bits > 0 && left < equals; now ^= 1) {
+    const int shift = max(bits - 11, 0);
+    for (int seg = 0; seg < segs; ++seg) {
+      if (segs > 1) load(seg);
+      each(seg, [&](int, int, uint32_t k) {
+        const uint32_t u = k - lo;
+        if (bits >= 32 || (u >> bits) == (prefix >> bits)) {
+          const int bin = (u >> shift) & ((1u << (bits - shift)) - 1);
+          atomicAdd(&hist[now][bin], 1);
+        }
+      });
     }
     __syncthreads();
-    if (tid == 0) {
-      int digit = 255, rest = left;
-      while (digit > 0 && hist[digit] < rest) rest -= hist[digit--];
-      s_digit = digit;
-      s_left = rest;
+    // a thread's bins from the top: the one in which the count from above reaches `left`
+    int h[BPT], sum = 0;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) {
+      h[i] = hist[now][EV_BINS - 1 - BPT * tid - i];
+      sum += h[i];
+      hist[now ^ 1][BPT * tid + i] = 0;
+    }
+    const int scan = wave_scan(sum);
+    if (lane == 63) totals[wave] = scan;
+    __syncthreads();
+    int before = scan - sum;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) before += w < wave ? totals[w] : 0;
+    if (before < left && before + sum >= left) {
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        if (before < left && before + h[i] >= left) {
+          s_digit = EV_BINS - 1 - BPT * tid - i;
+          s_left = left - before;
+          s_equals = h[i];
+        }
+        before += h[i];
+      }
     }
     __syncthreads();
     prefix |= static_cast<uint32_t>(s_digit) << shift;
     left = s_left;
-    __syncthreads();
+    equals = s_equals;
+    bits = shift;
   }
+  // kept: u >> bits above prefix >> bits, and of those equal there the first `left`
 
-  // ---- in slot order: what is kept, the holes below `keep`, the sources above
-  int equals = 0, holes = 0, sources = 0;
-  for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
-    const int j = j0 + tid;
-    const uint32_t key = j < n ? ev_token_key(a, b, head, j, from) : 0;
-    int total;
-    const bool equal = j < n && key == prefix;
-    const int er = equals + block_rank(equal, totals, total);
-    equals += total;
-    const bool kept = j < n && (key > prefix || (equal && er < left));
-    const bool hole = j < a.keep && !kept;
-    const int hr = holes + block_rank(hole, totals, total);
-    holes += total;
-    const bool source = j >= a.keep && kept;
-    const int sr = sources + block_rank(source, totals, total);
-    sources += total;
-    if (source) second[sr] = j;
-    if (a.out_table) {
-      if (j < a.keep) first[j] = kept ? j : -1 - hr;
-    } else if (hole) {
-      first[hr] = j;
+  // ---- exclusive ranks of a flag in slot order: of a group's first token. (Every wave scans the counts of all
+  // by itself; two count buffers in turn, as a wave may be a call ahead of another.)
+  int turn = 0;
+  const auto ranks = [&](uint32_t flags, int (&rank)[G], int& before) {
+    int* count = counts[turn];
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int c = __builtin_popcount((flags >> (4 * i)) & 15u);
+      const int scan = wave_scan(c);
+      rank[i] = scan - c;
+      if (lane == 63) count[i * WAVES + wave] = scan;
     }
+    __syncthreads();
+    constexpr int PER = (G * WAVES + 63) / 64;   // one count a lane, or two
+    int c[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = lane * PER + i < G * WAVES ? count[lane * PER + i] : 0;
+      sum += c[i];
+    }
+    const int run = before + wave_scan(sum) - sum;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int at = i * WAVES + wave, l = at / PER;
+      rank[i] += __builtin_amdgcn_readlane(run, l) + (PER == 2 && at % PER ? __builtin_amdgcn_readlane(c[0], l) : 0);
+    }
+    before = __builtin_amdgcn_readlane(run + sum, 63);
+  };
+  // tokens of a thread's group below the group's q-th
+  const auto lower = [](uint32_t flags, int number) {
+    return __builtin_popcount((flags >> (number & ~3)) & ((1u << (number & 3)) - 1));
+  };
+
+  int seen = 0, kept_before = 0, below = -1;   // below: c(keep)
+  for (int seg = 0; seg < segs; ++seg) {
+    if (segs > 1) load(seg);
+    uint32_t kept = 0, equal = 0;
+    each(seg, [&](int number, int, uint32_t k) {
+      const uint32_t u = bits < 32 ? (k - lo) >> bits : 0, p = bits < 32 ? prefix >> bits : 0;
+      if (u > p) kept |= 1u << number;
+      if (u == p) equal |= 1u << number;
+    });
+    int rank[G];
+    if (left < equals) {
+      // some of the equals only: the lowest slots
+      ranks(equal, rank, seen);
+      uint32_t some = 0;
+      each(seg, [&](int number, int, uint32_t) {
+        if (rank[number >> 2] + lower(equal, number) < left) some |= (equal >> number & 1u) << number;
+      });
+      equal = some;
+    }
+    kept |= equal;
+    ranks(kept, rank, kept_before);
+    if (below < 0 && keep < (seg + 1) * SEG) {
+      // (keep < n: the token of slot `keep` is in this segment)
+      each(seg, [&](int number, int j, uint32_t) {
+        if (j == keep) s_left = rank[number >> 2] + lower(kept, number);
+      });
+      __syncthreads();
+      below = s_left;
+    }
+    each(seg, [&](int number, int j, uint32_t) {
+      const bool is = (kept >> number) & 1u;
+      const int r = rank[number >> 2] + lower(kept, number);
+      if (j < keep) {
+        if constexpr (FUSED) {
+          if (!is) s_first[j - r] = j;
+        } else if (a.out_table) {
+          first[j] = is ? j : -1 - (j - r);
+        } else if (!is) {
+          first[j - r] = j;
+        }
+      } else if (is) {
+        if constexpr (FUSED) s_second[r - below] = j;
+        else second[r - below] = j;
+      }
+    });
   }
-  if (tid == 0) a.count[bh] = a.out_table ? a.keep : holes;
+  const int holes = keep - below;
+  if constexpr (FUSED) {
+    __syncthreads();
+    const int sub = tid & (lpr - 1);
+    for (int r = tid / lpr; r < holes; r += THREADS / lpr) {
+      const int src = s_second[r], dst = s_first[r];
+      ev_move(a, b, head, src, a.c.page_of(b, src), dst, a.c.page_of(b, dst), sub);
+    }
+  } else if (tid == 0) {
+    a.count[bh] = a.out_table ? keep : holes;
+  }
 }
 
 // One move per group of lpr lanes (16 bytes of k and v a lane).
@@ -155,20 +324,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, int lpr, i
       src = second[r];
       to = a.c.page_of(b, dst);
     }
-    const int page = a.c.page_of(b, src);
-    if (page < 0 || to < 0) continue;
-    const long long s = a.c.row_at(page, head, src), t = a.c.row_at(to, head, dst);
-    if (sub * 8 < a.c.d) {
-      const u32x4_t k = *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.c.k) + 2 * s + 16 * sub);
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.c.v) + 2 * s + 16 * sub);
-      *reinterpret_cast<u32x4_t*>(static_cast<char*>(a.c.k) + 2 * t + 16 * sub) = k;
-      *reinterpret_cast<u32x4_t*>(static_cast<char*>(a.c.v) + 2 * t + 16 * sub) = v;
-    }
-    if (sub == 0) {
-      const long long p = a.c.slot_at(page, head, src), q = a.c.slot_at(to, head, dst);
-      a.c.scores[q] = a.c.scores[p];
-      a.c.pos[q] = a.c.pos[p];
-    }
+    ev_move(a, b, head, src, a.c.page_of(b, src), dst, to, sub);
   }
 }
 

@@ -52,6 +52,37 @@ __device__ __forceinline__ void store8_dt(void* p, long long i0, int dt, const f
   else store8<bf16_t, VEC>(static_cast<bf16_t*>(p) + i0, v);
 }
 
+// Four elements as fp32. VEC: the address is aligned to all four of them. Stores: it always is.
+template <class T, bool VEC>
+__device__ __forceinline__ float4_t load4(const T* p) {
+  float4_t v;
+  if constexpr (VEC) {
+    typedef T vec_t __attribute__((ext_vector_type(4)));
+    const vec_t w = *reinterpret_cast<const vec_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(p[i]);
+  }
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, float4_t v) {
+  typedef T vec_t __attribute__((ext_vector_type(4)));
+  vec_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = static_cast<T>(v[i]);
+  *reinterpret_cast<vec_t*>(p) = w;
+}
+
+__device__ __forceinline__ void store4_dt(void* p, long long i0, int dt, float4_t v) {
+  if (dt == DT_F32) store4(static_cast<float*>(p) + i0, v);
+  else if (dt == DT_F16) store4(static_cast<_Float16*>(p) + i0, v);
+  else store4(static_cast<bf16_t*>(p) + i0, v);
+}
+
 __device__ __forceinline__ void store_dt(void* p, long long i, int dt, float v) {
   if (dt == DT_F32) static_cast<float*>(p)[i] = v;
   else if (dt == DT_F16) static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
@@ -67,6 +98,15 @@ __device__ __forceinline__ float wave_sum(float v, int lane) {
   v += lane_xor<16>(v, lane);
   v += lane_xor<32>(v, lane);
   return v;
+}
+
+__device__ __forceinline__ float wave_max(float v, int lane) {
+  v = fmaxf(v, lane_xor<1>(v, lane));
+  v = fmaxf(v, lane_xor<2>(v, lane));
+  v = fmaxf(v, lane_xor<4>(v, lane));
+  v = fmaxf(v, lane_xor<8>(v, lane));
+  v = fmaxf(v, lane_xor<16>(v, lane));
+  return fmaxf(v, lane_xor<32>(v, lane));
 }
 
 // The sum over aligned groups of n lanes (a power of 2 up to 64).

@@ -62,6 +62,12 @@ void launch_norm_r(const NormArgs& a, int r_dtype, bool vec, int64_t rows, hipSt
 
 // ---------------------------------------------------------------- cache
 
+// The tokens of a row that a call can see.
+int longest(const trellis_kv_cache* c) {
+  const int64_t cap = static_cast<int64_t>(c->width) * c->page_size;
+  return static_cast<int>(c->max_len < cap ? c->max_len : cap);
+}
+
 int validate_cache(const trellis_kv_cache* c) {
   if (!c || !c->k || !c->v || (c->rows != 0 && (!c->table || !c->lens))) return TRELLIS_ERR_NULL;
   if (c->dtype != TRELLIS_F16 && c->dtype != TRELLIS_BF16) return TRELLIS_ERR_DTYPE;
@@ -74,6 +80,8 @@ int validate_cache(const trellis_kv_cache* c) {
       c->page_stride < 0 || c->head_stride < 0 || c->slot_stride < c->head_dim ||
       c->slot_stride >= (int64_t(1) << 30) / c->page_size || c->table_stride < 0)
     return TRELLIS_ERR_ALIGN;
+  // token numbers, and one tile or segment past the last, stay within 32 bits
+  if (longest(c) > (1 << 30)) return TRELLIS_ERR_RANGE;
   return TRELLIS_OK;
 }
 
@@ -99,18 +107,13 @@ Cache cache_of(const trellis_kv_cache* c) {
   return r;
 }
 
-// The tokens of a row that a call can see.
-int longest(const trellis_kv_cache* c) {
-  const int64_t cap = static_cast<int64_t>(c->width) * c->page_size;
-  return static_cast<int>(c->max_len < cap ? c->max_len : cap);
-}
-
 int lanes_per_row(int d) { return 1 << log2_of((d + 7) / 8); }
 
 template <class TX, class TC>
-void launch_append(const AppendArgs& a, bool vec, int lpr, unsigned grid, hipStream_t st) {
-  if (vec) hipLaunchKernelGGL((append_kernel<TX, TC, true>), dim3(grid), dim3(256), 0, st, a, lpr);
-  else hipLaunchKernelGGL((append_kernel<TX, TC, false>), dim3(grid), dim3(256), 0, st, a, lpr);
+void launch_append(const AppendArgs& a, bool vec, int lpr, int rounds, int parts, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.tokens * parts));
+  if (vec) hipLaunchKernelGGL((append_kernel<TX, TC, true>), grid, dim3(256), 0, st, a, lpr, rounds, parts);
+  else hipLaunchKernelGGL((append_kernel<TX, TC, false>), grid, dim3(256), 0, st, a, lpr, rounds, parts);
 }
 
 // ---------------------------------------------------------------- attention
@@ -132,6 +135,7 @@ AttendPlan attend_plan(const trellis_kv_cache* c, int q_heads, bool accumulate) 
   const int64_t most = (n + ATT_CHUNK_MIN - 1) / ATT_CHUNK_MIN;
   const int64_t want = one > 0 ? (4LL * device_cus() + one - 1) / one : 1;
   p.splits = static_cast<int>(want < most ? want : most);
+  if (p.splits > ATT_SPLITS) p.splits = ATT_SPLITS;
   if (p.splits < 1) p.splits = 1;
   const size_t bh = static_cast<size_t>(c->rows) * q_heads;
   p.logit_stride = (static_cast<int64_t>(n) + 31) / 32 * 32;
@@ -177,8 +181,28 @@ int validate_evict(const trellis_kv_cache* c, int keep, int recent) {
   const int v = validate_cache(c);
   if (v) return v;
   if (!c->scores || !c->pos) return TRELLIS_ERR_NULL;
+  if (!aligned(c->scores, 16) || !aligned(c->pos, 16)) return TRELLIS_ERR_ALIGN;
   if (keep < 1 || recent < 0 || recent > keep) return TRELLIS_ERR_KEEP;
   return TRELLIS_OK;
+}
+
+template <int THREADS, int G, bool FUSED>
+void launch_evict_g(const EvictArgs& a, int lpr, unsigned grid, hipStream_t st) {
+  hipLaunchKernelGGL((evict_select_kernel<THREADS, G, FUSED>), dim3(grid), dim3(THREADS), 0, st, a, lpr);
+}
+
+// The smallest form whose registers hold the longest row (beyond 32768 tokens the last, in segments).
+template <bool FUSED>
+void launch_evict_ept(const EvictArgs& a, int n, int lpr, unsigned grid, hipStream_t st) {
+  if (n <= 2048) launch_evict_g<512, 1, FUSED>(a, lpr, grid, st);
+  else if (n <= 4096) launch_evict_g<1024, 1, FUSED>(a, lpr, grid, st);
+  else if (n <= 16384) launch_evict_g<1024, 4, FUSED>(a, lpr, grid, st);
+  else launch_evict_g<1024, 8, FUSED>(a, lpr, grid, st);
+}
+
+void launch_evict_select(const EvictArgs& a, int n, bool fused, int lpr, unsigned grid, hipStream_t st) {
+  if (fused) launch_evict_ept<true>(a, n, lpr, grid, st);
+  else launch_evict_ept<false>(a, n, lpr, grid, st);
 }
 
 struct EvictPlan {
@@ -262,7 +286,9 @@ int trellis_kv_append(const trellis_kv_cache* cache, const void* q, int64_t q_to
   if (!q || !k || !v || !q_out) return TRELLIS_ERR_NULL;
   if (cache->rows < 1) return TRELLIS_ERR_BATCH;
   const int xs = dtype_size(x_dtype);
-  if (!aligned(q, xs) || !aligned(k, xs) || !aligned(v, xs) || !aligned(q_out, 16)) return TRELLIS_ERR_ALIGN;
+  if (!aligned(q, xs) || !aligned(k, xs) || !aligned(v, xs) || !aligned(q_out, 16) ||
+      !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(cos, 16) || !aligned(sin, 16))
+    return TRELLIS_ERR_ALIGN;
   AppendArgs a;
   a.q = q;
   a.k = k;
@@ -292,21 +318,23 @@ int trellis_kv_append(const trellis_kv_cache* cache, const void* q, int64_t q_to
                    q_head_stride % per == 0 && k_token_stride % per == 0 && k_head_stride % per == 0 &&
                    v_token_stride % per == 0 && v_head_stride % per == 0;
   const int lpr = lanes_per_row(cache->head_dim);
-  const int64_t items = static_cast<int64_t>(tokens) * (q_heads + 2 * static_cast<int64_t>(cache->heads));
-  const int64_t blocks = (items + 256 / lpr - 1) / (256 / lpr);
-  if (!grid_fits(blocks, 256)) return TRELLIS_ERR_BATCH;
-  const unsigned grid = static_cast<unsigned>(blocks);
+  // a workgroup per token; while those do not fill the CUs, the token's heads over several
+  const int64_t heads = q_heads + 2 * static_cast<int64_t>(cache->heads), groups = 256 / lpr;
+  const int64_t all = (heads + groups - 1) / groups;
+  const int64_t parts = tokens * all <= 2 * device_cus() ? all : 1;
+  if (!grid_fits(tokens * parts, 256)) return TRELLIS_ERR_BATCH;
+  const int rounds = static_cast<int>((all + parts - 1) / parts);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool f16 = cache->dtype == TRELLIS_F16;
   if (x_dtype == TRELLIS_F32) {
-    if (f16) launch_append<float, _Float16>(a, vec, lpr, grid, st);
-    else launch_append<float, bf16_t>(a, vec, lpr, grid, st);
+    if (f16) launch_append<float, _Float16>(a, vec, lpr, rounds, static_cast<int>(parts), st);
+    else launch_append<float, bf16_t>(a, vec, lpr, rounds, static_cast<int>(parts), st);
   } else if (x_dtype == TRELLIS_F16) {
-    if (f16) launch_append<_Float16, _Float16>(a, vec, lpr, grid, st);
-    else launch_append<_Float16, bf16_t>(a, vec, lpr, grid, st);
+    if (f16) launch_append<_Float16, _Float16>(a, vec, lpr, rounds, static_cast<int>(parts), st);
+    else launch_append<_Float16, bf16_t>(a, vec, lpr, rounds, static_cast<int>(parts), st);
   } else {
-    if (f16) launch_append<bf16_t, _Float16>(a, vec, lpr, grid, st);
-    else launch_append<bf16_t, bf16_t>(a, vec, lpr, grid, st);
+    if (f16) launch_append<bf16_t, _Float16>(a, vec, lpr, rounds, static_cast<int>(parts), st);
+    else launch_append<bf16_t, bf16_t>(a, vec, lpr, rounds, static_cast<int>(parts), st);
   }
   return launched();
 }
@@ -407,10 +435,11 @@ int trellis_kv_evict(const trellis_kv_cache* cache, int keep, int recent, const 
   const int lpr = lanes_per_row(cache->head_dim);
   int blocks = most > 0 ? (most + 256 / lpr - 1) / (256 / lpr) : 0;
   if (blocks > 64) blocks = 64;
-  if (!grid_fits(bh, EV_THREADS) || !grid_fits(bh * blocks, 256)) return TRELLIS_ERR_BATCH;
+  if (!grid_fits(bh, 1024) || !grid_fits(bh * blocks, 256)) return TRELLIS_ERR_BATCH;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(bh)), dim3(EV_THREADS), 0, st, a);
-  if (blocks > 0)
+  const bool fused = !out_table && most <= EV_FUSED;
+  launch_evict_select(a, n, fused, lpr, static_cast<unsigned>(bh), st);
+  if (blocks > 0 && !fused)
     hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(bh * blocks)), dim3(256), 0, st, a, lpr, blocks);
   return launched();
 }
