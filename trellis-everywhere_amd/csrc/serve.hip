@@ -43,14 +43,20 @@ int device_cus() {
 
 template <class TX, class TR>
 void launch_norm(const NormArgs& a, bool vec, int64_t rows, hipStream_t st) {
-  // up to 8192 elements one chunk of 8 a thread, above four
-  const int chunks = a.width <= 8192 ? 1 : 4;
+  // the fewest chunks of 8 a thread that 1024 threads cover the row with
+  const int chunks = a.width <= 8192 ? 1 : a.width <= 16384 ? 2 : 4;
   const int threads = ((a.width + 8 * chunks - 1) / (8 * chunks) + 63) / 64 * 64;
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
-  if (vec && chunks == 1) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 1>), grid, block, 0, st, a);
-  else if (vec) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 4>), grid, block, 0, st, a);
-  else if (chunks == 1) hipLaunchKernelGGL((norm_kernel<TX, TR, false, 1>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((norm_kernel<TX, TR, false, 4>), grid, block, 0, st, a);
+  if (chunks == 1) {
+    if (vec) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 1>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((norm_kernel<TX, TR, false, 1>), grid, block, 0, st, a);
+  } else if (chunks == 2) {
+    if (vec) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 2>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((norm_kernel<TX, TR, false, 2>), grid, block, 0, st, a);
+  } else {
+    if (vec) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((norm_kernel<TX, TR, false, 4>), grid, block, 0, st, a);
+  }
 }
 
 template <class TX>
