@@ -22,18 +22,18 @@ def library():
     return _capi.load()
 
 
+# torch-dependent pieces load lazily so the format tools import without torch
+_LAZY = {"packed_linear": ("PackedLinear", "PackedGroup", "PackedOps", "load_packed", "encode_tiles"),
+         "modules": ("TrellisLinear", "TrellisGroupLinear", "swap_linears"),
+         "norms": ("rms_norm", "residual_norm"),
+         "kv_cache": ("append_kv", "paged_attention", "evict_kv", "PagedKVCache")}
+
+
 def __getattr__(name):
-    # torch-dependent pieces load lazily so the format tools import without torch
-    if name in ("PackedLinear", "PackedGroup", "PackedOps", "load_packed", "encode_tiles"):
-        from . import packed_linear
-        return getattr(packed_linear, name)
-    if name in ("TrellisLinear", "TrellisGroupLinear", "swap_linears"):
-        from . import modules
-        return getattr(modules, name)
-    if name in ("rms_norm", "residual_norm"):
-        from . import norms
-        return getattr(norms, name)
-    if name in ("append_kv", "paged_attention", "evict_kv", "PagedKVCache"):
-        from . import kv_cache
-        return getattr(kv_cache, name)
+    for module, names in _LAZY.items():
+        if name in names:
+            import importlib
+            value = getattr(importlib.import_module("." + module, __name__), name)
+            globals()[name] = value   # the next access is a plain one
+            return value
     raise AttributeError(name)

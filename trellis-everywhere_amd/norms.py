@@ -14,8 +14,9 @@ _DT = {torch.float32: _capi.DT_F32, torch.float16: _capi.DT_F16, torch.bfloat16:
 
 def refuse_grad(*tensors) -> None:
     """The operators record no gradient: a tensor that wants one is refused, not silently detached."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("forward only: call it under torch.no_grad() or detach the inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("forward only: call it under torch.no_grad() or detach the inputs")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -32,53 +33,61 @@ def _weight(name, w, width, dev):
 
 
 def _call(x, residual, weight, post_weight, gate, scale, eps, out_dtype, residual_out):
+    # (most of a small call's time is this function's: attributes are read once, and a tensor that is already
+    # [rows, width] and contiguous, as a decode loop's are, goes through without a view)
     refuse_grad(x, residual, weight, post_weight, gate)
     dev, shape, dt = x.device, x.shape, x.dtype
     if dev.type != "cuda":
         raise ValueError(f"the norms run on a GPU, not {dev}")
-    if x.dim() == 0:
+    if not shape:
         raise ValueError("x must have at least one dim")
-    width = shape[-1]
-    xdt, ydt = _DT.get(dt), _DT.get(out_dtype if out_dtype is not None else dt)
+    if out_dtype is None:
+        out_dtype = dt
+    width, xdt, ydt = shape[-1], _DT.get(dt), _DT.get(out_dtype)
     if xdt is None or ydt is None:
         raise ValueError(f"x dtype {dt} and out dtype {out_dtype} must be float32, float16 or bfloat16")
-    x2 = _rows(x)
-    rows = x2.shape[0]
+    plain = len(shape) == 2 and x.is_contiguous()
+    x2 = x if plain else _rows(x)
+    rows, ldx = x2.shape[0], width if plain else x2.stride(0)
     r_ptr = ldr = h_ptr = ldh = g_ptr = ldg = rdt = 0
     g_inner, h = 1, None
     if residual is not None:
+        rt = residual.dtype
+        rdt = _DT.get(rt)
+        if rdt is None:
+            raise ValueError(f"residual dtype {rt} not supported")
         if residual.shape != shape or residual.device != dev:
             raise ValueError(f"residual must be {tuple(shape)} on {dev}")
-        rdt = _DT.get(residual.dtype)
-        if rdt is None:
-            raise ValueError(f"residual dtype {residual.dtype} not supported")
-        r2 = _rows(residual)
+        r2 = residual if plain and residual.is_contiguous() else _rows(residual)
+        r_ptr, ldr = r2.data_ptr(), r2.stride(0)
         if residual_out is None:
-            h = torch.empty(shape, dtype=residual.dtype, device=dev)
+            h = torch.empty_like(x, dtype=rt) if plain else torch.empty(shape, dtype=rt, device=dev)
+            h_ptr, ldh = h.data_ptr(), width
         else:
             h = residual_out
-            if h.shape != shape or h.dtype != residual.dtype or h.device != dev:
+            if h.shape != shape or h.dtype != rt or h.device != dev:
                 raise ValueError("residual_out must have the residual's shape, dtype and device")
-        h2 = h if h.dim() == 2 else h.view(-1, width)
-        if h2.stride(1) != 1 and width != 1:
-            raise ValueError("residual_out must have unit column stride")
-        r_ptr, ldr, h_ptr, ldh = r2.data_ptr(), r2.stride(0), h2.data_ptr(), h2.stride(0)
+            h2 = h if len(shape) == 2 else h.view(-1, width)
+            if h2.stride(1) != 1 and width != 1:
+                raise ValueError("residual_out must have unit column stride")
+            h_ptr, ldh = h2.data_ptr(), h2.stride(0)
     if gate is not None:
         if gate.dtype != dt or gate.device != dev:
             raise ValueError(f"gate must be {dt} on {dev}")
-        g2 = gate.expand(shape)
-        if g2.dim() != 2:
-            g2 = g2.reshape(-1, width)
-        g_inner = 0 if g2.stride(1) == 0 or width == 1 else 1
-        if g_inner and g2.stride(1) != 1:
-            g2 = g2.contiguous()
-        g_ptr, ldg = g2.data_ptr(), g2.stride(0)
+        if not plain or gate.shape != shape or not gate.is_contiguous():
+            gate = gate.expand(shape)
+            if len(shape) != 2:
+                gate = gate.reshape(-1, width)
+            g_inner = 0 if gate.stride(1) == 0 or width == 1 else 1
+            if g_inner and gate.stride(1) != 1:
+                gate = gate.contiguous()
+        g_ptr, ldg = gate.data_ptr(), gate.stride(0)
     w_ptr = _weight("weight", weight, width, dev)
     p_ptr = 0 if post_weight is None else _weight("post_weight", post_weight, width, dev)
-    y = torch.empty(shape, dtype=dt if out_dtype is None else out_dtype, device=dev)
+    y = torch.empty_like(x, dtype=out_dtype) if plain else torch.empty(shape, dtype=out_dtype, device=dev)
     st = _capi.load().trellis_residual_norm(
-        x2.data_ptr(), x2.stride(0), xdt, r_ptr, ldr, rdt, g_ptr, ldg, g_inner, p_ptr, w_ptr, scale, eps,
-        h_ptr, ldh, y.data_ptr(), width, ydt, rows, width, _stream(dev))
+        x2.data_ptr(), ldx, xdt, r_ptr, ldr, rdt, g_ptr, ldg, g_inner, p_ptr, w_ptr, scale, eps, h_ptr, ldh,
+        y.data_ptr(), width, ydt, rows, width, _stream(dev))
     if st:
         _capi.check(st)
     return y, h
