@@ -22,7 +22,8 @@
 // keeping them out of its subnormals; bf16: 16 bits, three terms where q or out is fp32), the sums are fp32.
 // q of another type than the cache's is scaled by a power of 2 and split the same way.
 //
-// The chunks' results (maximum, sum, unnormalised out) meet in attend_join_kernel, in a fixed order.
+// The chunks' results (maximum, sum, unnormalised out) meet in attend_finish_kernel, in a fixed order; with scores
+// its other workgroups turn the logits that this kernel left into weights.
 #pragma once
 
 #include "serve.h"
@@ -42,21 +43,14 @@ struct AttendArgs {
   long long q_b, q_h;     // strides of q in elements
   int q_dt, q_vec;        // q_vec: q's rows are 16-byte aligned
   void* out;              // [rows][hq][d]
-  int out_dt, hq, group, row_blocks, splits;
+  int out_dt, hq, group, row_blocks, splits, chunk;
   float scale;            // times log2(e)
   float* part;            // splits > 1: [rows][kv heads][splits][hq of the kv head][d] unnormalised sums
-  float* ml;              // [rows][hq][splits][2] maximum and sum
-  float* total;           // with scores: [rows][hq][2] maximum and 1 / sum
+  float* ml;              // splits > 1 or with scores: [rows][hq][splits][2] maximum and sum
   float* logits;          // with scores: [rows][hq][logit_stride]
   long long logit_stride;
   Cache c;
 };
-
-// The chunk of a row of n tokens: at least ATT_CHUNK_MIN, so that short rows use fewer workgroups.
-__device__ __forceinline__ int att_chunk(int n, int splits) {
-  const int per = (n + splits - 1) / splits;
-  return max((per + ATT_CHUNK_MIN - 1) / ATT_CHUNK_MIN, 1) * ATT_CHUNK_MIN;
-}
 
 template <class T> struct AttType;
 template <> struct AttType<_Float16> {
@@ -81,9 +75,17 @@ __device__ __forceinline__ float sum_groups(float v, int lane) {
   return v + lane_xor<32>(v, lane);
 }
 
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// NT: nontemporal, for what is read once and not again soon.
+template <bool NT, class V>
+__device__ __forceinline__ V load_once(const V* p) {
+  return NT ? __builtin_nontemporal_load(p) : *p;
+}
+
 // T: the cache's type. DP: head dims padded to 64, 128 or 256; FULL: d == DP. EXACT: q or out is of another
-// type than the cache's.
-template <class T, int DP, bool FULL, bool EXACT>
+// type than the cache's. NT: keys and values by nontemporal loads.
+template <class T, int DP, bool FULL, bool EXACT, bool NT>
 __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
   typedef AttType<T> AT;
   typedef typename AT::vec8 vec8;
@@ -98,41 +100,38 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r16 = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
-  const int split = id % a.splits; id /= a.splits;
-  const int rb = id % a.row_blocks; id /= a.row_blocks;
-  const int head = id % a.c.heads, b = id / a.c.heads;
+  // Items (chunk, row, key-value head), heads fastest and chunks slowest: workgroups go to the XCDs in turn, so
+  // with chunks fastest one XCD got the first chunk of every ragged row and another their rarely used last. The
+  // row blocks of an item are 8 workgroups apart, on one XCD, where the second finds keys and values in its L2.
+  const unsigned bid = blockIdx.x, octet = bid / (8 * a.row_blocks), in8 = bid - octet * 8 * a.row_blocks;
+  const int rb = in8 >> 3, item = octet * 8 + (in8 & 7);
+  const int per = a.c.rows * a.c.heads;
+  if (item >= a.splits * per) return;
+  const int split = item / per, bh0 = item - split * per, b = bh0 / a.c.heads, head = bh0 - b * a.c.heads;
+  const int begin = split * a.chunk, t_first = begin + wave * ATT_TILE;
+  // the first tile's pages beside the length (of the table's last page where it has no such: that tile is not taken)
+  int first_page[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf)
+    first_page[hf] = a.c.table[b * a.c.table_stride + min((t_first + 16 * hf) >> a.c.page_shift, a.c.width - 1)];
   const int n = __builtin_amdgcn_readfirstlane(a.c.length(b));
-  const int chunk = att_chunk(n, a.splits);
-  const int begin = split * chunk, end = min(n, begin + chunk);
+  const int end = min(n, begin + a.chunk);
   if (begin >= n && split > 0) return;              // (a row of length 0 still writes its zeros)
   const int rows = min(16, a.group - rb * 16);      // query heads of this workgroup
   const int h0 = head * a.group + rb * 16;          // the first of them
   const int d = a.c.d;
 
-  // ---- q: lane (head r16, dims 32 j + 8 g ..), in NQ terms of T
+  // ---- q: lane (head r16, dims 32 j + 8 g ..), in NQ terms of T; zeros for heads and dims that are none
   vec8 q[NQ][KS];
   float fold = a.scale;
-  {
+  const long long q_at = b * a.q_b + (h0 + (r16 < rows ? r16 : 0)) * a.q_h + 8 * g;
+  const auto is_q = [&](int j) { return r16 < rows && (FULL || 32 * j + 8 * g < d); };
+  const auto load_q = [&](const auto* p, auto vec) {
     float f[KS][8];
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
-      const int dim = 32 * j + 8 * g;
-      if (r16 < rows && dim < d) {
-        const long long at = b * a.q_b + (h0 + r16) * a.q_h + dim;
-        if (a.q_dt == DT_F32) {
-          if (a.q_vec) load8<float, true>(static_cast<const float*>(a.q) + at, f[j]);
-          else load8<float, false>(static_cast<const float*>(a.q) + at, f[j]);
-        } else if (a.q_dt == DT_F16) {
-          if (a.q_vec) load8<_Float16, true>(static_cast<const _Float16*>(a.q) + at, f[j]);
-          else load8<_Float16, false>(static_cast<const _Float16*>(a.q) + at, f[j]);
-        } else {
-          if (a.q_vec) load8<bf16_t, true>(static_cast<const bf16_t*>(a.q) + at, f[j]);
-          else load8<bf16_t, false>(static_cast<const bf16_t*>(a.q) + at, f[j]);
-        }
-      }
+      const int off = FULL || 32 * j + 8 * g < d ? 32 * j : 0;
+      load8<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>, decltype(vec)::value>(p + q_at + off, f[j]);
     }
     if constexpr (EXACT) {
       // the row's largest element to [0.5, 1), so that no term leaves the type's range
@@ -140,7 +139,10 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
       for (int j = 0; j < KS; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[j][i]));
+        for (int i = 0; i < 8; ++i) {
+          if (!is_q(j)) f[j][i] = 0.f;
+          top = fmaxf(top, fabsf(f[j][i]));
+        }
       top = max_groups(top, lane);
       const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
       fold = __builtin_ldexpf(fold, e);
@@ -160,9 +162,13 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
       for (int j = 0; j < KS; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[0][j][i] = static_cast<T>(f[j][i]);
+        for (int i = 0; i < 8; ++i) q[0][j][i] = is_q(j) ? static_cast<T>(f[j][i]) : static_cast<T>(0.f);
     }
-  }
+  };
+  const auto load_q_as = [&](const auto* p) {
+    if (a.q_vec) load_q(p, std::true_type{});
+    else load_q(p, std::false_type{});
+  };
 
   // ---- the wave's tiles: begin / 32 + wave, + 4, ..
   float4_t o[DL];
@@ -171,59 +177,61 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
   float m = ATT_LOW, l = 0.f;
 
   u32x4_t kf[2][KS];
-  uint2 vf[8][VC];
+  u32x2_t vf[8][VC];
   const int sstr = static_cast<int>(a.c.slot_stride) * 2;      // bytes
   // the lane's byte offsets within a 16-token half
-  const int koff = r16 * sstr + g * 16;
-  const int voff = 4 * g * sstr + r16 * DL * 2;
-  int pg[2];                                                   // pages of the tile's halves
-  long long at[2];                                             // their element offsets
-  const auto locate = [&](int t0) {
-    // (a half that begins past the row's end may lie past the table: it is masked, any row serves)
+  const unsigned koff = r16 * sstr + g * 16;
+  const unsigned voff = 4 * g * sstr + r16 * DL * 2;
+  struct Where {
+    int t0;             // the tile's first token
+    bool ok[2];         // its halves' pages exist
+    long long at[2];    // the halves' element offsets
+  };
+  // page ids of a tile's halves (a half that begins past the row's end may lie past the table: it is masked, the
+  // other half's page serves)
+  const auto pages_of = [&](int t0, int (&pg)[2]) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int j = t0 + 16 * hf < n ? t0 + 16 * hf : t0;
-      pg[hf] = a.c.page_of(b, j);
-      at[hf] = a.c.row_at(max(pg[hf], 0), head, j);
+      pg[hf] = a.c.table[b * a.c.table_stride + (j >> a.c.page_shift)];
     }
   };
-  const auto load_k = [&]() {
+  const auto locate = [&](int t0, const int (&pg)[2]) {
+    Where w;
+    w.t0 = t0;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const char* p = static_cast<const char*>(a.c.k) + 2 * at[hf];
+      const int id = __builtin_amdgcn_readfirstlane(pg[hf]);
+      w.ok[hf] = static_cast<unsigned>(id) < static_cast<unsigned>(a.c.pages);
+      w.at[hf] = a.c.row_at(w.ok[hf] ? id : 0, head, t0 + 16 * hf < n ? t0 + 16 * hf : t0);
+    }
+    return w;
+  };
+  const auto load_k = [&](const Where& w) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const char* p = static_cast<const char*>(a.c.k) + 2 * w.at[hf];
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        if (FULL || 32 * j + 8 * g < d) kf[hf][j] = *reinterpret_cast<const u32x4_t*>(p + koff + 64 * j);
+        if (FULL || 32 * j + 8 * g < d) kf[hf][j] = load_once<NT>(reinterpret_cast<const u32x4_t*>(p + koff + 64 * j));
         else kf[hf][j] = u32x4_t{0, 0, 0, 0};
       }
     }
   };
-  const auto load_v = [&]() {
+  const auto load_v = [&](const Where& w) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const char* p = static_cast<const char*>(a.c.v) + 2 * at[i >> 2];
+      const char* p = static_cast<const char*>(a.c.v) + 2 * w.at[i >> 2];
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
-        if (FULL || r16 * DL + 4 * c < d) vf[i][c] = *reinterpret_cast<const uint2*>(p + voff + (i & 3) * sstr + 8 * c);
-        else vf[i][c] = make_uint2(0, 0);
+        if (FULL || r16 * DL + 4 * c < d) vf[i][c] = load_once<NT>(reinterpret_cast<const u32x2_t*>(p + voff + (i & 3) * sstr + 8 * c));
+        else vf[i][c] = u32x2_t{0, 0};
       }
     }
   };
-
-  const int step = ATT_TILE * ATT_WAVES;
-  int t0 = begin + wave * ATT_TILE;
-  bool have = t0 < end;
-  if (have) {
-    locate(t0);
-    load_k();
-    load_v();
-  }
-  while (have) {
-    const int cur = t0;
-    const bool whole = cur + ATT_TILE <= n && pg[0] >= 0 && pg[1] >= 0;
-    const bool ok0 = pg[0] >= 0, ok1 = pg[1] >= 0;
-    // ---- S^T = K Q^T
-    float s[8];
+  float s[8];
+  // S^T = K Q^T
+  const auto logits = [&]() {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -234,24 +242,26 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[4 * hf + r] = acc[r] * fold;
     }
-    if (!whole) {
+  };
+  // the weights against the running maximum, and out^T += V^T P^T
+  const auto accumulate = [&](const Where& w) {
+    if (w.t0 + ATT_TILE > n || !w.ok[0] || !w.ok[1]) {
       // tokens past the end and on missing pages: no weight, and nothing of what their memory holds
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int j = cur + 16 * (i >> 2) + 4 * g + (i & 3);
-        if (!(j < n && (i < 4 ? ok0 : ok1))) {
+        const int j = w.t0 + 16 * (i >> 2) + 4 * g + (i & 3);
+        if (!(j < n && w.ok[i >> 2])) {
           s[i] = -__builtin_inff();
 #pragma unroll
-          for (int c = 0; c < VC; ++c) vf[i][c] = make_uint2(0, 0);
+          for (int c = 0; c < VC; ++c) vf[i][c] = u32x2_t{0, 0};
         }
       }
     }
     if (a.logits && r16 < rows) {
-      float* p = a.logits + (static_cast<long long>(b) * a.hq + h0 + r16) * a.logit_stride + cur + 4 * g;
+      float* p = a.logits + (static_cast<long long>(b) * a.hq + h0 + r16) * a.logit_stride + w.t0 + 4 * g;
       *reinterpret_cast<float4_t*>(p) = float4_t{s[0], s[1], s[2], s[3]};
       *reinterpret_cast<float4_t*>(p + 16) = float4_t{s[4], s[5], s[6], s[7]};
     }
-    // ---- weights against the running maximum
     float top = s[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
@@ -266,26 +276,26 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
     vec8 p[NP];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float w = __builtin_amdgcn_exp2f(s[i] - m);
-      l += w;
+      float x = __builtin_amdgcn_exp2f(s[i] - m);
+      l += x;
 #pragma unroll
       for (int t = 0; t < NP; ++t) {
-        const T part = static_cast<T>(w);
+        const T part = static_cast<T>(x);
         p[t][i] = part;
-        w -= static_cast<float>(part);
+        x -= static_cast<float>(part);
       }
     }
-    // ---- out^T += V^T P^T, a dim pair (one 32-bit word of the 8 tokens' rows) at a time
+    // a dim pair (one 32-bit word of the 8 tokens' rows) at a time
 #pragma unroll
     for (int e = 0; e < DL; e += 2) {
-      uint32_t w[8];
+      uint32_t x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = (e & 2) ? vf[i][e / 4].y : vf[i][e / 4].x;
+      for (int i = 0; i < 8; ++i) x[i] = (e & 2) ? vf[i][e / 4].y : vf[i][e / 4].x;
       u32x4_t lo, hi;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        lo[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
-        hi[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+        lo[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
+        hi[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
       }
 #pragma unroll
       for (int t = 0; t < NP; ++t) {
@@ -293,12 +303,31 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
         o[e + 1] = AT::mfma(__builtin_bit_cast(vec8, hi), p[t], o[e + 1]);
       }
     }
-    t0 += step;
-    have = t0 < end;
-    if (have) {
-      locate(t0);
-      load_k();
-      load_v();
+  };
+
+  // q's loads and the first tile's go out together: q in the cache's type first, as it needs no conversion
+  int t0 = t_first, pg[2] = {first_page[0], t0 + 16 < n ? first_page[1] : first_page[0]};
+  if (!EXACT) load_q_as(static_cast<const T*>(a.q));
+  if (t0 < end) {
+    Where w = locate(t0, pg);
+    load_k(w);
+    load_v(w);
+    if (EXACT) {
+      if (a.q_dt == DT_F32) load_q_as(static_cast<const float*>(a.q));
+      else if (a.q_dt == DT_F16) load_q_as(static_cast<const _Float16*>(a.q));
+      else load_q_as(static_cast<const bf16_t*>(a.q));
+    }
+    while (true) {
+      const int next = t0 + ATT_TILE * ATT_WAVES;
+      const bool more = next < end;
+      pages_of(more ? next : t0, pg);
+      logits();
+      accumulate(w);
+      if (!more) break;
+      t0 = next;
+      w = locate(t0, pg);
+      load_k(w);
+      load_v(w);
     }
   }
   l = sum_groups(l, lane);
@@ -330,41 +359,38 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
       sum = __builtin_fmaf(s_l[w][row], f, sum);
       acc += *reinterpret_cast<const float4_t*>(&s_o[w][row][dim]) * f;
     }
+    const long long chunk_at = (bh + row) * a.splits + split;
     if (a.splits == 1) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // no token (or none on a page that exists)
-      if (dim < d) {
-        const long long o0 = (bh + row) * d + dim;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) store_dt(a.out, o0 + i, a.out_dt, acc[i] * inv);
-      }
-      if (a.total && dim == 0) {
-        a.total[2 * (bh + row)] = mx;
-        a.total[2 * (bh + row) + 1] = inv;
-      }
-    } else {
-      if (dim < d) *reinterpret_cast<float4_t*>(a.part + ((bh + row) * a.splits + split) * d + dim) = acc;
-      if (dim == 0) {
-        float* p = a.ml + 2 * ((bh + row) * a.splits + split);
-        p[0] = mx;
-        p[1] = sum;
-      }
+      if (dim < d) store4_dt(a.out, (bh + row) * d + dim, a.out_dt, acc * inv);
+    } else if (dim < d) {
+      *reinterpret_cast<float4_t*>(a.part + chunk_at * d + dim) = acc;
     }
+    if (a.ml && dim == 0) *reinterpret_cast<float2*>(a.ml + 2 * chunk_at) = make_float2(mx, sum);
   }
 }
 
 // The chunks of one (row, query head) joined: out = sum_c f_c part_c / sum_c f_c sum_c, f_c = 2^(m_c - max).
-// A workgroup's threads take the chunks' maxima and sums side by side, then the partial sums as (chunk group,
-// 4 dims), so that all of a round's loads are in flight together; one thread per dim that walked the chunks
-// one after another took 48 us for 64 chunks of 32 heads, this takes 4.
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+// A workgroup's threads take the chunks' maxima and sums side by side, and the partial sums as (chunk group,
+// 4 dims), the first ATT_AHEAD of a thread loaded before the maxima are known. (One thread per dim that walked the
+// chunks one after another took 48 us for 64 chunks of 32 heads; this takes JOIN_FIGURES.)
+constexpr int ATT_AHEAD = 8;
+
+__device__ __forceinline__ void attend_join(const AttendArgs& a, long long bh) {
   __shared__ float s_f[ATT_SPLITS], s_red[2][4];
   __shared__ float4_t s_acc[256];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const long long bh = blockIdx.x;
   const int b = static_cast<int>(bh / a.hq), d = a.c.d;
-  const int n = a.c.length(b), chunk = att_chunk(n, a.splits);
-  const int used = max((n + chunk - 1) / chunk, 1);
+  const int used = max((a.c.length(b) + a.chunk - 1) / a.chunk, 1);
   const float2* ml = reinterpret_cast<const float2*>(a.ml) + bh * a.splits;
+  const int quads = d / 4, groups = 256 / quads;
+  const int grp = tid / quads, dim = (tid - grp * quads) * 4;
+  const float* part = a.part + bh * a.splits * d + dim;
+  const bool mine = grp < groups;
+  float4_t ahead[ATT_AHEAD];
+#pragma unroll
+  for (int i = 0; i < ATT_AHEAD; ++i)
+    ahead[i] = *reinterpret_cast<const float4_t*>(part + static_cast<long long>(min(mine ? grp + i * groups : 0, used - 1)) * d);
   float m[ATT_SPLITS / 256], l[ATT_SPLITS / 256], mx = ATT_LOW;
 #pragma unroll
   for (int i = 0; i < ATT_SPLITS / 256; ++i) {
@@ -390,42 +416,66 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   __syncthreads();
   sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // no token (or none on a page that exists)
-  const int quads = d / 4, groups = 256 / quads;
-  const int grp = tid / quads, dim = (tid - grp * quads) * 4;
   float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
-  if (grp < groups) {
-#pragma unroll 8
-    for (int c = grp; c < used; c += groups)
-      acc += *reinterpret_cast<const float4_t*>(a.part + (bh * a.splits + c) * d + dim) * s_f[c];
+  if (mine) {
+#pragma unroll
+    for (int i = 0; i < ATT_AHEAD; ++i)
+      if (grp + i * groups < used) acc += ahead[i] * s_f[grp + i * groups];
+    for (int c = grp + ATT_AHEAD * groups; c < used; c += groups)
+      acc += *reinterpret_cast<const float4_t*>(part + static_cast<long long>(c) * d) * s_f[c];
   }
   s_acc[tid] = acc;
   __syncthreads();
   if (grp == 0) {
     for (int i = 1; i < groups; ++i) acc += s_acc[i * quads + tid];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) store_dt(a.out, bh * d + dim + i, a.out_dt, acc[i] * inv);
-  }
-  if (a.total && tid == 0) {
-    a.total[2 * bh] = mx;
-    a.total[2 * bh + 1] = inv;
+    store4_dt(a.out, bh * d + dim, a.out_dt, acc * inv);
   }
 }
 
-// score_j += sum over the key-value head's query heads of p_j.
-__global__ __launch_bounds__(256) void attend_score_kernel(AttendArgs a) {
-  int id = blockIdx.x;
-  const int per = (a.c.max_len + 255) / 256;
-  const int j = (id % per) * 256 + threadIdx.x; id /= per;
-  const int head = id % a.c.heads, b = id / a.c.heads;
-  if (j >= a.c.length(b)) return;
-  const int page = a.c.page_of(b, j);
-  if (page < 0) return;
+// score_j += sum over the key-value head's query heads of p_j, for 256 tokens of a (row, head): each wave first
+// joins the chunks' maxima and sums of its share of the query heads.
+__device__ __forceinline__ void attend_score(const AttendArgs& a, int id) {
+  __shared__ float s_m[64], s_inv[64];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int per = a.c.rows * a.c.heads, block = id / per, at = id - block * per;
+  const int b = at / a.c.heads, head = at - b * a.c.heads, n = a.c.length(b);
+  if (block * 256 >= n) return;
+  const int used = (n + a.chunk - 1) / a.chunk, j = block * 256 + tid;
+  const long long bh0 = static_cast<long long>(b) * a.hq + head * a.group;
+  const float2* ml = reinterpret_cast<const float2*>(a.ml) + bh0 * a.splits;
+  const float* logits = a.logits + bh0 * a.logit_stride + j;
   float sum = 0.f;
-  for (int i = 0; i < a.group; ++i) {
-    const long long bh = static_cast<long long>(b) * a.hq + head * a.group + i;
-    sum += exp2f(a.logits[bh * a.logit_stride + j] - a.total[2 * bh]) * a.total[2 * bh + 1];
+  for (int g0 = 0; g0 < a.group; g0 += 64) {
+    const int some = min(64, a.group - g0);
+    for (int i = wave; i < some; i += 4) {
+      float mx = ATT_LOW, total = 0.f;
+      for (int c = lane; c < used; c += 64) mx = fmaxf(mx, ml[(g0 + i) * a.splits + c].x);
+      mx = wave_max(mx, lane);
+      for (int c = lane; c < used; c += 64) {
+        const float2 v = ml[(g0 + i) * a.splits + c];
+        total = __builtin_fmaf(v.y, exp2f(v.x - mx), total);
+      }
+      total = wave_sum(total, lane);
+      if (lane == 0) {
+        s_m[i] = mx;
+        s_inv[i] = total == 0.f ? 0.f : 1.0f / total;
+      }
+    }
+    __syncthreads();
+    if (j < n)
+#pragma unroll 4
+      for (int i = 0; i < some; ++i) sum += exp2f(logits[(g0 + i) * a.logit_stride] - s_m[i]) * s_inv[i];
+    __syncthreads();
   }
-  a.c.scores[a.c.slot_at(page, head, j)] += sum;
+  if (j >= n) return;
+  const int page = a.c.page_of(b, j);
+  if (page >= 0) a.c.scores[a.c.slot_at(page, head, j)] += sum;
+}
+
+// The workgroups of the join, then those of the scores.
+__global__ __launch_bounds__(256) void attend_finish_kernel(AttendArgs a, int joins) {
+  if (static_cast<int>(blockIdx.x) < joins) attend_join(a, blockIdx.x);
+  else attend_score(a, blockIdx.x - joins);
 }
 
 }  // namespace trellis

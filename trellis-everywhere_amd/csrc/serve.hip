@@ -125,9 +125,9 @@ void launch_append(const AppendArgs& a, bool vec, int lpr, int rounds, int parts
 // ---------------------------------------------------------------- attention
 
 struct AttendPlan {
-  int splits, row_blocks;
+  int splits, row_blocks, chunk;
   int64_t logit_stride;
-  size_t off_ml, off_total, off_logits, ws;
+  size_t off_ml, off_logits, ws;
 };
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -137,40 +137,73 @@ AttendPlan attend_plan(const trellis_kv_cache* c, int q_heads, bool accumulate) 
   const int n = longest(c), group = q_heads / c->heads;
   p.row_blocks = (group + 15) / 16;
   const int64_t one = static_cast<int64_t>(c->rows) * c->heads * p.row_blocks;
-  // chunks of at least ATT_CHUNK_MIN tokens, enough of them for four workgroups per CU
-  const int64_t most = (n + ATT_CHUNK_MIN - 1) / ATT_CHUNK_MIN;
-  const int64_t want = one > 0 ? (4LL * device_cus() + one - 1) / one : 1;
-  p.splits = static_cast<int>(want < most ? want : most);
-  if (p.splits > ATT_SPLITS) p.splits = ATT_SPLITS;
-  if (p.splits < 1) p.splits = 1;
+  // One chunk up to 512 tokens (400 of 8 heads: 8.4 us either way, and a launch less). Above, chunks for two
+  // workgroups per CU where there is one row, for four where there are several, as of uneven lengths about half are
+  // empty (16 rows up to 4099 tokens for two / four: 43.1 / 38.2 us). Of one tile a wave at least (one row of 4000
+  // tokens of 8 heads in chunks of 128 / 256 / 512: 11.4 / 13.7 / 14.4 us; 32717: 35.6 / 32.9 / 31.1, and 38.9 in
+  // 2048), two for several rows (8 of 2000 in 128 / 256 / 512: 19.0 / 17.5 / 17.9); and 4096 tokens at most, for rows of
+  // uneven lengths (64 up to 8192 in 4096 / 8192: 232 / 241; where all are 4096 long, 2048 / 4096: 197 / 188).
+  int64_t splits = 1;
+  if (n > 512 && one > 0) {
+    const int64_t want = ((c->rows == 1 ? 2LL : 4LL) * device_cus() + one - 1) / one;
+    const int64_t shortest = c->rows == 1 ? ATT_CHUNK_MIN : 2 * ATT_CHUNK_MIN;
+    const int64_t least = (n + 4095) / 4096, most = (n + shortest - 1) / shortest;
+    splits = want > least ? want : least;
+    if (splits > most) splits = most;
+    if (splits > ATT_SPLITS) splits = ATT_SPLITS;
+  }
+  p.chunk = static_cast<int>(((n + splits - 1) / splits + ATT_CHUNK_MIN - 1) / ATT_CHUNK_MIN * ATT_CHUNK_MIN);
+  if (p.chunk < ATT_CHUNK_MIN) p.chunk = ATT_CHUNK_MIN;
+  p.splits = n > 0 ? (n + p.chunk - 1) / p.chunk : 1;
   const size_t bh = static_cast<size_t>(c->rows) * q_heads;
   p.logit_stride = (static_cast<int64_t>(n) + 31) / 32 * 32;
   size_t ws = p.splits > 1 ? up256(bh * p.splits * c->head_dim * 4) : 0;
   p.off_ml = ws;
-  if (p.splits > 1) ws += up256(bh * p.splits * 8);
-  p.off_total = ws;
-  if (accumulate) ws += up256(bh * 8);
+  if (p.splits > 1 || accumulate) ws += up256(bh * p.splits * 8);
   p.off_logits = ws;
   if (accumulate) ws += up256(bh * p.logit_stride * 4);
   p.ws = ws;
   return p;
 }
 
-template <class T, int DP>
-void launch_attend(const AttendArgs& a, bool exact, unsigned grid, hipStream_t st) {
-  const bool full = a.c.d == DP;
+// Nontemporal loads where a call of 16 MB and more reads whole 128-byte lines once: keys and values of some tens
+// of layers of that size do not stay in the 256 MB last-level cache until their next use (36 layers in turn: 4000
+// tokens of 8 heads of 128 11.4 -> 10.3 us, 16000 20.3 -> 19.1; one layer of 131072 101 -> 91 us, 64 rows of 8192
+// 379 -> 344). Not below (32 rows up to 512 tokens of 3 heads of 64: 7.6 -> 8.2), for other head dims (96: 81 -> 92) or
+// where a second workgroup reads the same lines (more than 16 query heads a head; 64 over 2: 42 -> 51).
+bool attend_streams(const trellis_kv_cache* c, const AttendPlan& p) {
+  const int64_t bytes = static_cast<int64_t>(c->rows) * longest(c) * c->heads * c->head_dim * 4;
+  return bytes >= (16 << 20) && p.row_blocks == 1 && c->head_dim % 64 == 0;
+}
+
+template <class T, int DP, bool FULL, bool EXACT>
+void launch_attend_nt(const AttendArgs& a, bool nt, unsigned grid, hipStream_t st) {
   const dim3 block(64 * ATT_WAVES);
-  if (full && exact) hipLaunchKernelGGL((attend_kernel<T, DP, true, true>), dim3(grid), block, 0, st, a);
-  else if (full) hipLaunchKernelGGL((attend_kernel<T, DP, true, false>), dim3(grid), block, 0, st, a);
-  else if (exact) hipLaunchKernelGGL((attend_kernel<T, DP, false, true>), dim3(grid), block, 0, st, a);
-  else hipLaunchKernelGGL((attend_kernel<T, DP, false, false>), dim3(grid), block, 0, st, a);
+  if constexpr (FULL) {
+    if (nt) {
+      hipLaunchKernelGGL((attend_kernel<T, DP, FULL, EXACT, true>), dim3(grid), block, 0, st, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((attend_kernel<T, DP, FULL, EXACT, false>), dim3(grid), block, 0, st, a);
+}
+
+template <class T, int DP>
+void launch_attend(const AttendArgs& a, bool exact, bool nt, unsigned grid, hipStream_t st) {
+  if (a.c.d == DP) {
+    if (exact) launch_attend_nt<T, DP, true, true>(a, nt, grid, st);
+    else launch_attend_nt<T, DP, true, false>(a, nt, grid, st);
+  } else {
+    if (exact) launch_attend_nt<T, DP, false, true>(a, nt, grid, st);
+    else launch_attend_nt<T, DP, false, false>(a, nt, grid, st);
+  }
 }
 
 template <class T>
-void launch_attend_d(const AttendArgs& a, bool exact, unsigned grid, hipStream_t st) {
-  if (a.c.d <= 64) launch_attend<T, 64>(a, exact, grid, st);
-  else if (a.c.d <= 128) launch_attend<T, 128>(a, exact, grid, st);
-  else launch_attend<T, 256>(a, exact, grid, st);
+void launch_attend_d(const AttendArgs& a, bool exact, bool nt, unsigned grid, hipStream_t st) {
+  if (a.c.d <= 64) launch_attend<T, 64>(a, exact, nt, grid, st);
+  else if (a.c.d <= 128) launch_attend<T, 128>(a, exact, nt, grid, st);
+  else launch_attend<T, 256>(a, exact, nt, grid, st);
 }
 
 int validate_attention(const trellis_kv_cache* c, int q_heads, int accumulate) {
@@ -379,25 +412,25 @@ int trellis_paged_attention(const trellis_kv_cache* cache, const void* q, int64_
   a.group = q_heads / cache->heads;
   a.row_blocks = p.row_blocks;
   a.splits = p.splits;
+  a.chunk = p.chunk;
   a.scale = scale * 1.44269504088896340736f;
   a.part = reinterpret_cast<float*>(ws);
-  a.ml = reinterpret_cast<float*>(ws + p.off_ml);
-  a.total = accumulate ? reinterpret_cast<float*>(ws + p.off_total) : nullptr;
+  a.ml = p.splits > 1 || accumulate ? reinterpret_cast<float*>(ws + p.off_ml) : nullptr;
   a.logits = accumulate ? reinterpret_cast<float*>(ws + p.off_logits) : nullptr;
   a.logit_stride = p.logit_stride;
   a.c = cache_of(cache);
   const int64_t one = static_cast<int64_t>(cache->rows) * cache->heads;
-  const int64_t blocks = one * p.row_blocks * p.splits, bh = static_cast<int64_t>(cache->rows) * q_heads;
-  const int64_t score_blocks = one * ((static_cast<int64_t>(cache->max_len) + 255) / 256);
-  if (!grid_fits(blocks, 64 * ATT_WAVES) || !grid_fits(bh, 256) || (accumulate && !grid_fits(score_blocks, 256)))
-    return TRELLIS_ERR_BATCH;
+  const int64_t blocks = (one * p.splits + 7) / 8 * 8 * p.row_blocks, bh = static_cast<int64_t>(cache->rows) * q_heads;
+  const int64_t joins = p.splits > 1 ? bh : 0;
+  const int64_t finish = joins + (accumulate ? one * ((longest(cache) + 255) / 256) : 0);
+  if (!grid_fits(blocks, 64 * ATT_WAVES) || !grid_fits(finish, 256)) return TRELLIS_ERR_BATCH;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool exact = q_dtype != cache->dtype || out_dtype == TRELLIS_F32;
-  if (cache->dtype == TRELLIS_F16) launch_attend_d<_Float16>(a, exact, static_cast<unsigned>(blocks), st);
-  else launch_attend_d<bf16_t>(a, exact, static_cast<unsigned>(blocks), st);
-  if (p.splits > 1) hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>(bh)), dim3(256), 0, st, a);
-  if (accumulate && score_blocks > 0)
-    hipLaunchKernelGGL(attend_score_kernel, dim3(static_cast<unsigned>(score_blocks)), dim3(256), 0, st, a);
+  const bool nt = attend_streams(cache, p);
+  if (cache->dtype == TRELLIS_F16) launch_attend_d<_Float16>(a, exact, nt, static_cast<unsigned>(blocks), st);
+  else launch_attend_d<bf16_t>(a, exact, nt, static_cast<unsigned>(blocks), st);
+  if (finish > 0)
+    hipLaunchKernelGGL(attend_finish_kernel, dim3(static_cast<unsigned>(finish)), dim3(256), 0, st, a, static_cast<int>(joins));
   return launched();
 }
 
