@@ -32,8 +32,8 @@ namespace trellis {
 
 constexpr int ATT_WAVES = 4;
 constexpr int ATT_TILE = 32;                          // tokens per tile
-constexpr int ATT_CHUNK_MIN = ATT_TILE * ATT_WAVES;   // the shortest chunk: a tile per wave
-constexpr int ATT_SPLITS = 1024;                      // the most chunks of a row
+constexpr int ATT_UNIT = ATT_TILE * ATT_WAVES;        // tokens per unit: a tile per wave
+constexpr int ATT_PARTS = 1024;                       // the most chunks of a row
 constexpr float ATT_LOW = -3.0e38f;                   // below every logit that counts
 constexpr float ATT_TOP = 11.f;                       // log2 of the weight at the maximum when it is set
 constexpr float ATT_SLACK = 4.f;                      // how far (log2) a logit may pass it
@@ -43,14 +43,70 @@ struct AttendArgs {
   long long q_b, q_h;     // strides of q in elements
   int q_dt, q_vec;        // q_vec: q's rows are 16-byte aligned
   void* out;              // [rows][hq][d]
-  int out_dt, hq, group, row_blocks, splits, chunk;
+  int out_dt, hq, group, row_blocks;
+  int aim;                // chunks wanted of the whole work; 0: a row is one chunk
+  int chunk;              // one row: its chunks' tokens
+  int items;              // workgroups (of one row block) that can have a chunk
   float scale;            // times log2(e)
-  float* part;            // splits > 1: [rows][kv heads][splits][hq of the kv head][d] unnormalised sums
-  float* ml;              // splits > 1 or with scores: [rows][hq][splits][2] maximum and sum
+  float* part;            // [items][group][d] unnormalised sums of rows of several chunks
+  float* ml;              // [items][group][2] their maximum and sum
+  float* total;           // with scores: [rows][hq][2] maximum and 1 / sum of rows of one chunk
   float* logits;          // with scores: [rows][hq][logit_stride]
   long long logit_stride;
   Cache c;
 };
+
+// A value that is the same in every lane, into a scalar register (a division leaves it in a vector register, and
+// addresses made from it in two a lane).
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// ---- chunks. The lengths are on the GPU, so that is where the chunks of several rows are made: all of the same
+// number of units, ceil(units / aim) up to 6, above that so many that there are up to 4 aim of them (rows of uneven
+// lengths then end together), at least 2. The chunks of all rows lie in a line, rows slowest, heads fastest; a
+// workgroup's number is its chunk's place in the line, and the place of its partial sums. Against chunks of one size
+// planned for the longest row: 16 rows up to 4099 tokens of 8 heads 39.3 -> 32.4 us, 64 up to 8192 228 -> 206, 4 up to
+// 8192 24.9 -> 18.4. (aim / 2 aim / 4 aim chunks of 32 rows up to 8192: 120 / 103 / 98 us; of 24 up to 4096, 6 units
+// each for aim: 43.0 / 45.1 / 45.0; of 32 up to 2048, 4 units: 36.1 / 36.5 / 36.4.)
+constexpr int ATT_LONG = 6;      // units of a chunk that more chunks are preferred to
+
+__host__ __device__ __forceinline__ int att_units(int n) { return (n + ATT_UNIT - 1) / ATT_UNIT; }
+
+// Lengths of rows r0 .. r0 + 63, one a lane.
+__device__ __forceinline__ int att_lengths(const Cache& c, int r0, int lane) {
+  const int b = r0 + lane, n = c.length(min(b, c.rows - 1));
+  return b < c.rows ? n : 0;
+}
+
+// Units of a chunk (by a whole wave); `len0`: att_lengths of rows 0 .. 63.
+__device__ __forceinline__ int att_chunk(const AttendArgs& a, int len0, int lane) {
+  int units = 0;
+  for (int r0 = 0; r0 < a.c.rows; r0 += 64)
+    units += __builtin_amdgcn_readlane(wave_scan(att_units(r0 ? att_lengths(a.c, r0, lane) : len0)), 63);
+  units *= a.c.heads;
+  const int even = (units + a.aim - 1) / a.aim;
+  return uniform(even <= ATT_LONG ? max(even, 2) : max((units + 4 * a.aim - 1) / (4 * a.aim), ATT_LONG));
+}
+
+struct Place {
+  int b, n;       // a row and its length
+  int chunks;     // of one head of it
+  int before;     // chunks of one head of all rows below it
+};
+
+// The row with chunk `pos` of the line, or (pos < 0) row `b`; chunks 0 where the line ends below pos.
+__device__ __forceinline__ Place att_find(const AttendArgs& a, int chunk, int pos, int b, int len0, int lane) {
+  int before = 0;
+  for (int r0 = 0; r0 < a.c.rows; r0 += 64) {
+    const int len = r0 ? att_lengths(a.c, r0, lane) : len0, mine = (att_units(len) + chunk - 1) / chunk, scan = wave_scan(mine);
+    const unsigned long long hit = pos < 0 ? (b < r0 + 64 ? 1ull << (b - r0) : 0) : __ballot((before + scan) * a.c.heads > pos);
+    if (hit) {
+      const int l = __builtin_ctzll(hit), chunks = __builtin_amdgcn_readlane(mine, l);
+      return {r0 + l, __builtin_amdgcn_readlane(len, l), chunks, before + __builtin_amdgcn_readlane(scan, l) - chunks};
+    }
+    before += __builtin_amdgcn_readlane(scan, 63);
+  }
+  return {0, 0, 0, before};
+}
 
 template <class T> struct AttType;
 template <> struct AttType<_Float16> {
@@ -100,26 +156,52 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r16 = lane & 15, g = lane >> 4;
-  // Items (chunk, row, key-value head), heads fastest and chunks slowest: workgroups go to the XCDs in turn, so
-  // with chunks fastest one XCD got the first chunk of every ragged row and another their rarely used last. The
-  // row blocks of an item are 8 workgroups apart, on one XCD, where the second finds keys and values in its L2.
+  // The row blocks of an item are 8 workgroups apart, on one XCD (workgroups go to the 8 XCDs in turn), where the
+  // second finds keys and values in its L2.
   const unsigned bid = blockIdx.x, octet = bid / (8 * a.row_blocks), in8 = bid - octet * 8 * a.row_blocks;
-  const int rb = in8 >> 3, item = octet * 8 + (in8 & 7);
-  const int per = a.c.rows * a.c.heads;
-  if (item >= a.splits * per) return;
-  const int split = item / per, bh0 = item - split * per, b = bh0 / a.c.heads, head = bh0 - b * a.c.heads;
-  const int begin = split * a.chunk, t_first = begin + wave * ATT_TILE;
-  // the first tile's pages beside the length (of the table's last page where it has no such: that tile is not taken)
-  int first_page[2];
-#pragma unroll
-  for (int hf = 0; hf < 2; ++hf)
-    first_page[hf] = a.c.table[b * a.c.table_stride + min((t_first + 16 * hf) >> a.c.page_shift, a.c.width - 1)];
-  const int n = __builtin_amdgcn_readfirstlane(a.c.length(b));
-  const int end = min(n, begin + a.chunk);
-  if (begin >= n && split > 0) return;              // (a row of length 0 still writes its zeros)
+  const int rb = uniform(in8 >> 3), item = uniform(octet * 8 + (in8 & 7));
+  if (item >= a.items) return;
+  int b, head, n, begin, size;
+  if (a.aim == 0) {
+    b = uniform(item / a.c.heads);
+    head = item - b * a.c.heads;
+    begin = 0;
+    n = size = a.c.length(b);
+  } else if (a.chunk) {
+    b = 0;
+    const int nth = uniform(item / a.c.heads);
+    head = item - nth * a.c.heads;
+    size = a.chunk;
+    begin = nth * size;
+    n = a.c.length(0);
+  } else {
+    const int len0 = att_lengths(a.c, 0, lane), units = att_chunk(a, len0, lane);
+    const Place at = att_find(a, units, item, 0, len0, lane);
+    if (at.chunks == 0) return;
+    const int off = item - at.before * a.c.heads, nth = uniform(off / a.c.heads);
+    b = at.b;
+    n = at.n;
+    head = off - nth * a.c.heads;
+    size = units * ATT_UNIT;
+    begin = nth * size;
+  }
+  b = uniform(b);
+  head = uniform(head);
+  begin = uniform(begin);
+  size = uniform(size);
   const int rows = min(16, a.group - rb * 16);      // query heads of this workgroup
   const int h0 = head * a.group + rb * 16;          // the first of them
   const int d = a.c.d;
+  int t0 = begin + wave * ATT_TILE;
+  // the first tile's pages beside the length (of the table's last page where it has no such: that tile is not taken)
+  int pg[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf)
+    pg[hf] = load_const(a.c.table + b * a.c.table_stride + min((t0 + 16 * hf) >> a.c.page_shift, a.c.width - 1));
+  n = uniform(n);
+  if (begin >= n && begin > 0) return;              // (a row of length 0 is one chunk where rows are, and gets its zeros)
+  const int end = min(n, begin + size);
+  const bool whole = end - begin == n;             // the row is one chunk
 
   // ---- q: lane (head r16, dims 32 j + 8 g ..), in NQ terms of T; zeros for heads and dims that are none
   vec8 q[NQ][KS];
@@ -170,7 +252,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
     else load_q(p, std::false_type{});
   };
 
-  // ---- the wave's tiles: begin / 32 + wave, + 4, ..
+  // ---- the wave's tiles: every fourth of the run
   float4_t o[DL];
 #pragma unroll
   for (int e = 0; e < DL; ++e) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -193,7 +275,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int j = t0 + 16 * hf < n ? t0 + 16 * hf : t0;
-      pg[hf] = a.c.table[b * a.c.table_stride + (j >> a.c.page_shift)];
+      pg[hf] = load_const(a.c.table + b * a.c.table_stride + (j >> a.c.page_shift));
     }
   };
   const auto locate = [&](int t0, const int (&pg)[2]) {
@@ -306,7 +388,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
   };
 
   // q's loads and the first tile's go out together: q in the cache's type first, as it needs no conversion
-  int t0 = t_first, pg[2] = {first_page[0], t0 + 16 < n ? first_page[1] : first_page[0]};
+  if (t0 + 16 >= n) pg[1] = pg[0];
   if (!EXACT) load_q_as(static_cast<const T*>(a.q));
   if (t0 < end) {
     Where w = locate(t0, pg);
@@ -359,43 +441,68 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
       sum = __builtin_fmaf(s_l[w][row], f, sum);
       acc += *reinterpret_cast<const float4_t*>(&s_o[w][row][dim]) * f;
     }
-    const long long chunk_at = (bh + row) * a.splits + split;
-    if (a.splits == 1) {
+    if (whole) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // no token (or none on a page that exists)
       if (dim < d) store4_dt(a.out, (bh + row) * d + dim, a.out_dt, acc * inv);
-    } else if (dim < d) {
-      *reinterpret_cast<float4_t*>(a.part + chunk_at * d + dim) = acc;
+      if (a.total && dim == 0) *reinterpret_cast<float2*>(a.total + 2 * (bh + row)) = make_float2(mx, inv);
+    } else {
+      const long long at = static_cast<long long>(item) * a.group + rb * 16 + row;
+      if (dim < d) *reinterpret_cast<float4_t*>(a.part + at * d + dim) = acc;
+      if (dim == 0) *reinterpret_cast<float2*>(a.ml + 2 * at) = make_float2(mx, sum);
     }
-    if (a.ml && dim == 0) *reinterpret_cast<float2*>(a.ml + 2 * chunk_at) = make_float2(mx, sum);
   }
 }
 
-// The chunks of one (row, query head) joined: out = sum_c f_c part_c / sum_c f_c sum_c, f_c = 2^(m_c - max).
-// A workgroup's threads take the chunks' maxima and sums side by side, and the partial sums as (chunk group,
-// 4 dims), the first ATT_AHEAD of a thread loaded before the maxima are known. (One thread per dim that walked the
-// chunks one after another took 48 us for 64 chunks of 32 heads; this takes JOIN_FIGURES.)
+// The chunks of a (row, key-value head): `used` of them, the i-th at place first + i * heads of the line.
+struct Parts {
+  int n, used, first, heads;
+  __device__ __forceinline__ long long at(int i) const { return first + static_cast<long long>(i) * heads; }
+};
+
+__device__ __forceinline__ Parts att_parts(const AttendArgs& a, int b, int head, int lane) {
+  if (a.aim == 0) return {a.c.length(b), 1, 0, 0};
+  if (a.chunk) {
+    const int n = a.c.length(0);
+    return {n, (n + a.chunk - 1) / a.chunk, head, a.c.heads};
+  }
+  const int len0 = att_lengths(a.c, 0, lane);
+  const Place at = att_find(a, att_chunk(a, len0, lane), -1, b, len0, lane);
+  return {at.n, at.chunks, at.before * a.c.heads + head, a.c.heads};
+}
+
+// The parts of one (row, query head) joined: out = sum_i f_i part_i / sum_i f_i sum_i, f_i = 2^(m_i - max).
+// A workgroup's threads take the parts' maxima and sums side by side, and the partial sums as (part group, 4
+// dims), the first ATT_AHEAD of a thread loaded before the maxima are known. (One thread per dim that walked the
+// parts one after another took 48 us for 64 parts of 32 heads; this takes JOIN_FIGURES.)
 constexpr int ATT_AHEAD = 8;
 
 __device__ __forceinline__ void attend_join(const AttendArgs& a, long long bh) {
-  __shared__ float s_f[ATT_SPLITS], s_red[2][4];
+  __shared__ float s_f[ATT_PARTS], s_red[2][4];
   __shared__ float4_t s_acc[256];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int b = static_cast<int>(bh / a.hq), d = a.c.d;
-  const int used = max((a.c.length(b) + a.chunk - 1) / a.chunk, 1);
-  const float2* ml = reinterpret_cast<const float2*>(a.ml) + bh * a.splits;
+  const int b = static_cast<int>(bh / a.hq), qh = static_cast<int>(bh - static_cast<long long>(b) * a.hq), d = a.c.d;
+  const int head = qh / a.group, in_group = qh - head * a.group;
+  const Parts parts = att_parts(a, b, head, lane);
   const int quads = d / 4, groups = 256 / quads;
   const int grp = tid / quads, dim = (tid - grp * quads) * 4;
-  const float* part = a.part + bh * a.splits * d + dim;
+  if (parts.used < 2) {
+    if (parts.used == 0 && grp == 0) store4_dt(a.out, bh * d + dim, a.out_dt, float4_t{0.f, 0.f, 0.f, 0.f});
+    return;
+  }
+  const int used = parts.used;
   const bool mine = grp < groups;
+  const auto part = [&](int i) {
+    return *reinterpret_cast<const float4_t*>(a.part + (parts.at(i) * a.group + in_group) * d + dim);
+  };
   float4_t ahead[ATT_AHEAD];
 #pragma unroll
-  for (int i = 0; i < ATT_AHEAD; ++i)
-    ahead[i] = *reinterpret_cast<const float4_t*>(part + static_cast<long long>(min(mine ? grp + i * groups : 0, used - 1)) * d);
-  float m[ATT_SPLITS / 256], l[ATT_SPLITS / 256], mx = ATT_LOW;
+  for (int i = 0; i < ATT_AHEAD; ++i) ahead[i] = part(min(mine ? grp + i * groups : 0, used - 1));
+  float m[ATT_PARTS / 256], l[ATT_PARTS / 256], mx = ATT_LOW;
 #pragma unroll
-  for (int i = 0; i < ATT_SPLITS / 256; ++i) {
-    const int c = tid + 256 * i;
-    const float2 v = c < used ? ml[c] : make_float2(ATT_LOW, 0.f);
+  for (int i = 0; i < ATT_PARTS / 256; ++i) {
+    const int p = tid + 256 * i;
+    float2 v = make_float2(ATT_LOW, 0.f);
+    if (p < used) v = reinterpret_cast<const float2*>(a.ml)[parts.at(p) * a.group + in_group];
     m[i] = v.x;
     l[i] = v.y;
     mx = fmaxf(mx, v.x);
@@ -406,7 +513,7 @@ __device__ __forceinline__ void attend_join(const AttendArgs& a, long long bh) {
   mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < ATT_SPLITS / 256; ++i) {
+  for (int i = 0; i < ATT_PARTS / 256; ++i) {
     const float f = exp2f(m[i] - mx);
     if (tid + 256 * i < used) s_f[tid + 256 * i] = f;
     sum = __builtin_fmaf(l[i], f, sum);
@@ -415,14 +522,13 @@ __device__ __forceinline__ void attend_join(const AttendArgs& a, long long bh) {
   if (lane == 0) s_red[1][wave] = sum;
   __syncthreads();
   sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // no token (or none on a page that exists)
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // no token on a page that exists
   float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
   if (mine) {
 #pragma unroll
     for (int i = 0; i < ATT_AHEAD; ++i)
       if (grp + i * groups < used) acc += ahead[i] * s_f[grp + i * groups];
-    for (int c = grp + ATT_AHEAD * groups; c < used; c += groups)
-      acc += *reinterpret_cast<const float4_t*>(part + static_cast<long long>(c) * d) * s_f[c];
+    for (int i = grp + ATT_AHEAD * groups; i < used; i += groups) acc += part(i) * s_f[i];
   }
   s_acc[tid] = acc;
   __syncthreads();
@@ -433,32 +539,41 @@ __device__ __forceinline__ void attend_join(const AttendArgs& a, long long bh) {
 }
 
 // score_j += sum over the key-value head's query heads of p_j, for 256 tokens of a (row, head): each wave first
-// joins the chunks' maxima and sums of its share of the query heads.
+// joins the maxima and sums of its share of the query heads.
 __device__ __forceinline__ void attend_score(const AttendArgs& a, int id) {
   __shared__ float s_m[64], s_inv[64];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int per = a.c.rows * a.c.heads, block = id / per, at = id - block * per;
-  const int b = at / a.c.heads, head = at - b * a.c.heads, n = a.c.length(b);
+  const int b = at / a.c.heads, head = at - b * a.c.heads;
+  const Parts parts = att_parts(a, b, head, lane);
+  const int n = parts.n, j = block * 256 + tid;
   if (block * 256 >= n) return;
-  const int used = (n + a.chunk - 1) / a.chunk, j = block * 256 + tid;
   const long long bh0 = static_cast<long long>(b) * a.hq + head * a.group;
-  const float2* ml = reinterpret_cast<const float2*>(a.ml) + bh0 * a.splits;
   const float* logits = a.logits + bh0 * a.logit_stride + j;
   float sum = 0.f;
   for (int g0 = 0; g0 < a.group; g0 += 64) {
     const int some = min(64, a.group - g0);
     for (int i = wave; i < some; i += 4) {
-      float mx = ATT_LOW, total = 0.f;
-      for (int c = lane; c < used; c += 64) mx = fmaxf(mx, ml[(g0 + i) * a.splits + c].x);
-      mx = wave_max(mx, lane);
-      for (int c = lane; c < used; c += 64) {
-        const float2 v = ml[(g0 + i) * a.splits + c];
-        total = __builtin_fmaf(v.y, exp2f(v.x - mx), total);
+      float mx = ATT_LOW, inv;
+      if (parts.used == 1) {
+        const float2 v = reinterpret_cast<const float2*>(a.total)[bh0 + g0 + i];
+        mx = v.x;
+        inv = v.y;
+      } else {
+        const auto ml = [&](int p) { return reinterpret_cast<const float2*>(a.ml)[parts.at(p) * a.group + g0 + i]; };
+        for (int p = lane; p < parts.used; p += 64) mx = fmaxf(mx, ml(p).x);
+        mx = wave_max(mx, lane);
+        float total = 0.f;
+        for (int p = lane; p < parts.used; p += 64) {
+          const float2 v = ml(p);
+          total = __builtin_fmaf(v.y, exp2f(v.x - mx), total);
+        }
+        total = wave_sum(total, lane);
+        inv = total == 0.f ? 0.f : 1.0f / total;
       }
-      total = wave_sum(total, lane);
       if (lane == 0) {
         s_m[i] = mx;
-        s_inv[i] = total == 0.f ? 0.f : 1.0f / total;
+        s_inv[i] = inv;
       }
     }
     __syncthreads();

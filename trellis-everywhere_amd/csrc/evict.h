@@ -43,17 +43,6 @@ __device__ __forceinline__ uint32_t ev_key(float score) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Inclusive sum over the wave's lanes up to this one (DPP row shifts, then row broadcasts).
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
-  return v;
-}
-
 __device__ __forceinline__ void ev_move(const EvictArgs& a, int b, int head, int from, int from_page, int to, int to_page,
                                         int sub) {
   if (from_page < 0 || to_page < 0) return;

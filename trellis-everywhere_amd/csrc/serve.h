@@ -109,6 +109,17 @@ __device__ __forceinline__ float wave_max(float v, int lane) {
   return fmaxf(v, lane_xor<32>(v, lane));
 }
 
+// Inclusive sum over the wave's lanes up to this one (DPP row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // The sum over aligned groups of n lanes (a power of 2 up to 64).
 __device__ __forceinline__ float group_sum(float v, int n, int lane) {
   if (n > 1) v += lane_xor<1>(v, lane);
@@ -118,6 +129,13 @@ __device__ __forceinline__ float group_sum(float v, int n, int lane) {
   if (n > 16) v += lane_xor<16>(v, lane);
   if (n > 32) v += lane_xor<32>(v, lane);
   return v;
+}
+
+// A load of what no kernel of the call writes: where the address is the same in every lane, by the scalar unit (from
+// plain memory the compiler does that only if nothing the kernel stores could be there).
+template <class T>
+__device__ __forceinline__ T load_const(const T* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p));
 }
 
 // A paged cache (struct trellis_kv_cache). Offsets in elements, 64-bit: a cache passes 2^31 elements.
@@ -134,11 +152,11 @@ struct Cache {
   // tokens of row b that a call sees: the row's length within what the call and its table can hold
   __device__ __forceinline__ int length(int b) const {
     const int cap = min(static_cast<long long>(max_len), static_cast<long long>(width) << page_shift);
-    return max(0, min(lens[b], cap));
+    return max(0, min(load_const(lens + b), cap));
   }
   // the page of logical slot j of row b (j within the table), or -1 where the table holds no page
   __device__ __forceinline__ int page_of(int b, int j) const {
-    const int id = table[b * table_stride + (j >> page_shift)];
+    const int id = load_const(table + b * table_stride + (j >> page_shift));
     return static_cast<unsigned>(id) < static_cast<unsigned>(pages) ? id : -1;
   }
   __device__ __forceinline__ int in_page(int j) const { return j & ((1 << page_shift) - 1); }

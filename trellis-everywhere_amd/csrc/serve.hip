@@ -125,9 +125,10 @@ void launch_append(const AppendArgs& a, bool vec, int lpr, int rounds, int parts
 // ---------------------------------------------------------------- attention
 
 struct AttendPlan {
-  int splits, row_blocks, chunk;
+  int aim, chunk, row_blocks;
+  int64_t items;
   int64_t logit_stride;
-  size_t off_ml, off_logits, ws;
+  size_t off_ml, off_total, off_logits, ws;
 };
 
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -136,33 +137,38 @@ AttendPlan attend_plan(const trellis_kv_cache* c, int q_heads, bool accumulate) 
   AttendPlan p;
   const int n = longest(c), group = q_heads / c->heads;
   p.row_blocks = (group + 15) / 16;
-  const int64_t one = static_cast<int64_t>(c->rows) * c->heads * p.row_blocks;
-  // One chunk up to 512 tokens (400 of 8 heads: 8.4 us either way, and a launch less). Above, chunks for two
-  // workgroups per CU where there is one row, for four where there are several, as of uneven lengths about half are
-  // empty (16 rows up to 4099 tokens for two / four: 43.1 / 38.2 us). Of one tile a wave at least (one row of 4000
-  // tokens of 8 heads in chunks of 128 / 256 / 512: 11.4 / 13.7 / 14.4 us; 32717: 35.6 / 32.9 / 31.1, and 38.9 in
-  // 2048), two for several rows (8 of 2000 in 128 / 256 / 512: 19.0 / 17.5 / 17.9); and 4096 tokens at most, for rows of
-  // uneven lengths (64 up to 8192 in 4096 / 8192: 232 / 241; where all are 4096 long, 2048 / 4096: 197 / 188).
-  int64_t splits = 1;
-  if (n > 512 && one > 0) {
-    const int64_t want = ((c->rows == 1 ? 2LL : 4LL) * device_cus() + one - 1) / one;
-    const int64_t shortest = c->rows == 1 ? ATT_CHUNK_MIN : 2 * ATT_CHUNK_MIN;
-    const int64_t least = (n + 4095) / 4096, most = (n + shortest - 1) / shortest;
-    splits = want > least ? want : least;
-    if (splits > most) splits = most;
-    if (splits > ATT_SPLITS) splits = ATT_SPLITS;
+  const int64_t one = static_cast<int64_t>(c->rows) * c->heads;
+  // One chunk a row up to 512 tokens (400 of 8 heads: 8.4 us either way, and a launch less), and beyond 512 rows.
+  // Otherwise chunks for two workgroups per CU, one where the head dim's registers leave room for no more (16 rows up
+  // to 4096 tokens of 2 heads of 256: 30.6 -> 26.5 us): a row's own are planned here (4000 tokens of 8 heads in
+  // chunks of 128 / 256 / 512: 11.4 / 13.7 / 14.4 us; 32717: 35.6 / 32.9 / 31.1, and 38.9 in 2048), those of several
+  // on the GPU (att_chunk).
+  p.aim = p.chunk = 0;
+  p.items = one;
+  if (n > 512 && c->rows <= 512 && one > 0) {
+    const int64_t units = one * att_units(n);
+    // no row may have more than ATT_PARTS chunks
+    const int64_t cap = static_cast<int64_t>(ATT_PARTS - 1) * c->heads / (c->rows == 1 ? 1 : 4);
+    int64_t aim = (c->head_dim > 128 ? 1 : 2) * device_cus() / p.row_blocks;
+    if (aim > cap) aim = cap;
+    p.aim = aim < 1 ? 1 : static_cast<int>(aim);
+    if (c->rows == 1) {
+      p.chunk = static_cast<int>((units + p.aim - 1) / p.aim) * ATT_UNIT;
+      p.items = static_cast<int64_t>((n + p.chunk - 1) / p.chunk) * c->heads;
+    } else {
+      const int64_t many = units / ATT_LONG < 4 * aim ? units / ATT_LONG : 4 * aim;
+      // (and every row and head one that is not full)
+      p.items = (many > p.aim ? many : p.aim) + one;
+      if (p.items > units) p.items = units;
+    }
   }
-  p.chunk = static_cast<int>(((n + splits - 1) / splits + ATT_CHUNK_MIN - 1) / ATT_CHUNK_MIN * ATT_CHUNK_MIN);
-  if (p.chunk < ATT_CHUNK_MIN) p.chunk = ATT_CHUNK_MIN;
-  p.splits = n > 0 ? (n + p.chunk - 1) / p.chunk : 1;
   const size_t bh = static_cast<size_t>(c->rows) * q_heads;
   p.logit_stride = (static_cast<int64_t>(n) + 31) / 32 * 32;
-  size_t ws = p.splits > 1 ? up256(bh * p.splits * c->head_dim * 4) : 0;
-  p.off_ml = ws;
-  if (p.splits > 1 || accumulate) ws += up256(bh * p.splits * 8);
-  p.off_logits = ws;
-  if (accumulate) ws += up256(bh * p.logit_stride * 4);
-  p.ws = ws;
+  const size_t slots = p.aim ? static_cast<size_t>(p.items) * group : 0;
+  p.off_ml = up256(slots * c->head_dim * 4);
+  p.off_total = p.off_ml + up256(slots * 8);
+  p.off_logits = p.off_total + (accumulate ? up256(bh * 8) : 0);
+  p.ws = p.off_logits + (accumulate ? up256(bh * p.logit_stride * 4) : 0);
   return p;
 }
 
@@ -411,19 +417,24 @@ int trellis_paged_attention(const trellis_kv_cache* cache, const void* q, int64_
   a.hq = q_heads;
   a.group = q_heads / cache->heads;
   a.row_blocks = p.row_blocks;
-  a.splits = p.splits;
+  a.aim = p.aim;
   a.chunk = p.chunk;
+  a.items = static_cast<int>(p.items);
   a.scale = scale * 1.44269504088896340736f;
   a.part = reinterpret_cast<float*>(ws);
-  a.ml = p.splits > 1 || accumulate ? reinterpret_cast<float*>(ws + p.off_ml) : nullptr;
+  a.ml = reinterpret_cast<float*>(ws + p.off_ml);
+  a.total = accumulate ? reinterpret_cast<float*>(ws + p.off_total) : nullptr;
   a.logits = accumulate ? reinterpret_cast<float*>(ws + p.off_logits) : nullptr;
   a.logit_stride = p.logit_stride;
   a.c = cache_of(cache);
-  const int64_t one = static_cast<int64_t>(cache->rows) * cache->heads;
-  const int64_t blocks = (one * p.splits + 7) / 8 * 8 * p.row_blocks, bh = static_cast<int64_t>(cache->rows) * q_heads;
-  const int64_t joins = p.splits > 1 ? bh : 0;
+  const int64_t one = static_cast<int64_t>(cache->rows) * cache->heads, bh = static_cast<int64_t>(cache->rows) * q_heads;
+  const int64_t blocks = (p.items + 7) / 8 * 8 * p.row_blocks;
+  const int64_t joins = p.aim ? bh : 0;
   const int64_t finish = joins + (accumulate ? one * ((longest(cache) + 255) / 256) : 0);
-  if (!grid_fits(blocks, 64 * ATT_WAVES) || !grid_fits(finish, 256)) return TRELLIS_ERR_BATCH;
+  // (chunks count the units of all rows and heads in 32 bits)
+  if (!grid_fits(blocks, 64 * ATT_WAVES) || !grid_fits(finish, 256) ||
+      one * ((longest(cache) + ATT_UNIT - 1) / ATT_UNIT) >= (int64_t(1) << 31))
+    return TRELLIS_ERR_BATCH;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool exact = q_dtype != cache->dtype || out_dtype == TRELLIS_F32;
   const bool nt = attend_streams(cache, p);
