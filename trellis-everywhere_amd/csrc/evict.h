@@ -159,10 +159,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
       if (segs > 1) load(seg);
       each(seg, [&](int, int, uint32_t k) {
         const uint32_t u = k - lo;
-        if (bits >= 32 || (u >> bits) == (prefix >> bits)) {
-          const int bin = (u >> shift) & ((1u << (bits - shift)) - 1);
-          atomicAdd(&hist[now][bin], 1);
-        }
+        if (bits >= 32 || (u >> bits) == (prefix >> bits)) atomicAdd(&hist[now][(u >> shift) & ((1u << (bits - shift)) - 1)], 1);
       });
     }
     __syncthreads();
@@ -256,9 +253,9 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
     ranks(kept, rank, kept_before);
     if (below < 0 && keep < (seg + 1) * SEG) {
       // (keep < n: the token of slot `keep` is in this segment)
-      each(seg, [&](int number, int j, uint32_t) {
-        if (j == keep) s_left = rank[number >> 2] + lower(kept, number);
-      });
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+        if (token(seg, i) == (keep & ~3)) s_left = rank[i] + lower(kept, 4 * i + (keep & 3));
       __syncthreads();
       below = s_left;
     }
