@@ -31,8 +31,9 @@ struct AppendArgs {
 // power of 2) a head, so the token's row, slot, page and angles are found once. A lane holds 8 dims of its
 // head: the rotary dims as 4 of the first half and their 4 partners of the second (nothing to exchange), the
 // others 8 in a row. VEC: every row of q, k and v is 16-byte aligned.
+// NT: nontemporal stores.
 // Bound: APPEND_FIGURES.
-template <class TX, class TC, bool VEC>
+template <class TX, class TC, bool VEC, bool NT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int lpr, int rounds, int parts) {
   const int lane = threadIdx.x & 63, sub = threadIdx.x & (lpr - 1), group = threadIdx.x / lpr, groups = 256 / lpr;
   const int heads = a.hq + 2 * a.c.heads, d = a.c.d;
@@ -106,12 +107,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int lpr, int 
       // a token without a slot (padding) gets zeros
       if (!live) x = y = float4_t{0.f, 0.f, 0.f, 0.f};
       const long long at = (static_cast<long long>(t) * a.hq + head) * d;
-      store4_dt(a.q_out, at + d0, a.q_dt, x);
-      store4_dt(a.q_out, at + d1, a.q_dt, y);
+      store4_dt<NT>(a.q_out, at + d0, a.q_dt, x);
+      store4_dt<NT>(a.q_out, at + d1, a.q_dt, y);
     } else if (live) {
       TC* dst = static_cast<TC*>(kind == 1 ? a.c.k : a.c.v) + a.c.row_at(page, head, slot);
-      store4(dst + d0, x);
-      store4(dst + d1, y);
+      store4<NT>(dst + d0, x);
+      store4<NT>(dst + d1, y);
       if (kind == 1 && sub == 0) {
         const long long p = a.c.slot_at(page, head, slot);
         if (a.c.scores) a.c.scores[p] = 0.f;

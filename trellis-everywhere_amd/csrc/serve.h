@@ -68,19 +68,22 @@ __device__ __forceinline__ float4_t load4(const T* p) {
   return v;
 }
 
-template <class T>
+// NT: a nontemporal store.
+template <bool NT = false, class T>
 __device__ __forceinline__ void store4(T* p, float4_t v) {
   typedef T vec_t __attribute__((ext_vector_type(4)));
   vec_t w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = static_cast<T>(v[i]);
-  *reinterpret_cast<vec_t*>(p) = w;
+  if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<vec_t*>(p));
+  else *reinterpret_cast<vec_t*>(p) = w;
 }
 
+template <bool NT = false>
 __device__ __forceinline__ void store4_dt(void* p, long long i0, int dt, float4_t v) {
-  if (dt == DT_F32) store4(static_cast<float*>(p) + i0, v);
-  else if (dt == DT_F16) store4(static_cast<_Float16*>(p) + i0, v);
-  else store4(static_cast<bf16_t*>(p) + i0, v);
+  if (dt == DT_F32) store4<NT>(static_cast<float*>(p) + i0, v);
+  else if (dt == DT_F16) store4<NT>(static_cast<_Float16*>(p) + i0, v);
+  else store4<NT>(static_cast<bf16_t*>(p) + i0, v);
 }
 
 __device__ __forceinline__ void store_dt(void* p, long long i, int dt, float v) {
