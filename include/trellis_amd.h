@@ -231,7 +231,8 @@ int trellis_residual_norm(const void *x, int64_t ldx, int x_dtype, const void *r
 typedef struct trellis_kv_cache {
   void *k, *v;               /* [pages][heads][page_size][head_dim] of `dtype`, 16-byte aligned */
   float *scores;             /* accumulated attention weight [pages][heads][page_size], or NULL */
-  int32_t *pos;              /* token positions [pages][heads][page_size], or NULL */
+  int32_t *pos;              /* token positions [pages][heads][page_size], or NULL (both 16-byte
+                              * aligned for the eviction) */
   const int32_t *table;      /* [rows][width] page ids, row stride table_stride */
   const int32_t *lens;       /* [rows] tokens per row */
   int64_t page_stride, head_stride, slot_stride;  /* of k and v, elements, multiples of 8 */
@@ -248,9 +249,9 @@ typedef struct trellis_kv_cache {
  *   starts: [rows + 1], tokens starts[b] .. starts[b+1]-1 belong to row b; NULL: token t is row t's
  *   lens counts these tokens already: the i-th of row b's n has slot lens[b] - n + i
  *   positions: [tokens], or NULL: the slots
- *   q_weight, k_weight: f32 [head_dim], both or neither: norm(x) = x * rsqrt(mean(x^2) + eps) * w
- *   cos, sin: f32 [n_positions][rot / 2], both or neither: pairs (i, i + rot/2) of the first rot
- *   dims are turned; a position outside the table makes them NaN
+ *   q_weight, k_weight: f32 [head_dim], 16-byte aligned, both or neither: norm(x) = x * rsqrt(mean(x^2) + eps) * w
+ *   cos, sin: f32 [n_positions][rot / 2], 16-byte aligned, both or neither: pairs (i, i + rot/2) of
+ *   the first rot dims are turned; a position outside the table makes them NaN
  * A token of no row, or whose slot the table does not hold, is not stored and its q' is 0. */
 int trellis_kv_append(const trellis_kv_cache *cache, const void *q, int64_t q_token_stride,
                       int64_t q_head_stride, const void *k, int64_t k_token_stride,
@@ -262,8 +263,10 @@ int trellis_kv_append(const trellis_kv_cache *cache, const void *q, int64_t q_to
 
 /* Attention of one new token per row: out[b][i] = sum_j p_j v_j, p = softmax over the row's tokens
  * of scale * q[b][i] . k_j, with key-value head i / (q_heads / heads). A row without tokens gives 0.
+ * Keys and values of a row's tokens are finite (another makes the row's heads NaN); memory of the
+ * pages past the row's last token is not looked at. The lengths are read on the GPU.
  *   q: [rows][q_heads][head_dim] of q_dtype, row and head strides in elements
- *   out: [rows][q_heads][head_dim] contiguous of out_dtype
+ *   out: [rows][q_heads][head_dim] contiguous of out_dtype, 16-byte aligned
  *   accumulate: also scores[token][heads] += the sum of p over the query heads of the key-value
  *   head (no page may then be in two rows' tables)
  * The workspace (trellis_attention_workspace_bytes, 256-byte aligned) needs no initialisation; it

@@ -35,7 +35,7 @@ def test_attention_codes(te):
     assert size(_cache(te), 3) == 19 and size(_cache(te), 0) == 19 and size(_cache(te, scores=None), 4, 1) == 1
     assert lib.trellis_attention_workspace_bytes(_cache(te), 4, 0, None) == 1
     assert size(_cache(te, max_len=1 << 20, width=1 << 16)) == 0 and n.value > 0
-    assert call(qd=3) == 9 and call(od=-1) == 9 and call(q=None) == 1 and call(out=None) == 1 and call(q=17) == 8
+    assert call(qd=3) == 9 and call(od=-1) == 9 and call(q=None) == 1 and call(out=None) == 1 and call(q=17) == 8 and call(out=24) == 8
     long = _cache(te, max_len=1 << 20, width=1 << 16)
     assert call(long) == 10 and call(long, ws=256, nb=16) == 10 and call(long, ws=264, nb=1 << 40) == 8
     assert call(_cache(te), acc=1) == 10

@@ -405,7 +405,7 @@ int trellis_paged_attention(const trellis_kv_cache* cache, const void* q, int64_
   if (cache->rows == 0) return TRELLIS_OK;
   if (!q || !out) return TRELLIS_ERR_NULL;
   const int qs = dtype_size(q_dtype);
-  if (!aligned(q, qs) || !aligned(out, dtype_size(out_dtype))) return TRELLIS_ERR_ALIGN;
+  if (!aligned(q, qs) || !aligned(out, 16)) return TRELLIS_ERR_ALIGN;
   const AttendPlan p = attend_plan(cache, q_heads, accumulate != 0);
   if (p.ws && (!workspace || ws_bytes < p.ws)) return TRELLIS_ERR_WORKSPACE;
   if (p.ws && !aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;

@@ -166,8 +166,10 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     max_len: the longest row the call has to expect; it plans the split over the length, and tokens past
         it are not seen. None: all that the table can hold. Give the batch's own bound where one is known.
     scores: each token's entry grows by the sum of its weights over the query heads of its head.
-    workspace: scratch for callers that keep it (a contiguous tensor of attention_workspace_bytes); None:
-        allocated for the call."""
+    Keys and values of a row's tokens have to be finite (another makes the row's heads NaN); what the pages hold
+    past them is not looked at.
+    workspace: scratch for a caller that keeps its own, any contiguous tensor on the device (too small a one raises
+        TRELLIS_ERR_WORKSPACE); None: taken from torch's allocator for the call."""
     refuse_grad(q)
     dev, c = _cache(k_pages, v_pages, scores, None, table, lens, max_len)
     rows, d = c.rows, c.head_dim
@@ -287,11 +289,14 @@ class PagedKVCache:
             self._upload_table()
         self.lengths = lengths
         self.seen = [p + c for p, c in zip(self.seen, counts)]
-        self._upload(self.lens, self.lengths)
-        self._upload(self.next_pos, self.seen)
         if all(c == 1 for c in counts):
-            self._starts, self._positions = None, self.next_pos - 1
+            # a decode step: nothing comes from the host
+            self.lens += 1
+            self._starts, self._positions = None, self.next_pos.clone()
+            self.next_pos += 1
         else:
+            self._upload(self.lens, self.lengths)
+            self._upload(self.next_pos, self.seen)
             starts = [0]
             for c in counts:
                 starts.append(starts[-1] + c)
