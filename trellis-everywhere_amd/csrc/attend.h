@@ -61,13 +61,14 @@ struct AttendArgs {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---- chunks. The lengths are on the GPU, so that is where the chunks of several rows are made: all of the same
-// number of units, ceil(units / aim) up to 6, above that so many that there are up to 4 aim of them (rows of uneven
-// lengths then end together), at least 2. The chunks of all rows lie in a line, rows slowest, heads fastest; a
+// number of units, ceil(units / aim) up to ATT_LONG, above that so many that there are up to 4 aim of them (rows of
+// uneven lengths then end together), at least 2. The chunks of all rows lie in a line, rows slowest, heads fastest; a
 // workgroup's number is its chunk's place in the line, and the place of its partial sums. Against chunks of one size
-// planned for the longest row: 16 rows up to 4099 tokens of 8 heads 39.3 -> 32.4 us, 64 up to 8192 228 -> 206, 4 up to
-// 8192 24.9 -> 18.4. (aim / 2 aim / 4 aim chunks of 32 rows up to 8192: 120 / 103 / 98 us; of 24 up to 4096, 6 units
-// each for aim: 43.0 / 45.1 / 45.0; of 32 up to 2048, 4 units: 36.1 / 36.5 / 36.4.)
-constexpr int ATT_LONG = 6;      // units of a chunk that more chunks are preferred to
+// planned for the longest row: 16 rows up to 4099 tokens of 8 heads 39.3 -> 32.4 us, 64 up to 8192 228 -> 203, 4 up to
+// 8192 24.9 -> 18.7. (aim, 2 aim, 4 aim chunks of 32 rows up to 8192: 120, 103, 98 us; of 24 up to 4096, 7 units each for
+// aim: 43, 45, 45; ATT_LONG of 6, 8, 10: those 24 rows 49.6, 43.0, 42.6, 48 rows up to 4096 85, 86, 90, 12 up to 8192 56,
+// 48, 48.)
+constexpr int ATT_LONG = 8;      // units of a chunk above which more chunks are preferred
 
 __host__ __device__ __forceinline__ int att_units(int n) { return (n + ATT_UNIT - 1) / ATT_UNIT; }
 
@@ -496,11 +497,15 @@ __device__ __forceinline__ void attend_join(const AttendArgs& a, long long bh) {
   };
   float4_t ahead[ATT_AHEAD];
 #pragma unroll
-  for (int i = 0; i < ATT_AHEAD; ++i) ahead[i] = part(min(mine ? grp + i * groups : 0, used - 1));
+  for (int i = 0; i < ATT_AHEAD; ++i)
+    if (i * groups < used) ahead[i] = part(min(mine ? grp + i * groups : 0, used - 1));
   float m[ATT_PARTS / 256], l[ATT_PARTS / 256], mx = ATT_LOW;
 #pragma unroll
   for (int i = 0; i < ATT_PARTS / 256; ++i) {
     const int p = tid + 256 * i;
+    m[i] = ATT_LOW;
+    l[i] = 0.f;
+    if (256 * i >= used) continue;
     float2 v = make_float2(ATT_LOW, 0.f);
     if (p < used) v = reinterpret_cast<const float2*>(a.ml)[parts.at(p) * a.group + in_group];
     m[i] = v.x;
