@@ -285,8 +285,8 @@ int trellis_paged_attention(const trellis_kv_cache *cache, const void *q, int64_
  * score and position move together. out_table NULL: in place (no page may be in two rows' tables).
  * Otherwise every kept token is copied to its slot of out_table's pages, which must not be among
  * the table's. new_lens[b] = min(length, keep); it must not be the cache's lens.
- * Workspace as for the attention. */
-int trellis_evict_workspace_bytes(const trellis_kv_cache *cache, int keep, size_t *bytes);
+ * Workspace as for the attention (apart: the call will have an out_table). */
+int trellis_evict_workspace_bytes(const trellis_kv_cache *cache, int keep, int apart, size_t *bytes);
 int trellis_kv_evict(const trellis_kv_cache *cache, int keep, int recent, const int32_t *next_pos,
                      const int32_t *out_table, int64_t out_table_stride, int out_width,
                      int32_t *new_lens, void *workspace, size_t ws_bytes, void *stream);

@@ -64,12 +64,16 @@ def test_append_codes(te):
 
 def test_evict_codes(te):
     lib, n = te.library(), ctypes.c_size_t(0)
-    call = lambda c=_cache(te), keep=4, recent=1, out=None, ow=0, new=16, ws=256, nb=1 << 20: \
+    # (up to 64 moves of a row and head need no workspace; here 100 can be, and an out table always needs one)
+    call = lambda c=_cache(te, width=32, max_len=512, table_stride=32), keep=100, recent=1, out=None, ow=0, new=16, ws=256, nb=1 << 20: \
         lib.trellis_kv_evict(c, keep, recent, None, out, 0, ow, new, ws, nb, None)
-    assert call(keep=0, recent=0) == 21 and call(recent=5) == 21 and call(recent=-1) == 21 and call(_cache(te, scores=None)) == 1
+    assert call(keep=0, recent=0) == 21 and call(recent=101) == 21 and call(recent=-1) == 21 and call(_cache(te, scores=None)) == 1
     assert call(_cache(te, pos=None)) == 1 and call(out=16, ow=0) == 20 and call(new=None) == 1 and call(new=512) == 12
     assert call(ws=None) == 10 and call(nb=8) == 10 and call(ws=264) == 8 and call(_cache(te, rows=0), new=None) == 0
-    assert lib.trellis_evict_workspace_bytes(_cache(te), 0, n) == 21 and lib.trellis_evict_workspace_bytes(_cache(te), 4, None) == 1
+    size = lib.trellis_evict_workspace_bytes
+    assert size(_cache(te), 0, 0, n) == 21 and size(_cache(te), 4, 0, None) == 1
+    assert size(_cache(te), 4, 0, n) == 0 and n.value == 0
+    assert size(_cache(te), 4, 1, n) == 0 and n.value > 0
 
 
 def test_norm_codes(te):

@@ -163,7 +163,7 @@ def load(path: str | None = None):
             ("trellis_kv_append", [C, P, L, L, P, L, L, P, L, L, I, I, I, P, P, P, P, F, P, P, I, I, P, I, P]),
             ("trellis_attention_workspace_bytes", [C, I, I, ctypes.POINTER(SZ)]),
             ("trellis_paged_attention", [C, P, L, L, I, I, F, I, P, I, P, SZ, P]),
-            ("trellis_evict_workspace_bytes", [C, I, ctypes.POINTER(SZ)]),
+            ("trellis_evict_workspace_bytes", [C, I, I, ctypes.POINTER(SZ)]),
             ("trellis_kv_evict", [C, I, I, P, P, L, I, P, P, SZ, P])):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, ctypes.c_int

@@ -252,15 +252,20 @@ void launch_evict_select(const EvictArgs& a, int n, bool fused, int lpr, unsigne
 }
 
 struct EvictPlan {
+  int most;       // the most moves a row and head can make
+  bool fused;     // few enough for the select kernel: no lists in the workspace
   size_t off_first, off_second, ws;
 };
 
-EvictPlan evict_plan(const trellis_kv_cache* c, int keep) {
+EvictPlan evict_plan(const trellis_kv_cache* c, int keep, bool apart) {
   EvictPlan p;
+  const int n = longest(c);
+  p.most = apart ? (keep < n ? keep : n) : n - keep < keep ? n - keep : keep;
+  p.fused = !apart && p.most <= EV_FUSED;
   const size_t bh = static_cast<size_t>(c->rows) * c->heads;
   p.off_first = up256(bh * 4);
   p.off_second = p.off_first + up256(bh * keep * 4);
-  p.ws = p.off_second + up256(bh * keep * 4);
+  p.ws = p.fused ? 0 : p.off_second + up256(bh * keep * 4);
   return p;
 }
 
@@ -449,11 +454,11 @@ int trellis_paged_attention(const trellis_kv_cache* cache, const void* q, int64_
   return launched();
 }
 
-int trellis_evict_workspace_bytes(const trellis_kv_cache* cache, int keep, size_t* bytes) {
+int trellis_evict_workspace_bytes(const trellis_kv_cache* cache, int keep, int apart, size_t* bytes) {
   if (!bytes) return TRELLIS_ERR_NULL;
   const int v = validate_evict(cache, keep, 0);
   if (v) return v;
-  *bytes = evict_plan(cache, keep).ws;
+  *bytes = evict_plan(cache, keep, apart != 0).ws;
   return TRELLIS_OK;
 }
 
@@ -466,9 +471,9 @@ int trellis_kv_evict(const trellis_kv_cache* cache, int keep, int recent, const 
   if (cache->rows == 0) return TRELLIS_OK;
   if (!new_lens) return TRELLIS_ERR_NULL;
   if (new_lens == cache->lens) return TRELLIS_ERR_RANGE;
-  const EvictPlan p = evict_plan(cache, keep);
-  if (!workspace || ws_bytes < p.ws) return TRELLIS_ERR_WORKSPACE;
-  if (!aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
+  const EvictPlan p = evict_plan(cache, keep, out_table != nullptr);
+  if (p.ws && (!workspace || ws_bytes < p.ws)) return TRELLIS_ERR_WORKSPACE;
+  if (p.ws && !aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
   char* ws = static_cast<char*>(workspace);
   EvictArgs a;
   a.c = cache_of(cache);
@@ -483,17 +488,14 @@ int trellis_kv_evict(const trellis_kv_cache* cache, int keep, int recent, const 
   a.first = reinterpret_cast<int32_t*>(ws + p.off_first);
   a.second = reinterpret_cast<int32_t*>(ws + p.off_second);
   const int64_t bh = static_cast<int64_t>(cache->rows) * cache->heads;
-  // the most moves a head can make, in groups of the rows one workgroup moves, up to 64 workgroups a head
-  const int n = longest(cache);
-  const int most = out_table ? (keep < n ? keep : n) : n - keep < keep ? n - keep : keep;
+  // the moves in groups of the rows one workgroup moves, up to 64 workgroups a row and head
   const int lpr = lanes_per_row(cache->head_dim);
-  int blocks = most > 0 ? (most + 256 / lpr - 1) / (256 / lpr) : 0;
+  int blocks = p.most > 0 ? (p.most + 256 / lpr - 1) / (256 / lpr) : 0;
   if (blocks > 64) blocks = 64;
   if (!grid_fits(bh, 1024) || !grid_fits(bh * blocks, 256)) return TRELLIS_ERR_BATCH;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool fused = !out_table && most <= EV_FUSED;
-  launch_evict_select(a, n, fused, lpr, static_cast<unsigned>(bh), st);
-  if (blocks > 0 && !fused)
+  launch_evict_select(a, longest(cache), p.fused, lpr, static_cast<unsigned>(bh), st);
+  if (blocks > 0 && !p.fused)
     hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(bh * blocks)), dim3(256), 0, st, a, lpr, blocks);
   return launched();
 }

@@ -222,7 +222,7 @@ def evict_kv(k_pages, v_pages, scores, pos, table, lens, keep: int, recent: int,
             raise ValueError(f"out_table must be int32 [{c.rows}, width] with unit column stride on {k_pages.device}")
         o_ptr, o_stride, o_width = out_table.data_ptr(), out_table.stride(0), out_table.shape[1]
     lib, need = _capi.load(), ctypes.c_size_t(0)
-    st = lib.trellis_evict_workspace_bytes(c, keep, need)
+    st = lib.trellis_evict_workspace_bytes(c, keep, 0 if out_table is None else 1, need)
     if st:
         _capi.check(st)
     new_lens = torch.empty_like(lens)
