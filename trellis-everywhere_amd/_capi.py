@@ -176,6 +176,29 @@ def load(path: str | None = None):
     return lib
 
 
+_serve = None
+
+
+def serve():
+    """The binding of the operators between the packed linears (_serve.so, csrc/bind.cpp), tied to the loaded library."""
+    global _serve
+    if _serve is None:
+        lib = load()
+        path = os.path.join(HERE, "_serve.so")
+        if not os.path.exists(path):
+            raise TrellisLibraryMissing(f"{path} is missing: build it with `python trellis-everywhere_amd/build.py`")
+        import importlib.util
+        import torch   # noqa: F401  (the binding links against torch's libraries, which this loads)
+        spec = importlib.util.spec_from_file_location("_serve", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "trellis_residual_norm", "trellis_kv_append", "trellis_attention_workspace_bytes", "trellis_paged_attention",
+            "trellis_evict_workspace_bytes", "trellis_kv_evict")])
+        _serve = module
+    return _serve
+
+
 def check(status: int) -> None:
     if status != 0:
         msg = load().trellis_strerror(status).decode()

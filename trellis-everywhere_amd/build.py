@@ -1,4 +1,4 @@
-"""Build the gfx950 HIP library libtrellis_amd.so in-tree with hipcc.
+"""Build the gfx950 HIP library libtrellis_amd.so in-tree with hipcc, and _serve.so, its binding for torch, with g++.
 
 Run as ``python trellis-everywhere_amd/build.py`` or through ``__graft_entry__.build()``.
 The .so lands next to this file so it travels with the source tree to the GPU box.
@@ -17,6 +17,10 @@ SOURCES = ["trellis_amd.hip", "kernels_k2.hip", "kernels_k3.hip", "kernels_k4.hi
 HEADERS = ["decode.h", "common.h", "gemv.h", "bgemm.h", "launch.h", "embed.h", "encode.h",
            "serve.h", "norm.h", "append.h", "attend.h", "evict.h"]
 
+# the Python side of the operators between the packed linears (host code against torch's C++ headers)
+BIND = "bind.cpp"
+BIND_LIB = os.path.join(HERE, "_serve.so")
+
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 FLAGS = [
@@ -31,8 +35,24 @@ FLAGS = [
 ]
 
 
+def bind_command(out: str) -> list[str]:
+    """The g++ line of the Python binding for the torch and the Python that run this."""
+    import sysconfig
+
+    import torch
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unused-function",
+            "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-I", os.path.join(ROOT, "include"), "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"),
+            "-isystem", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
+            "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, BIND), "-o", out,
+            "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every translation unit in parallel, then link the shared library."""
+    """Compile every translation unit in parallel, then link the shared library; the Python binding beside them."""
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
     inc = ["-I", os.path.join(ROOT, "include"), "-I", CSRC]
@@ -46,6 +66,10 @@ def build(verbose: bool = False) -> str:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                                             text=True)))
+    cmd = bind_command(BIND_LIB + ".tmp")
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    procs.append((BIND, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -53,7 +77,7 @@ def build(verbose: bool = False) -> str:
             failed.append(src)
             sys.stderr.write(out)
     if failed:
-        raise RuntimeError(f"hipcc failed for {failed}")
+        raise RuntimeError(f"the compiler failed for {failed}")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", LIB + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)
@@ -62,6 +86,7 @@ def build(verbose: bool = False) -> str:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"link failed ({res.returncode})")
     os.replace(LIB + ".tmp", LIB)
+    os.replace(BIND_LIB + ".tmp", BIND_LIB)
     return LIB
 
 

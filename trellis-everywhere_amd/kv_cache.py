@@ -1,7 +1,7 @@
 """A paged key-value cache and the attention that decodes from it (trellis_kv_append,
 trellis_paged_attention, trellis_kv_evict): what a decoder block runs between its q/k/v and its o linear
 (the reference's QKNORM, ROPE, cache copy and ATTN dispatches over one contiguous sequence,
-web/model.js:83-95). For serving: forward only.
+web/model.js:83-95). For serving: forward only. Arguments are checked in csrc/bind.cpp.
 
 append_kv, paged_attention and evict_kv work on tensors that the caller owns; PagedKVCache owns them.
 
@@ -14,93 +14,16 @@ append_kv, paged_attention and evict_kv work on tensors that the caller owns; Pa
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _capi
-from .norms import _DT, refuse_grad
-from .packed_linear import _raw_stream
-
-_CACHE_DT = {torch.float16: _capi.DT_F16, torch.bfloat16: _capi.DT_BF16}
 
 
-def _stream(index: int) -> int:
-    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
-
-
-
-def _cache(k_pages, v_pages, scores, pos, table, lens, max_len):
-    """(device index, C view of a cache: struct trellis_kv_cache), its arguments checked. (A small call's time is
-    mostly this: every attribute is read once, devices are compared by their index.)"""
-    dev, shape, strides, dtype = k_pages.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype
-    if dev < 0:
-        raise ValueError(f"the cache lives on a GPU, not {k_pages.device}")
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != strides or v_pages.dtype is not dtype:
-        raise ValueError("k_pages and v_pages must be [pages, heads, page_size, head_dim], alike in dtype and strides")
-    dt = _CACHE_DT.get(dtype)
-    if dt is None:
-        raise ValueError(f"cache dtype {dtype} must be float16 or bfloat16")
-    page_stride, head_stride, slot_stride, unit = strides
-    if unit != 1:
-        raise ValueError("k_pages and v_pages must have unit stride over head_dim")
-    if table.dtype is not torch.int32 or table.dim() != 2:
-        raise ValueError("table must be int32 [rows, width]")
-    (rows, width), (table_stride, unit) = table.shape, table.stride()
-    if unit != 1 and width != 1:
-        raise ValueError("table must have unit column stride")
-    if lens.dtype is not torch.int32 or lens.dim() != 1 or lens.shape[0] != rows or not lens.is_contiguous():
-        raise ValueError(f"lens must be a contiguous int32 [{rows}] tensor")
-    if v_pages.get_device() != dev or table.get_device() != dev or lens.get_device() != dev:
-        raise ValueError(f"k_pages, v_pages, table and lens must be on one device, {k_pages.device}")
-    s_ptr = p_ptr = None
-    if scores is not None:
-        if scores.dtype is not torch.float32 or scores.shape != shape[:3] or not scores.is_contiguous() or scores.get_device() != dev:
-            raise ValueError(f"scores must be a contiguous float32 {list(shape[:3])} tensor on {k_pages.device}")
-        s_ptr = scores.data_ptr()
-    if pos is not None:
-        if pos.dtype is not torch.int32 or pos.shape != shape[:3] or not pos.is_contiguous() or pos.get_device() != dev:
-            raise ValueError(f"pos must be a contiguous int32 {list(shape[:3])} tensor on {k_pages.device}")
-        p_ptr = pos.data_ptr()
-    pages, heads, page_size, d = shape
-    if max_len is None:
-        max_len = min(width * page_size, 1 << 30)
-    return dev, _capi.TrellisKVCache(
-        k_pages.data_ptr(), v_pages.data_ptr(), s_ptr, p_ptr, table.data_ptr(), lens.data_ptr(), page_stride, head_stride,
-        slot_stride, table_stride, pages, heads, page_size, d, dt, rows, width, max_len)
-
-
-def _dtype(name, dtype):
-    dt = _DT.get(dtype)
-    if dt is None:
-        raise ValueError(f"{name} dtype {dtype} must be float32, float16 or bfloat16")
-    return dt
-
-
-def _ints(name, t, n, dev):
-    if t is None:
-        return None
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.get_device() != dev:
-        raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor on the cache's device")
-    return t.data_ptr()
-
-
-def _floats(name, t, shape, dev):
-    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
-        raise ValueError(f"{name} must be a contiguous float32 {list(shape)} tensor on the cache's device")
-    return t.data_ptr()
-
-
-def _workspace(given, need, like):
-    """The call's scratch: the caller's, or a block of torch's allocator, which hands it on in stream order."""
-    if given is not None:
-        if given.device != like.device or not given.is_contiguous():
-            raise ValueError(f"workspace must be contiguous on {like.device}")
-        return given, given.data_ptr(), given.numel() * given.element_size()
-    if need == 0:
-        return None, None, 0
-    ws = torch.empty(need, dtype=torch.uint8, device=like.device)
-    return ws, ws.data_ptr(), need
+def _result(r):
+    """A call's result, or the error that its status names."""
+    if r.__class__ is int:
+        _capi.check(r)
+    return r
 
 
 def append_kv(q, k, v, k_pages, v_pages, table, lens, *, starts=None, positions=None, q_norm=None, k_norm=None,
@@ -117,43 +40,8 @@ def append_kv(q, k, v, k_pages, v_pages, table, lens, *, starts=None, positions=
     positions: int32 [tokens]; None: the slots (as long as nothing has been evicted).
     scores, pos: the new tokens' entries are set to 0 and to their positions.
     A token of no row, or whose slot the table does not hold (padding), is not stored and its q' is 0."""
-    refuse_grad(q, k, v, q_norm, k_norm)
-    dev, c = _cache(k_pages, v_pages, scores, pos, table, lens, None)
-    d, heads, rows = c.head_dim, c.heads, c.rows
-    if q.dim() != 3 or q.shape[2] != d:
-        raise ValueError(f"q must be [tokens, q_heads, {d}]")
-    tokens, hq, _ = q.shape
-    if k.shape != (tokens, heads, d) or v.shape != k.shape:
-        raise ValueError(f"k and v must be [{tokens}, {heads}, {d}]")
-    dt = q.dtype
-    if k.dtype is not dt or v.dtype is not dt or q.get_device() != dev or k.get_device() != dev or v.get_device() != dev:
-        raise ValueError(f"q, k and v must share a dtype on {k_pages.device}")
-    xdt = _dtype("q", dt)
-    (q_t, q_h, u), (k_t, k_h, x), (v_t, v_h, y) = q.stride(), k.stride(), v.stride()
-    if u != 1 or x != 1 or y != 1:
-        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-        (q_t, q_h, u), (k_t, k_h, x), (v_t, v_h, y) = q.stride(), k.stride(), v.stride()
-    if (q_norm is None) != (k_norm is None) or (cos is None) != (sin is None):
-        raise ValueError("q_norm and k_norm, and cos and sin, go together")
-    qw = kw = cp = sp = None
-    rot = n_pos = 0
-    if q_norm is not None:
-        qw, kw = _floats("q_norm", q_norm, (d,), dev), _floats("k_norm", k_norm, (d,), dev)
-    if cos is not None:
-        if cos.dim() != 2:
-            raise ValueError("cos and sin must be [positions, rotary dims / 2]")
-        n_pos, rot = cos.shape
-        cp, sp, rot = _floats("cos", cos, cos.shape, dev), _floats("sin", sin, cos.shape, dev), 2 * rot
-    s_ptr = None if starts is None else _ints("starts", starts, rows + 1, dev)
-    p_ptr = None if positions is None else _ints("positions", positions, tokens, dev)
-    odt = dt if q_dtype is None else q_dtype
-    out = torch.empty_like(q, dtype=odt) if q.is_contiguous() else torch.empty((tokens, hq, d), dtype=odt, device=q.device)
-    st = _capi.load().trellis_kv_append(
-        c, q.data_ptr(), q_t, q_h, k.data_ptr(), k_t, k_h, v.data_ptr(), v_t, v_h, xdt, tokens, hq, s_ptr, p_ptr, qw, kw,
-        eps, cp, sp, rot, n_pos, out.data_ptr(), _dtype("q'", odt), _stream(dev))
-    if st:
-        _capi.check(st)
-    return out
+    return _result(_capi.serve().append_kv(q, k, v, k_pages, v_pages, table, lens, starts, positions, q_norm, k_norm, eps,
+                                           cos, sin, scores, pos, q_dtype))
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = None, max_len: int | None = None,
@@ -170,33 +58,8 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     past them is not looked at.
     workspace: scratch for a caller that keeps its own, any contiguous tensor on the device (too small a one raises
         TRELLIS_ERR_WORKSPACE); None: taken from torch's allocator for the call."""
-    refuse_grad(q)
-    dev, c = _cache(k_pages, v_pages, scores, None, table, lens, max_len)
-    rows, d = c.rows, c.head_dim
-    if q.dim() != 3 or q.shape[0] != rows or q.shape[2] != d or q.get_device() != dev:
-        raise ValueError(f"q must be [{rows}, q_heads, {d}] on {k_pages.device}")
-    qdt = _dtype("q", q.dtype)
-    q_b, q_h, unit = q.stride()
-    if unit != 1:
-        q = q.contiguous()
-        q_b, q_h, unit = q.stride()
-    hq = q.shape[1]
-    if out is None:
-        odt = q.dtype if out_dtype is None else out_dtype
-        out = torch.empty_like(q, dtype=odt) if q.is_contiguous() else torch.empty((rows, hq, d), dtype=odt, device=q.device)
-    elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
-        raise ValueError(f"out must be a contiguous {list(q.shape)} tensor on {q.device}")
-    lib, need = _capi.load(), ctypes.c_size_t(0)
-    acc = 0 if scores is None else 1
-    st = lib.trellis_attention_workspace_bytes(c, hq, acc, need)
-    if st:
-        _capi.check(st)
-    ws, ws_ptr, ws_bytes = _workspace(workspace, need.value, q)
-    st = lib.trellis_paged_attention(c, q.data_ptr(), q_b, q_h, qdt, hq, d ** -0.5 if scale is None else scale, acc,
-                                     out.data_ptr(), _dtype("out", out.dtype), ws_ptr, ws_bytes, _stream(dev))
-    if st:
-        _capi.check(st)
-    return out
+    return _result(_capi.serve().paged_attention(q, k_pages, v_pages, table, lens, scale, max_len, scores, out, out_dtype,
+                                                 workspace))
 
 
 def evict_kv(k_pages, v_pages, scores, pos, table, lens, keep: int, recent: int, *, next_pos=None, out_table=None,
@@ -211,27 +74,8 @@ def evict_kv(k_pages, v_pages, scores, pos, table, lens, keep: int, recent: int,
         `table`), whose own stay as they are; None: in place, where no page may be in two rows' tables.
     Returns the new lengths min(lens, keep) as a new tensor; `lens` itself stays, for a model's other
     layers. Rows of up to `keep` tokens stay as they are."""
-    dev, c = _cache(k_pages, v_pages, scores, pos, table, lens, max_len)
-    if scores is None or pos is None:
-        raise ValueError("eviction goes by scores and pos")
-    n_ptr = None if next_pos is None else _ints("next_pos", next_pos, c.rows, dev)
-    o_ptr, o_stride, o_width = None, 0, 0
-    if out_table is not None:
-        if out_table.dtype is not torch.int32 or out_table.dim() != 2 or out_table.shape[0] != c.rows or \
-                (out_table.stride(1) != 1 and out_table.shape[1] != 1) or out_table.get_device() != dev:
-            raise ValueError(f"out_table must be int32 [{c.rows}, width] with unit column stride on {k_pages.device}")
-        o_ptr, o_stride, o_width = out_table.data_ptr(), out_table.stride(0), out_table.shape[1]
-    lib, need = _capi.load(), ctypes.c_size_t(0)
-    st = lib.trellis_evict_workspace_bytes(c, keep, 0 if out_table is None else 1, need)
-    if st:
-        _capi.check(st)
-    new_lens = torch.empty_like(lens)
-    ws, ws_ptr, ws_bytes = _workspace(workspace, need.value, k_pages)
-    st = lib.trellis_kv_evict(c, keep, recent, n_ptr, o_ptr, o_stride, o_width, new_lens.data_ptr(), ws_ptr, ws_bytes,
-                              _stream(dev))
-    if st:
-        _capi.check(st)
-    return new_lens
+    return _result(_capi.serve().evict_kv(k_pages, v_pages, scores, pos, table, lens, keep, recent, next_pos, out_table,
+                                          max_len, workspace))
 
 
 class PagedKVCache:
