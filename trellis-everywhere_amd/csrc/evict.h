@@ -159,7 +159,10 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
       if (segs > 1) load(seg);
       each(seg, [&](int, int, uint32_t k) {
         const uint32_t u = k - lo;
-        if (bits >= 32 || (u >> bits) == (prefix >> bits)) atomicAdd(&hist[now][(u >> shift) & ((1u << (bits - shift)) - 1)], 1);
+        // (the smallest key, which many tokens may share, such as no weight at all, is what is left of the count: adds
+        // to one address go one by one)
+        if (u != 0 && (bits >= 32 || (u >> bits) == (prefix >> bits)))
+          atomicAdd(&hist[now][(u >> shift) & ((1u << (bits - shift)) - 1)], 1);
       });
     }
     __syncthreads();
@@ -174,9 +177,16 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
     const int scan = wave_scan(sum);
     if (lane == 63) totals[wave] = scan;
     __syncthreads();
-    int before = scan - sum;
+    int before = scan - sum, counted = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) before += w < wave ? totals[w] : 0;
+    for (int w = 0; w < WAVES; ++w) {
+      before += w < wave ? totals[w] : 0;
+      counted += totals[w];
+    }
+    if (tid == THREADS - 1) {
+      h[BPT - 1] += equals - counted;
+      sum += equals - counted;
+    }
     if (before < left && before + sum >= left) {
 #pragma unroll
       for (int i = 0; i < BPT; ++i) {
