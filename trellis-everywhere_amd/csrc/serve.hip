@@ -2,7 +2,6 @@
 // launch planning and the dispatch to norm.h, append.h, attend.h and evict.h.
 #include <hip/hip_runtime.h>
 
-#include <cmath>
 #include <cstring>
 
 #include "trellis_amd.h"
@@ -180,7 +179,7 @@ AttendPlan attend_plan(const trellis_kv_cache* c, int q_heads, bool accumulate) 
 // where a second workgroup reads the same lines (more than 16 query heads a head; 64 over 2: 42 -> 51).
 bool attend_streams(const trellis_kv_cache* c, const AttendPlan& p) {
   const int64_t bytes = static_cast<int64_t>(c->rows) * longest(c) * c->heads * c->head_dim * 4;
-  return bytes >= (16 << 20) && p.row_blocks == 1 && c->head_dim % 64 == 0;
+  return bytes >= 16000000 && p.row_blocks == 1 && c->head_dim % 64 == 0;
 }
 
 template <class T, int DP, bool FULL, bool EXACT>
@@ -377,7 +376,7 @@ int trellis_kv_append(const trellis_kv_cache* cache, const void* q, int64_t q_to
   const int rounds = static_cast<int>((all + parts - 1) / parts);
   // prompts of 16 MB and more: what is written is not read again from the caches (6007 tokens of 48 heads of 128
   // 38.5 -> 30.5 us)
-  const bool nt = tokens * heads * cache->head_dim * 2 >= (16 << 20);
+  const bool nt = tokens * heads * cache->head_dim * 2 >= 16000000;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool f16 = cache->dtype == TRELLIS_F16;
   if (x_dtype == TRELLIS_F32) {

@@ -1,7 +1,7 @@
 """A paged key-value cache and the attention that decodes from it (trellis_kv_append,
 trellis_paged_attention, trellis_kv_evict): what a decoder block runs between its q/k/v and its o linear
 (the reference's QKNORM, ROPE, cache copy and ATTN dispatches over one contiguous sequence,
-web/model.js:83-95). For serving: forward only. Arguments are checked in csrc/bind.cpp.
+within web/model.js:77-102). For serving: forward only. Arguments are checked in csrc/bind.cpp.
 
 append_kv, paged_attention and evict_kv work on tensors that the caller owns; PagedKVCache owns them.
 

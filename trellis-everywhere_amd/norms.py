@@ -1,6 +1,6 @@
 """The norms around a decoder block with its residual (trellis_residual_norm): what runs between one
 packed linear's output and the next one's input (the reference's RMSNORM and ADD dispatches,
-web/model.js:79, 96-97, 101). For serving: forward only. Arguments are checked in csrc/bind.cpp.
+within web/model.js:77-102). For serving: forward only. Arguments are checked in csrc/bind.cpp.
 """
 from __future__ import annotations
 
