@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/ExpandUtils.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -82,8 +83,14 @@ double number(PyObject* o, const char* name) {
 
 int whole(PyObject* o, const char* name) {
   int overflow = 0;
-  const long long v = PyLong_Check(o) ? PyLong_AsLongLongAndOverflow(o, &overflow) : 0;
-  if (!PyLong_Check(o) || overflow || v < INT32_MIN || v > INT32_MAX) refuse("%s must be a whole number of 32 bits", name);
+  PyObject* index = PyNumber_Index(o);
+  const long long v = index ? PyLong_AsLongLongAndOverflow(index, &overflow) : 0;
+  if (!index) PyErr_Clear();
+  if (!index || overflow || v < INT32_MIN || v > INT32_MAX) {
+    Py_XDECREF(index);
+    refuse("%s must be a whole number of 32 bits", name);
+  }
+  Py_DECREF(index);
   return static_cast<int>(v);
 }
 
@@ -160,6 +167,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const float scale = static_cast<float>(number(a[5], "scale")), eps = static_cast<float>(number(a[6], "eps"));
     if (!on_gpu(x)) refuse("the norms run on a GPU");
     if (x.dim() == 0) refuse("x must have at least one dim");
+    const c10::DeviceGuard guard(x.device());   // launches go to the current device
     const int device = index_of(x), x_dt = dtype_code(x, "x");
     const at::ScalarType y_type = dtype_or(a[7], x, "out_dtype");
     const int64_t width = x.size(-1);
@@ -289,6 +297,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count(n, 17, "append_kv");
     const at::Tensor &q0 = tensor(a[0], "q"), &k0 = tensor(a[1], "k"), &v0 = tensor(a[2], "v");
     const CacheView w = cache_view(a[3], a[4], a[14], a[15], a[5], a[6], Py_None);
+    const c10::DeviceGuard guard(THPVariable_Unpack(a[3]).device());
     const int64_t d = w.c.head_dim;
     if (q0.dim() != 3 || q0.size(2) != d) refuse("q must be [tokens, q_heads, %d]", static_cast<int>(d));
     const int64_t tokens = q0.size(0), hq = q0.size(1);
@@ -336,6 +345,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count(n, 11, "paged_attention");
     const at::Tensor& q0 = tensor(a[0], "q");
     const CacheView w = cache_view(a[1], a[2], a[7], Py_None, a[3], a[4], a[6]);
+    const c10::DeviceGuard guard(THPVariable_Unpack(a[1]).device());
     const int64_t d = w.c.head_dim;
     if (q0.dim() != 3 || q0.size(0) != w.c.rows || q0.size(2) != d || q0.size(1) > INT32_MAX || !on_gpu(q0) || index_of(q0) != w.device)
       refuse("q must be [%d, q_heads, %d] on the cache's device", w.c.rows, static_cast<int>(d));
@@ -366,6 +376,7 @@ PyObject* evict_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     count(n, 12, "evict_kv");
     const CacheView w = cache_view(a[0], a[1], a[2], a[3], a[4], a[5], a[10]);
+    const c10::DeviceGuard guard(THPVariable_Unpack(a[0]).device());
     if (!w.c.scores || !w.c.pos) refuse("eviction goes by scores and pos");
     const int keep = whole(a[6], "keep"), recent = whole(a[7], "recent");
     const int32_t* next_pos = ints(a[8], "next_pos", w.c.rows, w.device);

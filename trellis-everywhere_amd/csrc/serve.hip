@@ -40,11 +40,16 @@ int device_cus() {
 
 // ---------------------------------------------------------------- residual norm
 
+// The fewest chunks of 8 a thread that 1024 threads cover a row with, and those threads.
+int norm_chunks(int width) { return width <= 8192 ? 1 : width <= 16384 ? 2 : 4; }
+int norm_threads(int width) {
+  const int per = 8 * norm_chunks(width);
+  return ((width + per - 1) / per + 63) / 64 * 64;
+}
+
 template <class TX, class TR>
 void launch_norm(const NormArgs& a, bool vec, int64_t rows, hipStream_t st) {
-  // the fewest chunks of 8 a thread that 1024 threads cover the row with
-  const int chunks = a.width <= 8192 ? 1 : a.width <= 16384 ? 2 : 4;
-  const int threads = ((a.width + 8 * chunks - 1) / (8 * chunks) + 63) / 64 * 64;
+  const int chunks = norm_chunks(a.width), threads = norm_threads(a.width);
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
   if (chunks == 1) {
     if (vec) hipLaunchKernelGGL((norm_kernel<TX, TR, true, 1>), grid, block, 0, st, a);
@@ -282,7 +287,7 @@ int trellis_residual_norm(const void* x, int64_t ldx, int x_dtype, const void* r
   if (!known_dtype(x_dtype) || !known_dtype(r_dtype) || !known_dtype(y_dtype)) return TRELLIS_ERR_DTYPE;
   if (rows == 0) return TRELLIS_OK;
   if (!x || !weight || !y) return TRELLIS_ERR_NULL;
-  if (!grid_fits(rows, 1024)) return TRELLIS_ERR_BATCH;
+  if (!grid_fits(rows, norm_threads(width))) return TRELLIS_ERR_BATCH;
   const int xs = dtype_size(x_dtype), rs = dtype_size(r_dtype), ys = dtype_size(y_dtype);
   if (!aligned(x, xs) || !aligned(y, ys) || (residual && !aligned(residual, rs)) || (h && !aligned(h, rs)) ||
       (gate && !aligned(gate, xs)) || !aligned(weight, 4) || (post_weight && !aligned(post_weight, 4)) ||
