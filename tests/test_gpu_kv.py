@@ -134,6 +134,25 @@ def test_attention(te, gpu_device, heads, group, d, page, x, cache, y):
     _attend(te, gpu_device, LENGTHS, heads, group, d, page, x, cache, y, seed=d + group)
 
 
+@pytest.mark.parametrize("heads,group,d,page", [(8, 4, 128, 64), (3, 3, 64, 16), (1, 17, 64, 32), (2, 40, 32, 128), (2, 2, 80, 32),
+                                                (1, 5, 96, 16), (2, 2, 256, 64), (1, 3, 136, 1024), (1, 1, 8, 16)])
+@pytest.mark.parametrize("x,cache,y", [(F16, F16, F16), (BF16, BF16, BF16), (F32, F16, F32), (F32, BF16, F32)])
+def test_attention_chunks_of_uneven_rows(te, gpu_device, heads, group, d, page, x, cache, y):
+    """Rows in several chunks (longer than 512 tokens), some in one, some empty."""
+    _attend(te, gpu_device, [0, 1300, 1, 513, 127, 0, 900], heads, group, d, page, x, cache, y, seed=d)
+    _attend(te, gpu_device, [1, 2049, 0], heads, group, d, page, x, cache, y, seed=d, scored=False, layout="sh")
+
+
+@pytest.mark.parametrize("rows,longest", [(65, 1400), (200, 900), (512, 600), (513, 600), (700, 40)])
+def test_attention_many_rows(te, gpu_device, rows, longest):
+    """More rows than a wave looks at at once, and more than are split at all."""
+    g = torch.Generator().manual_seed(rows)
+    lengths = torch.randint(0, longest, (rows,), generator=g).tolist()
+    lengths[0], lengths[63], lengths[-1] = longest, 0, longest
+    _attend(te, gpu_device, lengths, 1, 2, 16, 16, F16, F16, F32, seed=rows)
+    _attend(te, gpu_device, [0] * (rows - 1) + [longest], 2, 1, 8, 16, F16, F16, F16, seed=rows)
+
+
 @pytest.mark.parametrize("length", [1, 2, 100, 128, 129, 1000, 4097, 9001])
 def test_attention_split_over_one_row(te, gpu_device, length):
     """One row: every split of the length, and its join."""
@@ -205,9 +224,10 @@ def test_attention_infinite_logits(te, gpu_device):
     ref.close(got[1, :2], want[1, :2], F16, 1e-3)
 
 
-def test_attention_missing_pages(te, gpu_device):
+@pytest.mark.parametrize("first", [200, 1200])
+def test_attention_missing_pages(te, gpu_device, first):
     """Tokens on pages that do not exist count as absent; a row of only such tokens gives zeros."""
-    P = ref.Pages([200, 90, 20], 2, 16, 64, F16, 4)
+    P = ref.Pages([first, 90, 20], 2, 16, 64, F16, 4)
     P.table[0, 3], P.table[0, 6], P.table[1, 5] = -1, P.pages, 2 ** 31 - 1
     P.table[2] = -5
     q = torch.randn((3, 6, 64), generator=P.g).half()
@@ -218,9 +238,10 @@ def test_attention_missing_pages(te, gpu_device):
     assert float((scores.double().cpu() - want_scores).abs().max()) < 1e-3 and (got[2] == 0).all()
 
 
-def test_attention_shared_pages_and_repeats(te, gpu_device):
+@pytest.mark.parametrize("length", [300, 1700])
+def test_attention_shared_pages_and_repeats(te, gpu_device, length):
     """Rows may share pages (a common prefix) without scores; the same call twice is bit-identical."""
-    P = ref.Pages([300, 300], 2, 32, 128, F16, 6)
+    P = ref.Pages([length, length], 2, 32, 128, F16, 6)
     P.table[1, :5] = P.table[0, :5]
     q = torch.randn((2, 8, 128), generator=P.g).half()
     k, v, table, lens, _, _ = P.to(gpu_device)
@@ -296,6 +317,15 @@ def test_evict(te, gpu_device, values, apart, keep, recent):
     _evict(te, gpu_device, [0, 1, 16, 17, 33, 34, 64, 65, 201, 333], keep, recent, values=values, apart=apart, seed=keep)
 
 
+@pytest.mark.parametrize("values", ["spread", "ties", "equal"])
+def test_evict_very_long_rows(te, gpu_device, values):
+    """More tokens than the selection holds at once (32768), and the last lengths that it does."""
+    _evict(te, gpu_device, [33000], 20000, 100, heads=1, d=8, page=1024, values=values)
+    _evict(te, gpu_device, [33000, 70000], 3000, 0, heads=1, d=8, page=1024, values=values, apart=True)
+    _evict(te, gpu_device, [32768, 16385, 16384, 4097, 4096, 2048], 2040, 7, heads=1, d=8, page=1024, values=values)
+    _evict(te, gpu_device, [70000], 69990, 9, heads=1, d=8, page=1024, values=values)
+
+
 @pytest.mark.parametrize("values", ["spread", "ties", "odd"])
 def test_evict_long_rows(te, gpu_device, values):
     _evict(te, gpu_device, [5000, 2049, 1024], 1024, 100, heads=1, d=8, values=values)
@@ -330,11 +360,12 @@ def test_evict_max_len_bounds_what_is_seen(te, gpu_device):
 # ------------------------------------------------------------------ together
 
 
-def test_steps_in_a_graph_and_on_a_stream(te, gpu_device):
+@pytest.mark.parametrize("longest,keep", [(100, 50), (1400, 1000)])
+def test_steps_in_a_graph_and_on_a_stream(te, gpu_device, longest, keep):
     """append, attention with scores, eviction of one decode step captured in a HIP graph: every replay, with eager
     work between, equals the eager step on a copy of the same state."""
     dev = gpu_device
-    P = ref.Pages([60, 33, 1], 2, 16, 64, F16, 9, idle=0.0, room=40)
+    P = ref.Pages([60, 33, 1] if longest <= 512 else [longest - 40, 700, 1], 2, 16, 64, F16, 9, idle=0.0, room=40)
     state = P.to(dev)
     twin = [t.clone() for t in state]
     g = torch.Generator(device=dev).manual_seed(1)
@@ -344,8 +375,8 @@ def test_steps_in_a_graph_and_on_a_stream(te, gpu_device):
         k, v, table, lens, scores, pos = s
         lens.add_(1)
         q = te.append_kv(*x, k, v, table, lens, scores=scores, pos=pos)
-        out = te.paged_attention(q, k, v, table, lens, scores=scores, max_len=100, out_dtype=F32)
-        lens.copy_(te.evict_kv(k, v, scores, pos, table, lens, 50, 5, max_len=100))
+        out = te.paged_attention(q, k, v, table, lens, scores=scores, max_len=longest, out_dtype=F32)
+        lens.copy_(te.evict_kv(k, v, scores, pos, table, lens, keep, 5, max_len=longest))
         return out
 
     side = torch.cuda.Stream()
