@@ -72,6 +72,16 @@ def test_append(te, gpu_device, heads, group, d, rot, page, x, cache, qdt):
     _append(te, gpu_device, [0, 3, 1, 0, 70, 0], [4, 0, 31, 0, 15, 0], heads, group, d, page, x, cache, qdt, rot, False, seed=d + 1)
 
 
+def test_append_many_rows(te, gpu_device):
+    """More rows than a wave looks at at once, most of them with few tokens or none."""
+    g = torch.Generator().manual_seed(11)
+    for rows in (63, 64, 65, 200):
+        new = torch.randint(0, 4, (rows,), generator=g).tolist()
+        new[0], new[-1] = 0, 2
+        before = torch.randint(0, 40, (rows,), generator=g).tolist()
+        _append(te, gpu_device, new, before, 2, 2, 64, 16, F16, F16, F16, 64, True, seed=rows)
+
+
 def test_append_layouts(te, gpu_device):
     for x in (F32, F16):
         _append(te, gpu_device, [2, 0, 19], [5, 3, 7], 2, 4, 128, 16, x, F16, F16, 128, True, fused=True)

@@ -52,6 +52,14 @@ def test_rms_norm_shapes(te, gpu_device, x, shape):
         ref.close(got, want, x, _bound(want), "y")
 
 
+def test_many_rows(te, gpu_device):
+    a, res, w, _, _ = _inputs(70001, 24, F16, F32, 3)
+    want_y, want_h = ref.residual_norm(a, res, w)
+    y, h = te.residual_norm(a.to(gpu_device), res.to(gpu_device), w.to(gpu_device), out_dtype=F32)
+    ref.close(h, want_h, F32, _bound(want_h), "h")
+    ref.close(y, want_y, F32, 2 * _bound(want_y), "y")
+
+
 def test_gates_and_strides(te, gpu_device):
     """Gates broadcast per row, per column and whole; rows that are strided slices; odd addresses."""
     rows, width = 6, 264
