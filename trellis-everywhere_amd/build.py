@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtrellis_amd.so")
 SOURCES = ["trellis_amd.hip", "kernels_k2.hip", "kernels_k3.hip", "kernels_k4.hip", "serve.hip"]
 HEADERS = ["decode.h", "common.h", "gemv.h", "bgemm.h", "launch.h", "embed.h", "encode.h",
-           "serve.h", "norm.h", "append.h", "attend.h", "evict.h"]
+           "serve.h", "norm.h", "append.h", "attend_plan.h", "attend.h", "evict.h"]
 
 # the Python side of the operators between the packed linears (host code against torch's C++ headers)
 BIND = "bind.cpp"

@@ -29,6 +29,7 @@
 // its other workgroups turn the logits that this kernel left into weights.
 #pragma once
 
+#include "attend_plan.h"
 #include "serve.h"
 
 namespace trellis {
@@ -210,13 +211,13 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
   // ---- q: lane (head r16, dims 32 j + 8 g ..), in NQ terms of T; zeros for heads and dims that are none
   vec8 q[NQ][KS];
   float fold = a.scale;
-  const long long q_at = b * a.q_b + (h0 + (r16 < rows ? r16 : 0)) * a.q_h + 8 * g;
+  const long long q_at = b * a.q_b + (h0 + (r16 < rows ? r16 : 0)) * a.q_h;
   const auto is_q = [&](int j) { return r16 < rows && (FULL || 32 * j + 8 * g < d); };
   const auto load_q = [&](const auto* p, auto vec) {
     float f[KS][8];
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
-      const int off = FULL || 32 * j + 8 * g < d ? 32 * j : 0;
+      const int off = FULL ? 32 * j + 8 * g : att_q_dim(j, g, d);
       load8<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>, decltype(vec)::value>(p + q_at + off, f[j]);
     }
     if constexpr (EXACT) {
