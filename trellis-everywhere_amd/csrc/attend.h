@@ -34,10 +34,6 @@
 
 namespace trellis {
 
-constexpr int ATT_WAVES = 4;
-constexpr int ATT_TILE = 32;                          // tokens per tile
-constexpr int ATT_UNIT = ATT_TILE * ATT_WAVES;        // tokens per unit: a tile per wave
-constexpr int ATT_PARTS = 1024;                       // the most chunks of a row
 constexpr float ATT_LOW = -3.0e38f;                   // below every logit that counts
 constexpr float ATT_TOP = 11.f;                       // log2 of the weight at the maximum when it is set
 constexpr float ATT_SLACK = 4.f;                      // how far (log2) a logit may pass it
@@ -64,32 +60,19 @@ struct AttendArgs {
 // addresses made from it in two a lane).
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// ---- chunks. The lengths are on the GPU, so that is where the chunks of several rows are made: all of the same
-// number of units, ceil(units / aim) up to ATT_LONG, above that so many that there are up to 4 aim of them (rows of
-// uneven lengths then end together), at least 2. The chunks of all rows lie in a line, rows slowest, heads fastest; a
-// workgroup's number is its chunk's place in the line, and the place of its partial sums. Against chunks of one size
-// planned for the longest row: 16 rows up to 4099 tokens of 8 heads 39.3 -> 32.4 us, 64 up to 8192 228 -> 203, 4 up to
-// 8192 24.9 -> 18.7. (aim, 2 aim, 4 aim chunks of 32 rows up to 8192: 120, 103, 98 us; of 24 up to 4096, 7 units each for
-// aim: 43, 45, 45; ATT_LONG of 6, 8, 10: those 24 rows 49.6, 43.0, 42.6, 48 rows up to 4096 85, 86, 90, 12 up to 8192 56,
-// 48, 48.)
-constexpr int ATT_LONG = 8;      // units of a chunk above which more chunks are preferred
-
-__host__ __device__ __forceinline__ int att_units(int n) { return (n + ATT_UNIT - 1) / ATT_UNIT; }
-
 // Lengths of rows r0 .. r0 + 63, one a lane.
 __device__ __forceinline__ int att_lengths(const Cache& c, int r0, int lane) {
   const int b = r0 + lane, n = c.length(min(b, c.rows - 1));
   return b < c.rows ? n : 0;
 }
 
-// Units of a chunk (by a whole wave); `len0`: att_lengths of rows 0 .. 63.
+// Units of a chunk of several rows (by a whole wave); `len0`: att_lengths of rows 0 .. 63.
 __device__ __forceinline__ int att_chunk(const AttendArgs& a, int len0, int lane) {
   int units = 0;
   for (int r0 = 0; r0 < a.c.rows; r0 += 64)
     units += __builtin_amdgcn_readlane(wave_scan(att_units(r0 ? att_lengths(a.c, r0, lane) : len0)), 63);
   units *= a.c.heads;
-  const int even = (units + a.aim - 1) / a.aim;
-  return uniform(even <= ATT_LONG ? max(even, 2) : max((units + 4 * a.aim - 1) / (4 * a.aim), ATT_LONG));
+  return uniform(att_chunk_units(units, a.aim));
 }
 
 struct Place {

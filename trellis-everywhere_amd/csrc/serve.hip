@@ -129,9 +129,7 @@ void launch_append(const AppendArgs& a, bool vec, bool nt, int lpr, int rounds, 
 
 // ---------------------------------------------------------------- attention
 
-struct AttendPlan {
-  int aim, chunk, row_blocks;
-  int64_t items;
+struct AttendPlan : AttChunks {
   int64_t logit_stride;
   size_t off_ml, off_total, off_logits, ws;
 };
@@ -141,32 +139,7 @@ size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 AttendPlan attend_plan(const trellis_kv_cache* c, int q_heads, bool accumulate) {
   AttendPlan p;
   const int n = longest(c), group = q_heads / c->heads;
-  p.row_blocks = (group + 15) / 16;
-  const int64_t one = static_cast<int64_t>(c->rows) * c->heads;
-  // One chunk a row up to 512 tokens (400 of 8 heads: 8.4 us either way, and a launch less), and beyond 512 rows.
-  // Otherwise chunks for two workgroups per CU, one where the head dim's registers leave room for no more (16 rows up
-  // to 4096 tokens of 2 heads of 256: 30.6 -> 26.5 us): a row's own are planned here (4000 tokens of 8 heads in
-  // chunks of 128 / 256 / 512: 11.4 / 13.7 / 14.4 us; 32717: 35.6 / 32.9 / 31.1, and 38.9 in 2048), those of several
-  // on the GPU (att_chunk).
-  p.aim = p.chunk = 0;
-  p.items = one;
-  if (n > 512 && c->rows <= 512 && one > 0) {
-    const int64_t units = one * att_units(n);
-    // no row may have more than ATT_PARTS chunks
-    const int64_t cap = static_cast<int64_t>(ATT_PARTS - 1) * c->heads / (c->rows == 1 ? 1 : 4);
-    int64_t aim = (c->head_dim > 128 ? 1 : 2) * device_cus() / p.row_blocks;
-    if (aim > cap) aim = cap;
-    p.aim = aim < 1 ? 1 : static_cast<int>(aim);
-    if (c->rows == 1) {
-      p.chunk = static_cast<int>((units + p.aim - 1) / p.aim) * ATT_UNIT;
-      p.items = static_cast<int64_t>((n + p.chunk - 1) / p.chunk) * c->heads;
-    } else {
-      const int64_t many = units / ATT_LONG < 4 * aim ? units / ATT_LONG : 4 * aim;
-      // (and every row and head one that is not full)
-      p.items = (many > p.aim ? many : p.aim) + one;
-      if (p.items > units) p.items = units;
-    }
-  }
+  static_cast<AttChunks&>(p) = att_chunks(c->rows, c->heads, q_heads, c->head_dim, n, device_cus());
   const size_t bh = static_cast<size_t>(c->rows) * q_heads;
   p.logit_stride = (static_cast<int64_t>(n) + 31) / 32 * 32;
   const size_t slots = p.aim ? static_cast<size_t>(p.items) * group : 0;
