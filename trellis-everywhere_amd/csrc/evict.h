@@ -31,9 +31,10 @@ struct EvictArgs {
   int out_width;
   int keep, recent;
   int32_t* new_lens;          // [rows]
+  int list;                   // entries of a row and head's lists: min(keep, longest row)
   int32_t* count;             // workspace: [rows][heads] list lengths
-  int32_t* first;             // workspace: [rows][heads][keep]
-  int32_t* second;            // workspace: [rows][heads][keep]
+  int32_t* first;             // workspace: [rows][heads][list]
+  int32_t* second;            // workspace: [rows][heads][list]
 };
 // In place, entry r of the lists is the move second[r] -> first[r]. With an out table, entry j of `first` is
 // the source of slot j, or -1 - r: second[r].
@@ -80,8 +81,8 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
   const int n = a.c.length(b), keep = a.keep;
   const long long bh = blockIdx.x;
   if (tid == 0 && head == 0) a.new_lens[b] = min(n, keep);
-  int32_t* first = a.first + bh * keep;
-  int32_t* second = a.second + bh * keep;
+  int32_t* first = a.first + bh * a.list;
+  int32_t* second = a.second + bh * a.list;
   if (n <= keep) {
     // everything stays: nothing moves in place, all slots are copied to an out table
     if constexpr (!FUSED) {
@@ -307,8 +308,8 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, int lpr, i
   const int head = bh % a.c.heads, b = bh / a.c.heads;
   const int per = 256 / lpr, sub = threadIdx.x & (lpr - 1);
   const int count = a.count[bh];
-  const int32_t* first = a.first + bh * a.keep;
-  const int32_t* second = a.second + bh * a.keep;
+  const int32_t* first = a.first + bh * a.list;
+  const int32_t* second = a.second + bh * a.list;
   for (int r = (blockIdx.x % blocks) * per + threadIdx.x / lpr; r < count; r += blocks * per) {
     int src, dst, to;
     if (a.out_table) {

@@ -229,7 +229,8 @@ void launch_evict_select(const EvictArgs& a, int n, bool fused, int lpr, unsigne
 }
 
 struct EvictPlan {
-  int most;       // the most moves a row and head can make
+  int list;       // the most tokens of a row and head that are kept
+  int most;       // the most moves it can make
   bool fused;     // few enough for the select kernel: no lists in the workspace
   size_t off_first, off_second, ws;
 };
@@ -237,12 +238,13 @@ struct EvictPlan {
 EvictPlan evict_plan(const trellis_kv_cache* c, int keep, bool apart) {
   EvictPlan p;
   const int n = longest(c);
-  p.most = apart ? (keep < n ? keep : n) : n - keep < keep ? n - keep : keep;
+  p.list = keep < n ? keep : n;
+  p.most = apart ? p.list : n - keep < keep ? n - keep : keep;
   p.fused = !apart && p.most <= EV_FUSED;
   const size_t bh = static_cast<size_t>(c->rows) * c->heads;
   p.off_first = up256(bh * 4);
-  p.off_second = p.off_first + up256(bh * keep * 4);
-  p.ws = p.fused ? 0 : p.off_second + up256(bh * keep * 4);
+  p.off_second = p.off_first + up256(bh * p.list * 4);
+  p.ws = p.fused ? 0 : p.off_second + up256(bh * p.list * 4);
   return p;
 }
 
@@ -461,6 +463,7 @@ int trellis_kv_evict(const trellis_kv_cache* cache, int keep, int recent, const 
   a.keep = keep;
   a.recent = recent;
   a.new_lens = new_lens;
+  a.list = p.list;
   a.count = reinterpret_cast<int32_t*>(ws);
   a.first = reinterpret_cast<int32_t*>(ws + p.off_first);
   a.second = reinterpret_cast<int32_t*>(ws + p.off_second);
