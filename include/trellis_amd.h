@@ -284,7 +284,12 @@ int trellis_paged_attention(const trellis_kv_cache *cache, const void *q, int64_
  * slots; the others' slots take the kept tokens from above, both in ascending order. Key, value,
  * score and position move together. out_table NULL: in place (no page may be in two rows' tables).
  * Otherwise every kept token is copied to its slot of out_table's pages, which must not be among
- * the table's. new_lens[b] = min(length, keep); it must not be the cache's lens.
+ * the table's; keep is then at most the slots that out_table has, and every slot below the new
+ * length needs its page there (a token whose slot has none is lost).
+ * new_lens[b] = min(length, keep); it must not be the cache's lens.
+ * Tokens on pages that do not exist are absent: in place as many tokens are kept as there are slots
+ * below keep on pages that exist, and the others stay empty; into an out_table only the present
+ * tokens go, without gaps, and only they count for new_lens.
  * Workspace as for the attention (apart: the call will have an out_table). */
 int trellis_evict_workspace_bytes(const trellis_kv_cache *cache, int keep, int apart, size_t *bytes);
 int trellis_kv_evict(const trellis_kv_cache *cache, int keep, int recent, const int32_t *next_pos,

@@ -1,15 +1,18 @@
 // evict.h — eviction from a paged cache by accumulated attention weight. Per row b and key-value head, of
-// the n = length tokens (n > keep):
-//   kept: those with pos >= next_pos - recent, then the largest scores, `keep` in all; equal scores by
+// the n = length tokens, with `top` slots below which the kept ones end up:
+//   kept: those with pos >= next_pos - recent, then the largest scores, `top` in all; equal scores by
 //         the lowest slot (a NaN score counts as the largest);
-//   moved: a kept token below slot `keep` stays in its slot, and the slots that are not kept (holes) take
-//         the kept tokens from above `keep`, both in ascending order. Sources and holes are disjoint, so
+//   moved: a kept token below slot `top` stays in its slot, and the slots that are not kept (holes) take
+//         the kept tokens from above `top`, both in ascending order. Sources and holes are disjoint, so
 //         the moves of one head have no order among them.
-// In place only the moves are made; with an out table every kept token goes to its slot there.
+// In place only the moves are made, and top = keep (rows of up to keep tokens stay); with an out table every kept
+// token goes to its slot there, and top = min(keep, n, the table's slots).
+// A token on a page that does not exist is none: in place its slot is no hole, and as many tokens are kept as there
+// are slots below top; with an out table n counts the others alone, which close up.
 //
-// evict_select_kernel, one workgroup per (row, head): the keep-th largest key by 11-bit digits of the keys'
-// range (LDS histograms), then one scan in slot order that gives holes and sources their ranks: with c(j) the
-// kept tokens below slot j, a hole is the (j - c(j))-th, a source the (c(j) - c(keep))-th.
+// evict_select_kernel, one workgroup per (row, head): the smallest kept key by 11-bit digits of the keys'
+// range (LDS histograms), then one scan in slot order over the holes below `top` and the kept tokens above it, which
+// numbers both: holes first, so a source's rank less their count is the hole that it fills.
 // evict_move_kernel copies; a call whose rows can move EV_FUSED tokens at most copies in the first kernel.
 // Bound: the first kernel by its chain of dependent steps, the second by memory. 16 rows of 8 heads of 1025 tokens
 // 8.4 us (loads 1.6, three digits of 1.1 each, ranks 1.2, the move 0.8-1.1), with an out table 4 of up to 16000 14.2
@@ -78,19 +81,29 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
   __shared__ uint32_t s_lo[WAVES], s_hi[WAVES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int head = blockIdx.x % a.c.heads, b = blockIdx.x / a.c.heads;
-  const int n = a.c.length(b), keep = a.keep;
+  const bool apart = !FUSED && a.out_table;
+  const int n = a.c.length(b);
+  const int keep = apart ? min(static_cast<long long>(a.keep), static_cast<long long>(a.out_width) << a.c.page_shift) : a.keep;
   const long long bh = blockIdx.x;
-  if (tid == 0 && head == 0) a.new_lens[b] = min(n, keep);
   int32_t* first = a.first + bh * a.list;
   int32_t* second = a.second + bh * a.list;
+  const auto finish = [&](int len, int moves) {
+    if (tid != 0) return;
+    if (head == 0) a.new_lens[b] = len;
+    if constexpr (!FUSED) a.count[bh] = moves;
+  };
   if (n <= keep) {
-    // everything stays: nothing moves in place, all slots are copied to an out table
-    if constexpr (!FUSED) {
-      if (a.out_table)
-        for (int j = tid; j < n; j += THREADS) first[j] = j;
-      if (tid == 0) a.count[bh] = a.out_table ? n : 0;
+    // everything stays: nothing moves in place, all slots are copied to an out table (if all exist)
+    bool gap = false;
+    if (apart) {
+      for (int j = tid << a.c.page_shift; j < n; j += THREADS << a.c.page_shift) gap |= a.c.page_of(b, j) < 0;
+      gap = __syncthreads_or(gap);
     }
-    return;
+    if (!gap) {
+      if (apart)
+        for (int j = tid; j < n; j += THREADS) first[j] = j;
+      return finish(n, apart ? n : 0);
+    }
   }
   const int from = (a.next_pos ? a.next_pos[b] : n) - a.recent;
   const int segs = (n + SEG - 1) / SEG;
@@ -153,9 +166,28 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
     hi = max(hi, s_hi[w]);
   }
 
-  // ---- the keep-th largest key less lo, digit by digit; `left` of the tokens equal to it are kept
+  // ---- the slots that kept tokens end up in lie below `top`; `stay` of the tokens are kept. (Only a token without a
+  // page has a key of 0.)
+  int top = keep, stay = keep;
+  if (lo == 0) {
+    int there = 0;
+    for (int seg = 0; seg < segs; ++seg) {
+      if (segs > 1) load(seg);
+      each(seg, [&](int, int j, uint32_t k) { there += k != 0 && (apart || j < keep); });
+    }
+    there = wave_scan(there);
+    if (lane == 63) totals[wave] = there;
+    __syncthreads();
+    stay = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) stay += totals[w];
+    if (apart) top = stay = min(stay, keep);
+    if (stay == 0) return finish(apart ? 0 : keep, 0);
+  }
+
+  // ---- the smallest kept key less lo, digit by digit; `left` of the tokens equal to it are kept
   uint32_t prefix = 0;
-  int left = keep, equals = n, bits = hi > lo ? 32 - __builtin_clz(hi - lo) : 0;
+  int left = stay, equals = n, bits = hi > lo ? 32 - __builtin_clz(hi - lo) : 0;
   for (int now = 0; bits > 0 && left < equals; now ^= 1) {
     const int shift = max(bits - 11, 0);
     for (int seg = 0; seg < segs; ++seg) {
@@ -243,7 +275,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
     return __builtin_popcount((flags >> (number & ~3)) & ((1u << (number & 3)) - 1));
   };
 
-  int seen = 0, kept_before = 0, below = -1;   // below: c(keep)
+  int seen = 0, before = 0, holes = -1;
   for (int seg = 0; seg < segs; ++seg) {
     if (segs > 1) load(seg);
     uint32_t kept = 0, equal = 0;
@@ -263,33 +295,39 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
       equal = some;
     }
     kept |= equal;
-    ranks(kept, rank, kept_before);
-    if (below < 0 && keep < (seg + 1) * SEG) {
-      // (keep < n: the token of slot `keep` is in this segment)
+    // holes below `top`, kept tokens from there on
+    uint32_t moved = 0;
+    each(seg, [&](int number, int j, uint32_t k) {
+      const bool is = (kept >> number) & 1u;
+      if (j < top ? !is && (apart || k != 0) : is) moved |= 1u << number;
+    });
+    ranks(moved, rank, before);
+    if (holes < 0 && top < (seg + 1) * SEG) {
+      // (top < n: the token of slot `top` is in this segment)
 #pragma unroll
       for (int i = 0; i < G; ++i)
-        if (token(seg, i) == (keep & ~3)) s_left = rank[i] + lower(kept, 4 * i + (keep & 3));
+        if (token(seg, i) == (top & ~3)) s_left = rank[i] + lower(moved, 4 * i + (top & 3));
       __syncthreads();
-      below = s_left;
+      holes = s_left;
     }
     each(seg, [&](int number, int j, uint32_t) {
-      const bool is = (kept >> number) & 1u;
-      const int r = rank[number >> 2] + lower(kept, number);
-      if (j < keep) {
+      const bool is = (moved >> number) & 1u;
+      const int r = rank[number >> 2] + lower(moved, number);
+      if (j < top) {
         if constexpr (FUSED) {
-          if (!is) s_first[j - r] = j;
-        } else if (a.out_table) {
-          first[j] = is ? j : -1 - (j - r);
-        } else if (!is) {
-          first[j - r] = j;
+          if (is) s_first[r] = j;
+        } else if (apart) {
+          first[j] = is ? -1 - r : j;
+        } else if (is) {
+          first[r] = j;
         }
       } else if (is) {
-        if constexpr (FUSED) s_second[r - below] = j;
-        else second[r - below] = j;
+        if constexpr (FUSED) s_second[r - holes] = j;
+        else second[r - holes] = j;
       }
     });
   }
-  const int holes = keep - below;
+  finish(top, apart ? top : holes);
   if constexpr (FUSED) {
     __syncthreads();
     const int sub = tid & (lpr - 1);
@@ -297,8 +335,6 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
       const int src = s_second[r], dst = s_first[r];
       ev_move(a, b, head, src, a.c.page_of(b, src), dst, a.c.page_of(b, dst), sub);
     }
-  } else if (tid == 0) {
-    a.count[bh] = a.out_table ? keep : holes;
   }
 }
 

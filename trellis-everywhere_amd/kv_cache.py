@@ -72,6 +72,11 @@ def evict_kv(k_pages, v_pages, scores, pos, table, lens, keep: int, recent: int,
     next_pos: int32 [rows], positions each row has seen; None: its length (nothing evicted before).
     out_table: int32 [rows, width]: the kept tokens are copied to these pages instead (none of them in
         `table`), whose own stay as they are; None: in place, where no page may be in two rows' tables.
+        It needs a page for every slot below the new lengths; one with fewer slots than `keep` keeps what
+        it has slots for.
+    Tokens on pages that do not exist are absent. In place their slots stay empty, and as many tokens are
+    kept as there are slots below `keep` on pages that exist; into an out_table only the present tokens go,
+    without gaps, and the new lengths count them alone.
     Returns the new lengths min(lens, keep) as a new tensor; `lens` itself stays, for a model's other
     layers. Rows of up to `keep` tokens stay as they are."""
     return _result(_capi.serve().evict_kv(k_pages, v_pages, scores, pos, table, lens, keep, recent, next_pos, out_table,
