@@ -23,7 +23,8 @@
 //     stay below 2^15), checked by one ballot, so a tile costs no exchange between lane groups.
 // Precision: the weights enter their product as two terms of the cache's type (f16: 22 bits, their scale
 // keeping them out of its subnormals; bf16: 16 bits, three terms where q or out is fp32), the sums are fp32.
-// q of another type than the cache's is scaled by a power of 2 and split the same way.
+// q of another type than the cache's (or with an fp32 out) is scaled by a power of 2 and split the same way: into an
+// f16 cache 22 bits of each element down to 2^-17 of its row's largest, 2^-39 of that below.
 //
 // The chunks' results (maximum, sum, unnormalised out) meet in attend_finish_kernel, in a fixed order; with scores
 // its other workgroups turn the logits that this kernel left into weights.
@@ -136,6 +137,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
   constexpr bool BF = sizeof(T) == 2 && !std::is_same<T, _Float16>::value;
   constexpr int NQ = EXACT ? (BF ? 3 : 2) : 1;      // terms of q
   constexpr int NP = EXACT && BF ? 3 : 2;           // terms of the weights
+  constexpr int UP = BF ? 0 : 15;                   // log2 that q's largest element stays below
   constexpr int KS = DP / 32;                       // k-steps of the first product
   constexpr int DL = DP / 16;                       // dims per lane of V
   constexpr int VC = DL / 4;                        // 8-byte pieces of them
@@ -204,7 +206,8 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
       load8<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>, decltype(vec)::value>(p + q_at + off, f[j]);
     }
     if constexpr (EXACT) {
-      // the row's largest element to [0.5, 1), so that no term leaves the type's range
+      // the row's largest element to just below 2^UP, so that no term leaves the type's range: for f16 as high as it
+      // goes, as what the second term holds of the row's small elements lies near its subnormals
       float top = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j)
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
           top = fmaxf(top, fabsf(f[j][i]));
         }
       top = max_groups(top, lane);
-      const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+      const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) - UP : 0;
       fold = __builtin_ldexpf(fold, e);
 #pragma unroll
       for (int j = 0; j < KS; ++j)
