@@ -338,8 +338,10 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
     float top = s[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
-    if (__any(top > m + (ATT_TOP + ATT_SLACK))) {
-      const float to = fmaxf(m, max_groups(top, lane) - ATT_TOP);
+    if (__any(top - m > ATT_TOP + ATT_SLACK)) {
+      const float most = max_groups(top, lane);
+      float to = fmaxf(m, most - ATT_TOP);
+      if (most - to > ATT_TOP + ATT_SLACK) to = most;   // (of 2^27 and more that difference is rounded, up to 16)
       const float f = exp2f(m - to);
       m = to;
       l *= f;
