@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/ExpandUtils.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
@@ -63,6 +64,9 @@ const at::Tensor* optional_tensor(PyObject* o, const char* name) {
   const at::Tensor& t = THPVariable_Unpack(o);
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse("forward only: call it under torch.no_grad() or detach the inputs (%s wants a gradient)", name);
+  // (no_grad does not switch forward-mode differentiation off; its dual numbers are of one level)
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    refuse("forward only: unpack the dual tensor (%s carries a tangent)", name);
   return &t;
 }
 
