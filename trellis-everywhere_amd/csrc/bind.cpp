@@ -126,6 +126,15 @@ at::Tensor make(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& l
   return at::empty(sizes, like.options().dtype(dtype).requires_grad(false));
 }
 
+// A tensor that the call has written into: autograd counts such writes, so that a backward pass that saved the tensor
+// before them raises an error. (Inference tensors have no count.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject* o) {
+  if (o != Py_None) written(THPVariable_Unpack(o));
+}
+
 // Sizes and type of a tensor that has to be dense and on the device.
 void expect(const at::Tensor& t, const char* name, at::ScalarType dtype, at::IntArrayRef sizes, int device) {
   if (t.scalar_type() != dtype || t.sizes() != sizes || !t.is_contiguous() || !on_gpu(t) || index_of(t) != device)
@@ -217,6 +226,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                               weight.const_data_ptr<float>(), scale, eps, residual ? h2.data_ptr() : nullptr,
                               residual ? h2.stride(0) : 0, y.data_ptr(), width, dtype_code(y_type), rows,
                               static_cast<int>(std::min<int64_t>(width, INT32_MAX)), stream_of(device)));
+    if (residual) written(a[8]);
     if (!residual) return THPVariable_Wrap(std::move(y));
     PyObject* py = THPVariable_Wrap(std::move(y));
     PyObject* ph = a[8] == Py_None ? THPVariable_Wrap(std::move(h)) : Py_NewRef(a[8]);
@@ -339,6 +349,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           v.const_data_ptr(), v.stride(0), v.stride(1), x_dt, static_cast<int>(tokens), static_cast<int>(hq),
                           starts, positions, f32(qw), f32(kw), eps, f32(cos), f32(sin), rot, n_pos, out.data_ptr(),
                           dtype_code(out_type), stream_of(w.device)));
+    for (const int i : {3, 4, 14, 15}) written(a[i]);
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -371,6 +382,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Scratch ws(a[10], need, q0);
     check(entry.paged_attention(&w.c, q.const_data_ptr(), q.stride(0), q.stride(1), q_dt, hq, static_cast<float>(scale),
                                 accumulate, out.data_ptr(), out_dt, ws.p, ws.bytes, stream_of(w.device)));
+    for (const int i : {7, 8, 10}) written(a[i]);
     return given ? Py_NewRef(a[8]) : THPVariable_Wrap(std::move(out));
   });
 }
@@ -395,6 +407,7 @@ PyObject* evict_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Scratch ws(a[11], need, lens);
     check(entry.kv_evict(&w.c, keep, recent, next_pos, to ? to->const_data_ptr<int32_t>() : nullptr, to ? to->stride(0) : 0,
                          to ? static_cast<int>(to->size(1)) : 0, out.data_ptr<int32_t>(), ws.p, ws.bytes, stream_of(w.device)));
+    for (const int i : {0, 1, 2, 3, 11}) written(a[i]);
     return THPVariable_Wrap(std::move(out));
   });
 }
