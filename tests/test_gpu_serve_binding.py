@@ -57,3 +57,25 @@ def test_inference_tensors(te, gpu_device):
         te.paged_attention(q, k, v, table, lens, scores=scores)
         te.evict_kv(k, v, scores, pos, table, lens, 4, 1)
     assert (k[table[0, 2].item(), :, 7] == 0).all()
+
+
+def test_out_of_memory_is_torchs_error(te, gpu_device):
+    """An output or scratch that does not fit raises what torch raises, so that a caller can catch it."""
+    big = torch.zeros((1, 32768), dtype=F16, device=gpu_device).expand(1 << 18, 32768)     # 32 GiB of f32 out of 64 KiB
+    weight = torch.ones(32768, device=gpu_device)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.05)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            te.rms_norm(big, weight, out_dtype=F32)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert te.rms_norm(big[:2], weight).shape == (2, 32768)
+
+
+def test_transforms_are_refused(te, gpu_device):
+    x, w = torch.ones((2, 64), device=gpu_device), torch.ones(64, device=gpu_device)
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.vmap(lambda t: te.rms_norm(t, w))(x)
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(lambda t: te.rms_norm(t, w), (x,), (x,))

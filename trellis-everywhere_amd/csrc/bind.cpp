@@ -19,6 +19,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -150,8 +151,9 @@ PyObject* guarded(F f) {
     return nullptr;
   } catch (const Status& s) {
     return PyLong_FromLong(s.code);
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    // torch's own errors as torch raises them (out of memory among them)
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }
