@@ -52,7 +52,9 @@ def bind_command(out: str) -> list[str]:
 
 
 def build(verbose: bool = False) -> str:
-    """Compile every translation unit in parallel, then link the shared library; the Python binding beside them."""
+    """Compile every translation unit in parallel, then link the shared library; the Python binding beside them.
+    The library needs hipcc alone: it is in place before a failure of the binding is raised, and without torch the
+    binding, which only torch loads, is left out."""
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
     inc = ["-I", os.path.join(ROOT, "include"), "-I", CSRC]
@@ -66,18 +68,26 @@ def build(verbose: bool = False) -> str:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                                             text=True)))
-    cmd = bind_command(BIND_LIB + ".tmp")
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    procs.append((BIND, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    bind, missing = None, None
+    try:
+        cmd = bind_command(BIND_LIB + ".tmp")
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        bind = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    except (ImportError, OSError) as e:      # no torch, one that does not load, or no C++ compiler
+        if getattr(e, "name", None) == "torch":
+            print(f"no torch: {os.path.basename(BIND_LIB)} is not built", file=sys.stderr, flush=True)
+        else:
+            missing = e
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
         if p.returncode != 0:
             failed.append(src)
             sys.stderr.write(out)
+    bound = bind.communicate()[0] if bind else ""
     if failed:
-        raise RuntimeError(f"the compiler failed for {failed}")
+        raise RuntimeError(f"hipcc failed for {failed}")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", LIB + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)
@@ -86,7 +96,11 @@ def build(verbose: bool = False) -> str:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"link failed ({res.returncode})")
     os.replace(LIB + ".tmp", LIB)
-    os.replace(BIND_LIB + ".tmp", BIND_LIB)
+    if missing or (bind and bind.returncode != 0):
+        sys.stderr.write(bound)
+        raise RuntimeError(f"the library is built, its binding {BIND} is not") from missing
+    if bind:
+        os.replace(BIND_LIB + ".tmp", BIND_LIB)
     return LIB
 
 
