@@ -178,6 +178,8 @@ class PagedKVCache:
 
     def release(self, row: int) -> None:
         """The row's sequence has ended: its pages go back to the pool, the row is empty."""
+        if not 0 <= row < len(self.lengths):
+            raise ValueError(f"row must be in 0 .. {len(self.lengths) - 1}")
         self.seen[row] = 0
         self._upload(self.next_pos, self.seen)
         self._set_lengths([0 if b == row else n for b, n in enumerate(self.lengths)])
