@@ -111,6 +111,9 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))
         self._owned: list[list[int]] = [[] for _ in range(rows)]
         self._starts = self._positions = None
+        # rows that the last grow() gave tokens, on the device (None: all); lens of these and of the others
+        self._fed: torch.Tensor | None = None
+        self._lens_of: tuple[torch.Tensor, torch.Tensor] | None = None
 
     def _upload(self, dst: torch.Tensor, values) -> None:
         dst.copy_(torch.tensor(values, dtype=torch.int32))
@@ -138,8 +141,11 @@ class PagedKVCache:
             self._upload_table()
         self.lengths = lengths
         self.seen = [p + c for p, c in zip(self.seen, counts)]
+        self._fed, self._lens_of = None, None
+        if self.scores[0] is not None and not all(counts):
+            self._fed = torch.tensor([c > 0 for c in counts]).to(self.device)
         if all(c == 1 for c in counts):
-            # a decode step: nothing comes from the host
+            # a decode step: but for the table, where a row takes a page, nothing comes from the host
             self.lens += 1
             self._starts, self._positions = None, self.next_pos.clone()
             self.next_pos += 1
@@ -161,9 +167,19 @@ class PagedKVCache:
                          positions=self._positions, scores=self.scores[layer], pos=self.pos[layer], **rotary)
 
     def attend(self, layer: int, q, *, scale: float | None = None, out_dtype=None):
-        """paged_attention of one query token per row (a row without tokens gives zeros)."""
-        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, scale=scale,
-                               max_len=max(self.lengths), scores=self.scores[layer], out_dtype=out_dtype)
+        """paged_attention of one query token per row (a row without tokens gives zeros). An evictable cache adds the
+        weights to its scores, of the rows that the last grow() gave tokens: the others wait, and what is asked of
+        them meanwhile does not count."""
+        def ask(lens, scores):
+            return paged_attention(q, self.k[layer], self.v[layer], self.table, lens, scale=scale,
+                                   max_len=max(self.lengths), scores=scores, out_dtype=out_dtype)
+
+        if self._fed is None:
+            return ask(self.lens, self.scores[layer])
+        if self._lens_of is None:
+            self._lens_of = self.lens * self._fed, self.lens * ~self._fed
+        fed, waiting = self._lens_of
+        return ask(fed, self.scores[layer]).add_(ask(waiting, None))     # each row is empty in one of them
 
     def evict(self, keep: int, recent: int) -> None:
         """evict_kv of every layer, in place; the pages that the rows no longer fill go back to the pool."""
@@ -186,7 +202,7 @@ class PagedKVCache:
         self._upload(self.lens, self.lengths)
 
     def _set_lengths(self, lengths) -> None:
-        self._starts = self._positions = None
+        self._starts = self._positions = self._lens_of = None
         self.lengths, freed = lengths, False
         for own, n in zip(self._owned, lengths):
             while len(own) > -(-n // self.page_size):
