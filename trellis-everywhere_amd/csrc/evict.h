@@ -295,12 +295,14 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, int 
       equal = some;
     }
     kept |= equal;
-    // holes below `top`, kept tokens from there on
-    uint32_t moved = 0;
-    each(seg, [&](int number, int j, uint32_t k) {
-      const bool is = (kept >> number) & 1u;
-      if (j < top ? !is && (apart || k != 0) : is) moved |= 1u << number;
-    });
+    // holes below `top`, kept tokens from there on: a group's tokens below `top` flip
+    uint32_t moved = kept;
+#pragma unroll
+    for (int i = 0; i < G; ++i) moved ^= ((1u << min(max(top - token(seg, i), 0), 4)) - 1) << (4 * i);
+    if (lo == 0 && !apart)
+      each(seg, [&](int number, int j, uint32_t k) {
+        if (k == 0 && j < top) moved &= ~(1u << number);
+      });
     ranks(moved, rank, before);
     if (holes < 0 && top < (seg + 1) * SEG) {
       // (top < n: the token of slot `top` is in this segment)
