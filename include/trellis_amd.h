@@ -217,7 +217,8 @@ int trellis_encode_tiles(const float *w, uint32_t ntiles, int K, int codebook, u
  *   x: x_dtype, row stride ldx elements; gate: x_dtype, row stride ldg (0: one row for all),
  *   gate_inner 1, or 0 for one value per row; residual and h: r_dtype; y: y_dtype
  *   weight, post_weight: f32 [width]
- * h may be NULL (not wanted) or the residual itself; no other output may overlap an input. */
+ * h may be NULL (not wanted) or the residual itself; no other output may overlap an input. A launch
+ * holds less than 2^32 threads, one for up to 8 elements: more rows are TRELLIS_ERR_BATCH. */
 #define TRELLIS_NORM_MAX_WIDTH 32768
 int trellis_residual_norm(const void *x, int64_t ldx, int x_dtype, const void *residual,
                           int64_t ldr, int r_dtype, const void *gate, int64_t ldg, int gate_inner,

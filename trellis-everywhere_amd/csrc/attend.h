@@ -20,9 +20,10 @@
 //     group's 8 tokens (whole rows per 16 lanes) and transposes in its own registers (v_perm_b32);
 //   * both products leave the head on l % 16, so the running maximum and the sum are per-lane values.
 //     The maximum that the weights are taken against moves only when a logit passes it by 2^4 (the weights
-//     stay below 2^15), checked by one ballot, so a tile costs no exchange between lane groups.
+//     are at most 2^15), checked by one ballot, so a tile costs no exchange between lane groups.
 // Precision: the weights enter their product as two terms of the cache's type (f16: 22 bits, their scale
-// keeping them out of its subnormals; bf16: 16 bits, three terms where q or out is fp32), the sums are fp32.
+// keeping them out of its subnormals; bf16: 16 bits, of which a 16-bit out keeps 8 or 11, and three terms, 24 bits,
+// where q is of another type or out is fp32), the sums are fp32.
 // q of another type than the cache's (or with an fp32 out) is scaled by a power of 2 and split the same way: into an
 // f16 cache 22 bits of each element down to 2^-17 of its row's largest, 2^-39 of that below.
 //

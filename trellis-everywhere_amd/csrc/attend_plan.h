@@ -33,7 +33,9 @@ struct AttChunks {
   int64_t items;    // the most chunks that can be made
 };
 
-// One chunk a row up to 512 tokens (400 of 8 heads: 8.4 us either way, and a launch less), and beyond 512 rows.
+// One chunk a row up to 512 tokens (400 of 8 heads: 8.4 us either way, and a launch less), and beyond 512 rows, where
+// rows alone fill the CUs and every workgroup would look through all lengths (512 rows in chunks / 513 whole: of 1024
+// tokens of 8 heads 386 / 339 us, of up to 4096 tokens of 2 heads 213 / 226, one of 8192 among rows of 64 118 / 121).
 // Otherwise chunks for two workgroups per CU, one where the head dim's registers leave room for no more (16 rows up
 // to 4096 tokens of 2 heads of 256: 30.6 -> 26.5 us): a row's own are planned here (4000 tokens of 8 heads in
 // chunks of 128 / 256 / 512: 11.4 / 13.7 / 14.4 us; 32717: 35.6 / 32.9 / 31.1, and 38.9 in 2048), those of several

@@ -15,9 +15,11 @@
 // numbers both: holes first, so a source's rank less their count is the hole that it fills.
 // evict_move_kernel copies; a call whose rows can move EV_FUSED tokens at most copies in the first kernel.
 // Bound: the first kernel by its chain of dependent steps, the second by memory. 16 rows of 8 heads of 1025 tokens
-// 8.4 us (loads 1.6, three digits of 1.1 each, ranks 1.2, the move 0.8-1.1), with an out table 4 of up to 16000 14.2
-// (loads 3.4, a digit of all keys 2.3, of few 1.5, ranks 3.5) and the copies 8.4 (34 MB, 4.0 TB/s). With 8-bit
-// digits found by one thread and every step's keys read again: 47.8 and 92.7.
+// 8.5 us (loads 1.6, three digits of 1.1 each, ranks 1.2, the move 0.8-1.1), with an out table 4 of up to 16000 14.5
+// (loads 3.4, a digit of all keys 2.3, of few 1.5, ranks 3.5) and the copies 8.7 (34 MB, 3.9 TB/s); in place 4 of 16000
+// cut to 2048 17.5 and 11.6. A row of 32000, with 32 keys a thread, 28.0 and 6.3; of 100000, read again in segments for
+// each step, 122 and 9.5. With 8-bit digits found by one thread and every step's keys read again the first two took 47.8
+// and 92.7.
 #pragma once
 
 #include "serve.h"

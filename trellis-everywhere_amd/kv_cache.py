@@ -52,7 +52,9 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     out_dtype (q's if None), or fills a contiguous `out`.
 
     max_len: the longest row the call has to expect; it plans the split over the length, and tokens past
-        it are not seen. None: all that the table can hold. Give the batch's own bound where one is known.
+        it are not seen. None: all that the table can hold. Give the batch's own bound where one is known: a
+        single row is split for it (4000 tokens take 9.6 us under 8192, 13.9 under 32768, 31 under 131072),
+        and `scores` need scratch for it, 4 bytes per row, query head and token.
     scores: each token's entry grows by the sum of its weights over the query heads of its head.
     Keys and values of a row's tokens have to be finite (another makes the row's heads NaN); what the pages hold
     past them is not looked at.
@@ -89,7 +91,9 @@ class PagedKVCache:
 
     A step calls grow() once, then append() and attend() for each layer; evict() once after a step keeps
     the rows within a budget. The page tables, lengths and positions are shared by the layers. Calls are
-    ordered on the current stream; use the cache on one stream at a time."""
+    ordered on the current stream; use the cache on one stream at a time. A grow(), evict() or release() that
+    changes a row's pages sends the table anew and waits for the stream (a budget that is a multiple of
+    page_size takes and frees a page each step)."""
 
     def __init__(self, layers: int, heads: int, head_dim: int, *, rows: int, max_len: int, pages: int | None = None,
                  page_size: int = 64, dtype: torch.dtype = torch.float16, device="cuda", evictable: bool = False):
