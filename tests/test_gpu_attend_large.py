@@ -54,3 +54,15 @@ def test_a_maximum_that_grows_by_rounded_units(te, gpu_device, x, y, more):
     share = 2.0 ** -more
     want = (v[0].double() * share + v[128].double()) / (1 + share)
     ref.close(got, want, y, 2.0 ** -19 * max(1.0, float(v.abs().max())))
+
+
+@pytest.mark.parametrize("y", [BF16, F32])
+@pytest.mark.parametrize("n", [1, 3, 100, 700])
+def test_large_bf16_values(te, gpu_device, y, n):
+    """bf16 values up to 2^116 average to what they are: 16-bit (bf16 out) or 24-bit weights and their fp32 sums."""
+    g = torch.Generator().manual_seed(n)
+    q, k, v = torch.randn(64, generator=g).to(BF16), torch.randn((n, 64), generator=g).to(BF16), torch.rand((n, 64), generator=g)
+    v = (v * 2.0 ** 116).to(BF16)
+    got = _run(te, gpu_device, q, k.float(), v.float(), BF16, y, 0.125)
+    want = torch.softmax(k.double() @ q.double() * 0.125, 0) @ v.double()
+    ref.close(got, want, y, 2.0 ** 116 * (2.0 ** -15 if y == BF16 else 2.0 ** -23 * (3 * n + 200)))

@@ -20,7 +20,7 @@
 //     group's 8 tokens (whole rows per 16 lanes) and transposes in its own registers (v_perm_b32);
 //   * both products leave the head on l % 16, so the running maximum and the sum are per-lane values.
 //     The maximum that the weights are taken against moves only when a logit passes it by 2^4 (the weights
-//     are at most 2^15), checked by one ballot, so a tile costs no exchange between lane groups.
+//     are at most 2^15, of bf16 2^4), checked by one ballot, so a tile costs no exchange between lane groups.
 // Precision: the weights enter their product as two terms of the cache's type (f16: 22 bits, their scale
 // keeping them out of its subnormals; bf16: 16 bits, of which a 16-bit out keeps 8 or 11, and three terms, 24 bits,
 // where q is of another type or out is fp32), the sums are fp32.
@@ -37,7 +37,7 @@
 namespace trellis {
 
 constexpr float ATT_LOW = -3.0e38f;                   // below every logit that counts
-constexpr float ATT_TOP = 11.f;                       // log2 of the weight at the maximum when it is set
+constexpr float ATT_TOP = 11.f;                       // f16: log2 of the weight at the maximum when it is set
 constexpr float ATT_SLACK = 4.f;                      // how far (log2) a logit may pass it
 
 struct AttendArgs {
@@ -139,6 +139,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
   constexpr int NQ = EXACT ? (BF ? 3 : 2) : 1;      // terms of q
   constexpr int NP = EXACT && BF ? 3 : 2;           // terms of the weights
   constexpr int UP = BF ? 0 : 15;                   // log2 that q's largest element stays below
+  constexpr float TOP = BF ? 0.f : ATT_TOP;         // (bf16 has no subnormals to keep out of, and values up to 2^128)
   constexpr int KS = DP / 32;                       // k-steps of the first product
   constexpr int DL = DP / 16;                       // dims per lane of V
   constexpr int VC = DL / 4;                        // 8-byte pieces of them
@@ -339,10 +340,10 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void attend_kernel(AttendArgs a) {
     float top = s[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
-    if (__any(top - m > ATT_TOP + ATT_SLACK)) {
+    if (__any(top - m > TOP + ATT_SLACK)) {
       const float most = max_groups(top, lane);
-      float to = fmaxf(m, most - ATT_TOP);
-      if (most - to > ATT_TOP + ATT_SLACK) to = most;   // (of 2^27 and more that difference is rounded, up to 16)
+      float to = fmaxf(m, most - TOP);
+      if (most - to > TOP + ATT_SLACK) to = most;   // (of 2^27 and more that difference is rounded, up to 16)
       const float f = exp2f(m - to);
       m = to;
       l *= f;
