@@ -64,7 +64,9 @@ typedef enum trellis_status {
   TRELLIS_ERR_HEADS = 19,      /* head dim not a multiple of 8 in [8,256], query heads not a positive
                                 * multiple of the cache's, or rotary dims not a multiple of 16 in [16,dim] */
   TRELLIS_ERR_PAGE = 20,       /* page size not a power of 2 in [16,1024], or an empty table or pool */
-  TRELLIS_ERR_KEEP = 21        /* eviction: keep < 1, or recent outside 0 .. keep */
+  TRELLIS_ERR_KEEP = 21,       /* eviction: keep < 1, or recent outside 0 .. keep */
+  TRELLIS_ERR_BEAMS = 22,      /* beams or k outside 1 .. TRELLIS_BEAM_MAX, or an empty vocabulary */
+  TRELLIS_ERR_LAYERS = 23      /* no layer, or layers of pools that differ in sizes, strides or dtype */
 } trellis_status;
 
 /* Flags of trellis_packed_linear_ex / trellis_packed_linear_group_ex. */
@@ -296,6 +298,65 @@ int trellis_evict_workspace_bytes(const trellis_kv_cache *cache, int keep, int a
 int trellis_kv_evict(const trellis_kv_cache *cache, int keep, int recent, const int32_t *next_pos,
                      const int32_t *out_table, int64_t out_table_stride, int out_width,
                      int32_t *new_lens, void *workspace, size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------- several hypotheses over a cache
+ * Drafted tokens in a tree, prompts, beams, and what moves cache entries for them (no reference
+ * counterpart: it decodes one sequence a token at a time, web/model.js:77-102). */
+
+/* Attention of several new tokens per row. Row b's n = starts[b+1] - starts[b] tokens (starts:
+ * [rows + 1]; NULL: tokens / rows each) are the newest of its lens[b], in its last n slots. The i-th
+ * sees the slots below lens[b] - n, itself and its ancestors:
+ *   out = sum_j p_j v_j, p = softmax over the tokens j it sees of scale * q . k_j
+ *   parents: [tokens], the number within the row of the token that each one continues; one that is
+ *   not below the token's own is none (the token then continues the cached tokens). NULL: each
+ *   continues the token before it, so that it sees all of them: a prompt, or part of one.
+ *   q: [tokens][q_heads][head_dim] of q_dtype, token and head strides in elements
+ *   out: [tokens][q_heads][head_dim] contiguous of out_dtype, 16-byte aligned
+ * A token of no row, one whose slot the table (or max_len) does not hold, and one all of whose tokens
+ * lie on pages that do not exist give 0. Keys and values of a row's tokens are finite, those of tokens
+ * that another one does not see included. Workspace as for trellis_paged_attention. */
+int trellis_tree_attention_workspace_bytes(const trellis_kv_cache *cache, int tokens, int q_heads,
+                                           int q_dtype, int out_dtype, size_t *bytes);
+int trellis_tree_attention(const trellis_kv_cache *cache, const void *q, int64_t q_token_stride,
+                           int64_t q_head_stride, int q_dtype, int tokens, int q_heads,
+                           const int32_t *starts, const int32_t *parents, float scale, void *out,
+                           int out_dtype, void *workspace, size_t ws_bytes, void *stream);
+
+/* Beam search's selection: per batch element, of the candidates (beam j, token v) at
+ *   scores[j] + logits[j][v] - log sum_u exp(logits[j][u])
+ * the k largest in order, equal ones by the lower beam, then the lower token. An ended beam offers one
+ * candidate, (j, end_token) at scores[j], and its logits are not read. A candidate that is -inf or not
+ * a number is none; where fewer than k are left, the rest get score -inf, beam 0 and end_token.
+ *   logits: [batch][beams][vocab] of `dtype`, batch and beam strides in elements, below +inf
+ *   scores: f32 [batch][beams]; ended: [batch][beams], 0 or not, or NULL
+ *   new_scores f32, new_beams, new_tokens int32: [batch][k]
+ * Beams are compared in 64 bits; new_scores are rounded once. The workspace
+ * (trellis_beam_workspace_bytes, 256-byte aligned) needs no initialisation. */
+#define TRELLIS_BEAM_MAX 64
+int trellis_beam_workspace_bytes(int batch, int beams, int vocab, int k, size_t *bytes);
+int trellis_beam_select(const void *logits, int64_t batch_stride, int64_t beam_stride, int dtype,
+                        int batch, int beams, int vocab, const float *scores, const uint8_t *ended,
+                        int end_token, int k, float *new_scores, int32_t *new_beams,
+                        int32_t *new_tokens, void *workspace, size_t ws_bytes, void *stream);
+
+/* Pages copied in all layers: the first counts[i] tokens (counts NULL: all) of page dst[i] become those
+ * of page src[i], keys, values and (where a layer has them) scores and positions.
+ *   layers: n_layers caches, alike but for their pointers; table, lens and max_len are not looked at
+ *   src, dst, counts: int32 [n]; no page may be in dst twice, or in dst and src (but src[i] == dst[i],
+ *   and ids outside the pool, copy nothing) */
+int trellis_kv_copy_pages(const trellis_kv_cache *layers, int n_layers, const int32_t *src,
+                          const int32_t *dst, const int32_t *counts, int n, void *stream);
+
+/* Of each row's n = starts[b+1] - starts[b] newest tokens, in its slots from base = lens[b] - n on, those
+ * on its path stay, in place and in all layers: token path[b][i] moves to slot base + i, key, value,
+ * score and position together. The path [rows][path_width] (row stride path_stride) holds ascending
+ * numbers below n and ends at the first entry that is not one (-1). new_lens[b] = base + the path's
+ * length; it must not be the layers' lens. No page that holds new tokens may be in two rows' tables. A
+ * token whose old or new slot is on no page is not moved.
+ *   layers: as above, with one table and lens for all (the first's are read) */
+int trellis_kv_keep(const trellis_kv_cache *layers, int n_layers, const int32_t *starts,
+                    const int32_t *path, int64_t path_stride, int path_width, int32_t *new_lens,
+                    void *stream);
 
 /* Human-readable name of a status code. */
 const char *trellis_strerror(int status);

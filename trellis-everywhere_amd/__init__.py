@@ -14,7 +14,8 @@ from .format import PackedRecord, fit_block, read_packed, write_packed
 __all__ = ["PackedRecord", "read_packed", "write_packed", "fit_block", "TrellisError",
            "TrellisLibraryMissing", "PackedLinear", "PackedGroup", "PackedOps", "load_packed",
            "encode_tiles", "library", "TrellisLinear", "TrellisGroupLinear", "swap_linears",
-           "rms_norm", "residual_norm", "append_kv", "paged_attention", "evict_kv", "PagedKVCache"]
+           "rms_norm", "residual_norm", "append_kv", "paged_attention", "evict_kv", "PagedKVCache",
+           "tree_attention", "beam_select", "copy_pages", "keep_kv"]
 
 
 def library():
@@ -26,7 +27,8 @@ def library():
 _LAZY = {"packed_linear": ("PackedLinear", "PackedGroup", "PackedOps", "load_packed", "encode_tiles"),
          "modules": ("TrellisLinear", "TrellisGroupLinear", "swap_linears"),
          "norms": ("rms_norm", "residual_norm"),
-         "kv_cache": ("append_kv", "paged_attention", "evict_kv", "PagedKVCache")}
+         "beams": ("beam_select",),
+         "kv_cache": ("append_kv", "paged_attention", "tree_attention", "evict_kv", "copy_pages", "keep_kv", "PagedKVCache")}
 
 
 def __getattr__(name):

@@ -24,7 +24,8 @@ STATUS_NAMES = {
     11: "TRELLIS_ERR_BATCH", 12: "TRELLIS_ERR_RANGE", 13: "TRELLIS_ERR_LAUNCH",
     14: "TRELLIS_ERR_GROUP", 15: "TRELLIS_ERR_FLAGS", 16: "TRELLIS_ERR_SCRATCH",
     17: "TRELLIS_ERR_CAPTURE", 18: "TRELLIS_ERR_WIDTH", 19: "TRELLIS_ERR_HEADS",
-    20: "TRELLIS_ERR_PAGE", 21: "TRELLIS_ERR_KEEP",
+    20: "TRELLIS_ERR_PAGE", 21: "TRELLIS_ERR_KEEP", 22: "TRELLIS_ERR_BEAMS",
+    23: "TRELLIS_ERR_LAYERS",
 }
 
 # TRELLIS_NOALLOC_SCRATCH_BYTES: the static workspace of trellis_packed_linear_group_noalloc
@@ -42,7 +43,13 @@ EXPORTED = ("trellis_workspace_bytes", "trellis_packed_linear", "trellis_decode_
             "trellis_packed_linear_ex", "trellis_packed_linear_group_ex",
             "trellis_packed_linear_group_noalloc", "trellis_residual_norm", "trellis_kv_append",
             "trellis_attention_workspace_bytes", "trellis_paged_attention",
-            "trellis_evict_workspace_bytes", "trellis_kv_evict")
+            "trellis_evict_workspace_bytes", "trellis_kv_evict",
+            "trellis_tree_attention_workspace_bytes", "trellis_tree_attention",
+            "trellis_beam_workspace_bytes", "trellis_beam_select", "trellis_kv_copy_pages",
+            "trellis_kv_keep")
+
+# those that _serve.so calls, in the order in which it takes their addresses
+BOUND = EXPORTED[EXPORTED.index("trellis_residual_norm"):]
 
 
 class TrellisLibraryMissing(RuntimeError):
@@ -164,7 +171,13 @@ def load(path: str | None = None):
             ("trellis_attention_workspace_bytes", [C, I, I, ctypes.POINTER(SZ)]),
             ("trellis_paged_attention", [C, P, L, L, I, I, F, I, P, I, P, SZ, P]),
             ("trellis_evict_workspace_bytes", [C, I, I, ctypes.POINTER(SZ)]),
-            ("trellis_kv_evict", [C, I, I, P, P, L, I, P, P, SZ, P])):
+            ("trellis_kv_evict", [C, I, I, P, P, L, I, P, P, SZ, P]),
+            ("trellis_tree_attention_workspace_bytes", [C, I, I, I, I, ctypes.POINTER(SZ)]),
+            ("trellis_tree_attention", [C, P, L, L, I, I, I, P, P, F, P, I, P, SZ, P]),
+            ("trellis_beam_workspace_bytes", [I, I, I, I, ctypes.POINTER(SZ)]),
+            ("trellis_beam_select", [P, L, L, I, I, I, I, P, P, I, I, P, P, P, P, SZ, P]),
+            ("trellis_kv_copy_pages", [C, I, P, P, P, I, P]),
+            ("trellis_kv_keep", [C, I, P, P, L, I, P, P])):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, ctypes.c_int
     lib.trellis_strerror.argtypes = [ctypes.c_int]
@@ -192,9 +205,7 @@ def serve():
         spec = importlib.util.spec_from_file_location("_serve", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
-        module.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "trellis_residual_norm", "trellis_kv_append", "trellis_attention_workspace_bytes", "trellis_paged_attention",
-            "trellis_evict_workspace_bytes", "trellis_kv_evict")])
+        module.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in BOUND])
         _serve = module
     return _serve
 

@@ -13,9 +13,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtrellis_amd.so")
-SOURCES = ["trellis_amd.hip", "kernels_k2.hip", "kernels_k3.hip", "kernels_k4.hip", "serve.hip"]
+SOURCES = ["trellis_amd.hip", "kernels_k2.hip", "kernels_k3.hip", "kernels_k4.hip", "serve.hip", "search.hip"]
 HEADERS = ["decode.h", "common.h", "gemv.h", "bgemm.h", "launch.h", "embed.h", "encode.h",
-           "serve.h", "norm.h", "append.h", "attend_plan.h", "attend.h", "evict.h"]
+           "serve.h", "serve_host.h", "norm.h", "append.h", "attend_plan.h", "attend.h", "evict.h",
+           "tree.h", "beam.h", "pages.h"]
 
 # the Python side of the operators between the packed linears (host code against torch's C++ headers)
 BIND = "bind.cpp"

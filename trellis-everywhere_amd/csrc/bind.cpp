@@ -24,7 +24,9 @@
 
 #include <cmath>
 #include <cstdarg>
+#include <cstring>
 #include <string>
+#include <vector>
 
 #include "trellis_amd.h"
 
@@ -38,6 +40,12 @@ struct Entry {
   decltype(&trellis_paged_attention) paged_attention;
   decltype(&trellis_evict_workspace_bytes) evict_workspace_bytes;
   decltype(&trellis_kv_evict) kv_evict;
+  decltype(&trellis_tree_attention_workspace_bytes) tree_attention_workspace_bytes;
+  decltype(&trellis_tree_attention) tree_attention;
+  decltype(&trellis_beam_workspace_bytes) beam_workspace_bytes;
+  decltype(&trellis_beam_select) beam_select;
+  decltype(&trellis_kv_copy_pages) kv_copy_pages;
+  decltype(&trellis_kv_keep) kv_keep;
 } entry = {};
 
 struct Refused {};   // a Python error is set
@@ -246,11 +254,13 @@ struct CacheView {
   int device;
 };
 
-// k_pages, v_pages, scores, pos, table, lens of a call; max_len None: all that the table can hold.
+// k_pages, v_pages, scores, pos, table, lens of a call (table and lens None: one that takes none); max_len None: all that
+// the table can hold.
 CacheView cache_view(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject* pos_o, PyObject* table_o, PyObject* lens_o,
                      PyObject* max_len) {
-  const at::Tensor &k = tensor(k_o, "k_pages"), &v = tensor(v_o, "v_pages"), &table = tensor(table_o, "table"),
-                   &lens = tensor(lens_o, "lens");
+  const at::Tensor &k = tensor(k_o, "k_pages"), &v = tensor(v_o, "v_pages");
+  const bool rows = table_o != Py_None || lens_o != Py_None;
+  const at::Tensor *table = rows ? &tensor(table_o, "table") : nullptr, *lens = rows ? &tensor(lens_o, "lens") : nullptr;
   const at::Tensor *scores = optional_tensor(scores_o, "scores"), *pos = optional_tensor(pos_o, "pos");
   if (!on_gpu(k)) refuse("the cache lives on a GPU");
   const int device = index_of(k);
@@ -258,24 +268,25 @@ CacheView cache_view(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject*
     refuse("k_pages and v_pages must be [pages, heads, page_size, head_dim], alike in dtype and strides");
   if (k.scalar_type() != at::kHalf && k.scalar_type() != at::kBFloat16) refuse("cache dtype must be float16 or bfloat16");
   if (k.stride(3) != 1) refuse("k_pages and v_pages must have unit stride over head_dim");
-  if (table.scalar_type() != at::kInt || table.dim() != 2 || (table.stride(1) != 1 && table.size(1) != 1))
+  if (rows && (table->scalar_type() != at::kInt || table->dim() != 2 || (table->stride(1) != 1 && table->size(1) != 1)))
     refuse("table must be int32 [rows, width] with unit column stride");
-  if (!on_gpu(v) || !on_gpu(table) || index_of(v) != device || index_of(table) != device)
+  if (!on_gpu(v) || index_of(v) != device || (rows && (!on_gpu(*table) || index_of(*table) != device)))
     refuse("k_pages, v_pages, table and lens must be on one device");
   const at::IntArrayRef plane = k.sizes().slice(0, 3);
-  expect(lens, "lens", at::kInt, {table.size(0)}, device);
+  if (rows) expect(*lens, "lens", at::kInt, {table->size(0)}, device);
   if (scores) expect(*scores, "scores", at::kFloat, plane, device);
   if (pos) expect(*pos, "pos", at::kInt, plane, device);
-  for (const int64_t size : {k.size(0), k.size(1), k.size(2), k.size(3), table.size(0), table.size(1)})
+  const int64_t height = rows ? table->size(0) : 0, width = rows ? table->size(1) : 1;
+  for (const int64_t size : {k.size(0), k.size(1), k.size(2), k.size(3), height, width})
     if (size > INT32_MAX) refuse("the cache's sizes must fit 32 bits");
   CacheView w;
   w.device = device;
   w.c = {k.data_ptr(), v.data_ptr(), scores ? scores->data_ptr<float>() : nullptr, pos ? pos->data_ptr<int32_t>() : nullptr,
-         table.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), k.stride(0), k.stride(1), k.stride(2), table.stride(0),
-         static_cast<int32_t>(k.size(0)), static_cast<int32_t>(k.size(1)), static_cast<int32_t>(k.size(2)),
-         static_cast<int32_t>(k.size(3)), dtype_code(k.scalar_type()), static_cast<int32_t>(table.size(0)),
-         static_cast<int32_t>(table.size(1)),
-         max_len == Py_None ? static_cast<int32_t>(std::min<int64_t>(table.size(1) * k.size(2), 1 << 30)) : whole(max_len, "max_len")};
+         rows ? table->const_data_ptr<int32_t>() : nullptr, rows ? lens->const_data_ptr<int32_t>() : nullptr, k.stride(0),
+         k.stride(1), k.stride(2), rows ? table->stride(0) : 0, static_cast<int32_t>(k.size(0)), static_cast<int32_t>(k.size(1)),
+         static_cast<int32_t>(k.size(2)), static_cast<int32_t>(k.size(3)), dtype_code(k.scalar_type()),
+         static_cast<int32_t>(height), static_cast<int32_t>(width),
+         max_len == Py_None ? static_cast<int32_t>(std::min<int64_t>(width * k.size(2), 1 << 30)) : whole(max_len, "max_len")};
   return w;
 }
 
@@ -414,25 +425,180 @@ PyObject* evict_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------- several hypotheses
+
+// q, k_pages, v_pages, table, lens, starts, parents, scale, max_len, out, out_dtype, workspace -> out
+PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 12, "tree_attention");
+    const at::Tensor& q0 = tensor(a[0], "q");
+    const CacheView w = cache_view(a[1], a[2], Py_None, Py_None, a[3], a[4], a[8]);
+    const c10::DeviceGuard guard(THPVariable_Unpack(a[1]).device());
+    const int64_t d = w.c.head_dim;
+    if (q0.dim() != 3 || q0.size(2) != d || q0.size(0) > INT32_MAX || q0.size(1) > INT32_MAX || !on_gpu(q0) || index_of(q0) != w.device)
+      refuse("q must be [tokens, q_heads, %d] on the cache's device", static_cast<int>(d));
+    const int q_dt = dtype_code(q0, "q"), tokens = static_cast<int>(q0.size(0)), hq = static_cast<int>(q0.size(1));
+    const int32_t* starts = ints(a[5], "starts", static_cast<int64_t>(w.c.rows) + 1, w.device);
+    const int32_t* parents = ints(a[6], "parents", tokens, w.device);
+    if (!starts && (w.c.rows == 0 ? tokens != 0 : tokens % w.c.rows != 0))
+      refuse("without starts every row has the same number of tokens: %d are no multiple of %d rows", tokens, w.c.rows);
+    const at::Tensor q = as_heads(q0);
+    const at::Tensor* given = optional_tensor(a[9], "out");
+    at::Tensor out;
+    if (given) {
+      out = *given;
+      if (out.sizes() != q0.sizes() || !out.is_contiguous() || !on_gpu(out) || index_of(out) != w.device)
+        refuse("out must be contiguous with q's sizes and device");
+    } else {
+      out = make(q0.sizes(), dtype_or(a[10], q0, "out_dtype"), q0);
+    }
+    const int out_dt = dtype_code(out, "out");
+    const double scale = a[7] == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : number(a[7], "scale");
+    size_t need = 0;
+    check(entry.tree_attention_workspace_bytes(&w.c, tokens, hq, q_dt, out_dt, &need));
+    const Scratch ws(a[11], need, q0);
+    check(entry.tree_attention(&w.c, q.const_data_ptr(), q.stride(0), q.stride(1), q_dt, tokens, hq, starts, parents,
+                               static_cast<float>(scale), out.data_ptr(), out_dt, ws.p, ws.bytes, stream_of(w.device)));
+    for (const int i : {9, 11}) written(a[i]);
+    return given ? Py_NewRef(a[9]) : THPVariable_Wrap(std::move(out));
+  });
+}
+
+// logits, scores, k, ended, end_token, workspace -> (scores, beams, tokens)
+PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 6, "beam_select");
+    const at::Tensor &x0 = tensor(a[0], "logits"), &scores = tensor(a[1], "scores");
+    const at::Tensor* ended = optional_tensor(a[3], "ended");
+    if (!on_gpu(x0)) refuse("the selection runs on a GPU");
+    const c10::DeviceGuard guard(x0.device());
+    const int device = index_of(x0), x_dt = dtype_code(x0, "logits"), k = whole(a[2], "k"), end_token = whole(a[4], "end_token");
+    if (x0.dim() != 3) refuse("logits must be [batch, beams, vocab]");
+    const int64_t batch = x0.size(0), beams = x0.size(1), vocab = x0.size(2);
+    if (batch > INT32_MAX || beams > INT32_MAX || vocab > INT32_MAX) refuse("the logits' sizes must fit 32 bits");
+    expect(scores, "scores", at::kFloat, {batch, beams}, device);
+    if (ended) expect(*ended, "ended", at::kBool, {batch, beams}, device);
+    const at::Tensor x = as_heads(x0);
+    size_t need = 0;
+    check(entry.beam_workspace_bytes(static_cast<int>(batch), static_cast<int>(beams), static_cast<int>(vocab), k, &need));
+    at::Tensor out = make({batch, k}, at::kFloat, x0), from = make({batch, k}, at::kInt, x0), token = make({batch, k}, at::kInt, x0);
+    const Scratch ws(a[5], need, x0);
+    check(entry.beam_select(x.const_data_ptr(), x.stride(0), x.stride(1), x_dt, static_cast<int>(batch), static_cast<int>(beams),
+                            static_cast<int>(vocab), scores.const_data_ptr<float>(),
+                            ended ? reinterpret_cast<const uint8_t*>(ended->const_data_ptr<bool>()) : nullptr, end_token, k,
+                            out.data_ptr<float>(), from.data_ptr<int32_t>(), token.data_ptr<int32_t>(), ws.p, ws.bytes,
+                            stream_of(device)));
+    written(a[5]);
+    PyObject* parts[3] = {THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(from)), THPVariable_Wrap(std::move(token))};
+    PyObject* all = parts[0] && parts[1] && parts[2] ? PyTuple_Pack(3, parts[0], parts[1], parts[2]) : nullptr;
+    for (PyObject* p : parts) Py_XDECREF(p);
+    return all;
+  });
+}
+
+// The tensors of a model's layers: one tensor, or a list or tuple with one for each layer. None: no layer has one.
+struct PerLayer {
+  PyObject* const* items;
+  Py_ssize_t n;
+  PyObject* alone;
+  PerLayer(PyObject* o, const char* name) : alone(o) {
+    if (PyList_Check(o) || PyTuple_Check(o)) {
+      items = PySequence_Fast_ITEMS(o);
+      n = PySequence_Fast_GET_SIZE(o);
+      if (n == 0) refuse("%s holds no layer", name);
+    } else {
+      items = nullptr;
+      n = o == Py_None ? 0 : 1;
+    }
+  }
+  PyObject* operator[](Py_ssize_t i) const { return n == 0 ? Py_None : items ? items[i] : alone; }
+  void all_written() const {
+    for (Py_ssize_t i = 0; i < n; ++i) written((*this)[i]);
+  }
+};
+
+// One cache a layer; table and lens None: a call that takes none.
+struct LayerViews {
+  PerLayer k, v, scores, pos;
+  std::vector<trellis_kv_cache> c;
+  int device;
+  LayerViews(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject* pos_o, PyObject* table, PyObject* lens)
+      : k(k_o, "k_pages"), v(v_o, "v_pages"), scores(scores_o, "scores"), pos(pos_o, "pos") {
+    if (v.n != k.n || (scores.n && scores.n != k.n) || (pos.n && pos.n != k.n))
+      refuse("k_pages, v_pages, scores and pos must have as many layers");
+    if (k.n > INT16_MAX) refuse("too many layers");
+    c.reserve(k.n);
+    for (Py_ssize_t i = 0; i < k.n; ++i) {
+      const CacheView w = cache_view(k[i], v[i], scores[i], pos[i], table, lens, Py_None);
+      if (i && w.device != device) refuse("the layers must be on one device");
+      device = w.device;
+      c.push_back(w.c);
+    }
+  }
+  void all_written() const {
+    for (const PerLayer* p : {&k, &v, &scores, &pos}) p->all_written();
+  }
+};
+
+// k_pages, v_pages, src, dst, counts, scores, pos -> None
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 7, "copy_pages");
+    const LayerViews w(a[0], a[1], a[5], a[6], Py_None, Py_None);
+    const at::Tensor &src = tensor(a[2], "src"), &first = THPVariable_Unpack(w.k[0]);
+    const c10::DeviceGuard guard(first.device());
+    if (src.dim() != 1 || src.size(0) > INT32_MAX) refuse("src must be int32 [n]");
+    const int64_t pages = src.size(0);
+    tensor(a[3], "dst");
+    check(entry.kv_copy_pages(w.c.data(), static_cast<int>(w.c.size()), ints(a[2], "src", pages, w.device),
+                              ints(a[3], "dst", pages, w.device), ints(a[4], "counts", pages, w.device),
+                              static_cast<int>(pages), stream_of(w.device)));
+    w.all_written();
+    Py_RETURN_NONE;
+  });
+}
+
+// k_pages, v_pages, table, lens, starts, path, scores, pos -> new lens
+PyObject* keep_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 8, "keep_kv");
+    tensor(a[2], "table");
+    const LayerViews w(a[0], a[1], a[6], a[7], a[2], a[3]);
+    const c10::DeviceGuard guard(THPVariable_Unpack(w.k[0]).device());
+    const at::Tensor &path = tensor(a[5], "path"), &lens = THPVariable_Unpack(a[3]);
+    const int rows = w.c[0].rows;
+    tensor(a[4], "starts");
+    if (path.scalar_type() != at::kInt || path.dim() != 2 || path.size(0) != rows || path.size(1) > INT32_MAX ||
+        (path.stride(1) != 1 && path.size(1) > 1) || !on_gpu(path) || index_of(path) != w.device)
+      refuse("path must be int32 [%d, width] with unit column stride on the cache's device", rows);
+    at::Tensor out = make(lens.sizes(), at::kInt, lens);
+    check(entry.kv_keep(w.c.data(), static_cast<int>(w.c.size()), ints(a[4], "starts", static_cast<int64_t>(rows) + 1, w.device),
+                        path.const_data_ptr<int32_t>(), path.stride(0), static_cast<int>(path.size(1)), out.data_ptr<int32_t>(),
+                        stream_of(w.device)));
+    w.all_written();
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 // The addresses of the library's entry points, in the order of Entry.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    count(n, 6, "bind");
-    void* p[6];
-    for (int i = 0; i < 6; ++i) {
+    constexpr Py_ssize_t have = sizeof(Entry) / sizeof(void*);
+    count(n, have, "bind");
+    void* p[have];
+    for (Py_ssize_t i = 0; i < have; ++i) {
       p[i] = PyLong_AsVoidPtr(a[i]);
       if (!p[i]) refuse("bind takes addresses");
     }
-    entry = {reinterpret_cast<decltype(entry.residual_norm)>(p[0]), reinterpret_cast<decltype(entry.kv_append)>(p[1]),
-             reinterpret_cast<decltype(entry.attention_workspace_bytes)>(p[2]),
-             reinterpret_cast<decltype(entry.paged_attention)>(p[3]),
-             reinterpret_cast<decltype(entry.evict_workspace_bytes)>(p[4]), reinterpret_cast<decltype(entry.kv_evict)>(p[5])};
+    static_assert(sizeof(p) == sizeof(entry), "every entry is one address");
+    std::memcpy(&entry, p, sizeof(entry));
     Py_RETURN_NONE;
   });
 }
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(residual_norm), METHOD(append_kv), METHOD(paged_attention), METHOD(evict_kv),
+                         METHOD(tree_attention), METHOD(beam_select), METHOD(copy_pages), METHOD(keep_kv),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serve", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

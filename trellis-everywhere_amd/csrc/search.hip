@@ -1,0 +1,225 @@
+// search.hip — C ABI of the operators that carry several hypotheses over a paged cache (include/trellis_amd.h):
+// validation, launch planning and the dispatch to tree.h, beam.h and pages.h.
+#include <hip/hip_runtime.h>
+
+#include "beam.h"
+#include "pages.h"
+#include "serve_host.h"
+#include "tree.h"
+
+using namespace trellis;
+
+namespace {
+
+// ---------------------------------------------------------------- attention of several new tokens
+
+int validate_tree(const trellis_kv_cache* c, int q_heads, int tokens, int q_dtype, int out_dtype) {
+  const int v = validate_cache(c);
+  if (v) return v;
+  if (q_heads < 1 || q_heads % c->heads) return TRELLIS_ERR_HEADS;
+  if (!known_dtype(q_dtype) || !known_dtype(out_dtype)) return TRELLIS_ERR_DTYPE;
+  if (tokens < 0 || (tokens > 0 && c->rows < 1)) return TRELLIS_ERR_BATCH;
+  return TRELLIS_OK;
+}
+
+// ---------------------------------------------------------------- beams
+
+int validate_beam(int batch, int beams, int vocab, int k) {
+  if (batch < 0) return TRELLIS_ERR_BATCH;
+  if (beams < 1 || beams > BEAM_MOST || k < 1 || k > BEAM_MOST || vocab < 1) return TRELLIS_ERR_BEAMS;
+  return TRELLIS_OK;
+}
+
+struct BeamPlan {
+  size_t off_best, ws;
+};
+
+BeamPlan beam_plan(int batch, int beams, int k) {
+  const size_t rows = static_cast<size_t>(batch) * beams;
+  BeamPlan p;
+  p.off_best = up256(rows * 8);
+  p.ws = p.off_best + up256(rows * k * 8);
+  return p;
+}
+
+// ---------------------------------------------------------------- pages
+
+// Layers of one pool geometry; the pointers of `count` of them.
+int validate_layers(const trellis_kv_cache* c, int layers) {
+  if (layers < 1) return TRELLIS_ERR_LAYERS;
+  if (!c) return TRELLIS_ERR_NULL;
+  for (int i = 0; i < layers; ++i) {
+    const int v = validate_cache(c + i);
+    if (v) return v;
+    if (c[i].page_stride != c->page_stride || c[i].head_stride != c->head_stride || c[i].slot_stride != c->slot_stride ||
+        c[i].pages != c->pages || c[i].heads != c->heads || c[i].page_size != c->page_size || c[i].head_dim != c->head_dim ||
+        c[i].dtype != c->dtype)
+      return TRELLIS_ERR_LAYERS;
+    if (!aligned(c[i].scores, 4) || !aligned(c[i].pos, 4)) return TRELLIS_ERR_ALIGN;
+  }
+  return TRELLIS_OK;
+}
+
+Layers layers_of(const trellis_kv_cache* c, int count) {
+  Layers l = {};
+  for (int i = 0; i < count; ++i) {
+    l.k[i] = c[i].k;
+    l.v[i] = c[i].v;
+    l.scores[i] = c[i].scores;
+    l.pos[i] = c[i].pos;
+  }
+  return l;
+}
+
+}  // namespace
+
+extern "C" {
+
+int trellis_tree_attention_workspace_bytes(const trellis_kv_cache* cache, int tokens, int q_heads, int q_dtype, int out_dtype,
+                                           size_t* bytes) {
+  if (!bytes) return TRELLIS_ERR_NULL;
+  const int v = validate_tree(cache, q_heads, tokens, q_dtype, out_dtype);
+  if (v) return v;
+  *bytes = 0;
+  return TRELLIS_OK;
+}
+
+int trellis_tree_attention(const trellis_kv_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                           int q_dtype, int tokens, int q_heads, const int32_t* starts, const int32_t* parents, float scale,
+                           void* out, int out_dtype, void* workspace, size_t ws_bytes, void* stream) {
+  const int v = validate_tree(cache, q_heads, tokens, q_dtype, out_dtype);
+  if (v) return v;
+  if (!starts && cache->rows > 0 && tokens % cache->rows) return TRELLIS_ERR_BATCH;
+  if (tokens == 0) return TRELLIS_OK;
+  if (!q || !out) return TRELLIS_ERR_NULL;
+  if (!aligned(q, dtype_size(q_dtype)) || !aligned(out, 16)) return TRELLIS_ERR_ALIGN;
+  TreeArgs a;
+  a.q = q;
+  a.q_t = q_token_stride;
+  a.q_h = q_head_stride;
+  a.q_dt = q_dtype;
+  a.out_dt = out_dtype;
+  a.tokens = tokens;
+  a.hq = q_heads;
+  a.group = q_heads / cache->heads;
+  a.starts = starts;
+  a.each = starts ? 0 : tokens / cache->rows;
+  a.parents = parents;
+  a.out = out;
+  a.scale = scale;
+  a.c = cache_of(cache);
+  const int64_t blocks = static_cast<int64_t>(tokens) * q_heads;
+  if (!grid_fits(blocks, 64)) return TRELLIS_ERR_BATCH;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(64);
+  if (cache->dtype == TRELLIS_F16) hipLaunchKernelGGL(tree_kernel<_Float16>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(tree_kernel<bf16_t>, grid, block, 0, st, a);
+  return launched();
+}
+
+int trellis_beam_workspace_bytes(int batch, int beams, int vocab, int k, size_t* bytes) {
+  if (!bytes) return TRELLIS_ERR_NULL;
+  const int v = validate_beam(batch, beams, vocab, k);
+  if (v) return v;
+  *bytes = beam_plan(batch, beams, k).ws;
+  return TRELLIS_OK;
+}
+
+int trellis_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride, int dtype, int batch, int beams,
+                        int vocab, const float* scores, const uint8_t* ended, int end_token, int k, float* new_scores,
+                        int32_t* new_beams, int32_t* new_tokens, void* workspace, size_t ws_bytes, void* stream) {
+  const int v = validate_beam(batch, beams, vocab, k);
+  if (v) return v;
+  if (!known_dtype(dtype)) return TRELLIS_ERR_DTYPE;
+  if (end_token < 0 || end_token >= vocab) return TRELLIS_ERR_RANGE;
+  if (batch == 0) return TRELLIS_OK;
+  if (!logits || !scores || !new_scores || !new_beams || !new_tokens) return TRELLIS_ERR_NULL;
+  if (!aligned(logits, dtype_size(dtype)) || !aligned(scores, 4) || !aligned(new_scores, 4) || !aligned(new_beams, 4) ||
+      !aligned(new_tokens, 4))
+    return TRELLIS_ERR_ALIGN;
+  const BeamPlan p = beam_plan(batch, beams, k);
+  if (!workspace || ws_bytes < p.ws) return TRELLIS_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
+  const int64_t rows = static_cast<int64_t>(batch) * beams;
+  if (!grid_fits(rows, 256)) return TRELLIS_ERR_BATCH;
+  BeamArgs a;
+  a.x = logits;
+  a.x_b = batch_stride;
+  a.x_j = beam_stride;
+  a.batch = batch;
+  a.beams = beams;
+  a.vocab = vocab;
+  a.k = k;
+  a.end_token = end_token;
+  a.scores = scores;
+  a.ended = ended;
+  a.out_scores = new_scores;
+  a.out_beams = new_beams;
+  a.out_tokens = new_tokens;
+  char* ws = static_cast<char*>(workspace);
+  a.lse = reinterpret_cast<double*>(ws);
+  a.best = reinterpret_cast<uint2*>(ws + p.off_best);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(rows)), block(256);
+  if (dtype == TRELLIS_F32) hipLaunchKernelGGL(beam_row_kernel<float>, grid, block, 0, st, a);
+  else if (dtype == TRELLIS_F16) hipLaunchKernelGGL(beam_row_kernel<_Float16>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(beam_row_kernel<bf16_t>, grid, block, 0, st, a);
+  hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(64), 0, st, a);
+  return launched();
+}
+
+int trellis_kv_copy_pages(const trellis_kv_cache* layers, int n_layers, const int32_t* src, const int32_t* dst,
+                          const int32_t* counts, int n, void* stream) {
+  const int v = validate_layers(layers, n_layers);
+  if (v) return v;
+  if (n < 0) return TRELLIS_ERR_BATCH;
+  if (n == 0) return TRELLIS_OK;
+  if (!src || !dst) return TRELLIS_ERR_NULL;
+  CopyArgs a;
+  a.c = cache_of(layers);
+  a.src = src;
+  a.dst = dst;
+  a.counts = counts;
+  a.n = n;
+  const int lpr = lanes_per_row(layers->head_dim), rows = 256 / lpr * PAGE_AHEAD, parts = (layers->page_size + rows - 1) / rows;
+  const int64_t one = static_cast<int64_t>(n) * layers->heads * parts;
+  const int most = n_layers < PAGE_LAYERS ? n_layers : PAGE_LAYERS;
+  if (one > INT32_MAX || !grid_fits(one * most, 256)) return TRELLIS_ERR_BATCH;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int at = 0; at < n_layers; at += PAGE_LAYERS) {
+    const int some = n_layers - at < PAGE_LAYERS ? n_layers - at : PAGE_LAYERS;
+    a.l = layers_of(layers + at, some);
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(static_cast<unsigned>(one * some)), dim3(256), 0, st, a, lpr, parts);
+  }
+  return launched();
+}
+
+int trellis_kv_keep(const trellis_kv_cache* layers, int n_layers, const int32_t* starts, const int32_t* path,
+                    int64_t path_stride, int path_width, int32_t* new_lens, void* stream) {
+  const int v = validate_layers(layers, n_layers);
+  if (v) return v;
+  if (path_width < 0 || path_stride < 0) return TRELLIS_ERR_RANGE;
+  if (layers->rows == 0) return TRELLIS_OK;
+  if (!starts || (path_width > 0 && !path) || !new_lens) return TRELLIS_ERR_NULL;
+  if (new_lens == layers->lens) return TRELLIS_ERR_RANGE;
+  KeepArgs a;
+  a.c = cache_of(layers);
+  a.starts = starts;
+  a.path = path;
+  a.path_stride = path_stride;
+  a.path_width = path_width;
+  const int lpr = lanes_per_row(layers->head_dim);
+  const int64_t one = static_cast<int64_t>(layers->rows) * layers->heads;
+  const int most = n_layers < PAGE_LAYERS ? n_layers : PAGE_LAYERS;
+  if (!grid_fits(one * most, 256)) return TRELLIS_ERR_BATCH;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int at = 0; at < n_layers; at += PAGE_LAYERS) {
+    const int some = n_layers - at < PAGE_LAYERS ? n_layers - at : PAGE_LAYERS;
+    a.l = layers_of(layers + at, some);
+    a.new_lens = at == 0 ? new_lens : nullptr;
+    hipLaunchKernelGGL(keep_kernel, dim3(static_cast<unsigned>(one * some)), dim3(256), 0, st, a, lpr);
+  }
+  return launched();
+}
+
+}  // extern "C"

@@ -640,6 +640,8 @@ const char* trellis_strerror(int status) {
              "cache's heads, rotary dims a multiple of 16 up to the head dim";
     case TRELLIS_ERR_PAGE: return "page size must be a power of 2 in [16,1024], pool and table not empty";
     case TRELLIS_ERR_KEEP: return "eviction needs keep >= 1 and 0 <= recent <= keep";
+    case TRELLIS_ERR_BEAMS: return "beams and k must be in 1 .. TRELLIS_BEAM_MAX, the vocabulary not empty";
+    case TRELLIS_ERR_LAYERS: return "layers must be at least one, alike in sizes, strides and dtype";
     default: return "unknown trellis status";
   }
 }

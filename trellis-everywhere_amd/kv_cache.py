@@ -64,6 +64,43 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
                                                  workspace))
 
 
+def tree_attention(q, k_pages, v_pages, table, lens, *, starts=None, parents=None, scale: float | None = None,
+                   max_len: int | None = None, out=None, out_dtype=None, workspace=None):
+    """Attention of several new tokens per row: drafted tokens in a tree, or a prompt. Row b's n = starts[b+1] - starts[b]
+    tokens are the newest of its lens[b] (append_kv has put their keys and values there, in its last n slots); the i-th
+    sees the tokens before them, itself and its ancestors: softmax(scale * q.k) v over these, scale d**-0.5 if None.
+
+    q: [tokens, q_heads, d], any token and head strides; query head i over key-value head i // (q_heads // heads)
+    starts: int32 [rows + 1], row by row as for append_kv; None: the same number of tokens for each row
+    parents: int32 [tokens], the number within its row of the token that each one continues; one that is not below the
+        token's own (-1) is none: it continues the cached tokens. None: each continues the one before it, so that it
+        sees them all (a prompt, or part of one).
+    Returns [tokens, q_heads, d] of out_dtype (q's if None), or fills a contiguous `out`. Zeros for a token of no row
+    (padding), for one whose slot the table or max_len does not hold, and where every page it could see is missing.
+    max_len, workspace: as for paged_attention. Keys and values of a row's tokens have to be finite, those that a token
+        does not see among them."""
+    return _result(_capi.serve().tree_attention(q, k_pages, v_pages, table, lens, starts, parents, scale, max_len, out,
+                                                out_dtype, workspace))
+
+
+def copy_pages(k_pages, v_pages, src, dst, *, counts=None, scores=None, pos=None) -> None:
+    """Page dst[i] becomes page src[i], its first counts[i] tokens if given (int32 [n] each), in one launch for up to 32
+    layers: k_pages and v_pages (scores, pos) are one layer's tensor, or a list with one for each layer.
+    No page may be in dst twice, or in src and dst; src[i] == dst[i], and ids outside the pool, copy nothing."""
+    return _result(_capi.serve().copy_pages(k_pages, v_pages, src, dst, counts, scores, pos))
+
+
+def keep_kv(k_pages, v_pages, table, lens, starts, path, *, scores=None, pos=None):
+    """After a check of drafted tokens: of each row's n = starts[b+1] - starts[b] newest tokens those on its path stay.
+    Token path[b, i] moves to slot lens[b] - n + i, in place, key, value, score and position together, in one launch for
+    up to 32 layers (lists as for copy_pages).
+
+    path: int32 [rows, width], ascending numbers below n; it ends at the first entry that is not one (-1)
+    Returns the new lengths lens - n + the paths' as a new tensor. No page that holds new tokens may be in two rows'
+    tables; a token whose old or new slot is on no page is not moved."""
+    return _result(_capi.serve().keep_kv(k_pages, v_pages, table, lens, starts, path, scores, pos))
+
+
 def evict_kv(k_pages, v_pages, scores, pos, table, lens, keep: int, recent: int, *, next_pos=None, out_table=None,
              max_len: int | None = None, workspace=None):
     """Evict by accumulated attention weight: of each row's tokens, per key-value head, `keep` stay: those of
