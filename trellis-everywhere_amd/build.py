@@ -13,10 +13,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtrellis_amd.so")
-SOURCES = ["trellis_amd.hip", "kernels_k2.hip", "kernels_k3.hip", "kernels_k4.hip", "serve.hip", "search.hip"]
+SOURCES = ["trellis_amd.hip", "kernels_k2.hip", "kernels_k3.hip", "kernels_k4.hip", "serve.hip",
+           "search.hip", "tree_f16.hip", "tree_bf16.hip"]
 HEADERS = ["decode.h", "common.h", "gemv.h", "bgemm.h", "launch.h", "embed.h", "encode.h",
            "serve.h", "serve_host.h", "norm.h", "append.h", "attend_plan.h", "attend.h", "evict.h",
-           "tree.h", "beam.h", "pages.h"]
+           "tree_plan.h", "tree_rows.h", "tree.h", "tree_join.h", "beam.h", "pages.h"]
 
 # the Python side of the operators between the packed linears (host code against torch's C++ headers)
 BIND = "bind.cpp"

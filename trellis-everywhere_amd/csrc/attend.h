@@ -36,10 +36,6 @@
 
 namespace trellis {
 
-constexpr float ATT_LOW = -3.0e38f;                   // below every logit that counts
-constexpr float ATT_TOP = 11.f;                       // f16: log2 of the weight at the maximum when it is set
-constexpr float ATT_SLACK = 4.f;                      // how far (log2) a logit may pass it
-
 struct AttendArgs {
   const void* q;
   long long q_b, q_h;     // strides of q in elements
@@ -57,10 +53,6 @@ struct AttendArgs {
   long long logit_stride;
   Cache c;
 };
-
-// A value that is the same in every lane, into a scalar register (a division leaves it in a vector register, and
-// addresses made from it in two a lane).
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Lengths of rows r0 .. r0 + 63, one a lane.
 __device__ __forceinline__ int att_lengths(const Cache& c, int r0, int lane) {

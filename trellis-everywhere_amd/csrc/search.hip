@@ -6,6 +6,7 @@
 #include "pages.h"
 #include "serve_host.h"
 #include "tree.h"
+#include "tree_join.h"
 
 using namespace trellis;
 
@@ -19,7 +20,24 @@ int validate_tree(const trellis_kv_cache* c, int q_heads, int tokens, int q_dtyp
   if (q_heads < 1 || q_heads % c->heads) return TRELLIS_ERR_HEADS;
   if (!known_dtype(q_dtype) || !known_dtype(out_dtype)) return TRELLIS_ERR_DTYPE;
   if (tokens < 0 || (tokens > 0 && c->rows < 1)) return TRELLIS_ERR_BATCH;
+  // (queries are counted in 32 bits)
+  if (static_cast<int64_t>(tokens) * q_heads >= (int64_t(1) << 31)) return TRELLIS_ERR_BATCH;
   return TRELLIS_OK;
+}
+
+struct TreePlan : TreeChunks {
+  int qr;
+  size_t off_ml, ws;
+};
+
+TreePlan tree_plan(const trellis_kv_cache* c, int q_heads, int tokens) {
+  TreePlan p;
+  static_cast<TreeChunks&>(p) = tree_chunks(c->rows, c->heads, q_heads, c->head_dim, tokens, longest(c), device_cus());
+  p.qr = 32 * p.waves;
+  const size_t slots = p.aim ? static_cast<size_t>(p.items) * p.qr : 0;
+  p.off_ml = up256(slots * c->head_dim * 4);
+  p.ws = p.off_ml + up256(slots * 8);
+  return p;
 }
 
 // ---------------------------------------------------------------- beams
@@ -80,7 +98,7 @@ int trellis_tree_attention_workspace_bytes(const trellis_kv_cache* cache, int to
   if (!bytes) return TRELLIS_ERR_NULL;
   const int v = validate_tree(cache, q_heads, tokens, q_dtype, out_dtype);
   if (v) return v;
-  *bytes = 0;
+  *bytes = tree_plan(cache, q_heads, tokens).ws;
   return TRELLIS_OK;
 }
 
@@ -92,12 +110,19 @@ int trellis_tree_attention(const trellis_kv_cache* cache, const void* q, int64_t
   if (!starts && cache->rows > 0 && tokens % cache->rows) return TRELLIS_ERR_BATCH;
   if (tokens == 0) return TRELLIS_OK;
   if (!q || !out) return TRELLIS_ERR_NULL;
-  if (!aligned(q, dtype_size(q_dtype)) || !aligned(out, 16)) return TRELLIS_ERR_ALIGN;
-  TreeArgs a;
+  const int qs = dtype_size(q_dtype);
+  if (!aligned(q, qs) || !aligned(out, 16)) return TRELLIS_ERR_ALIGN;
+  const TreePlan p = tree_plan(cache, q_heads, tokens);
+  if (p.ws && (!workspace || ws_bytes < p.ws)) return TRELLIS_ERR_WORKSPACE;
+  if (p.ws && !aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
+  char* ws = static_cast<char*>(workspace);
+  TreeLaunch l;
+  TreeArgs& a = l.a;
   a.q = q;
   a.q_t = q_token_stride;
   a.q_h = q_head_stride;
   a.q_dt = q_dtype;
+  a.q_vec = aligned(q, 16) && q_token_stride * qs % 16 == 0 && q_head_stride * qs % 16 == 0;
   a.out_dt = out_dtype;
   a.tokens = tokens;
   a.hq = q_heads;
@@ -106,14 +131,26 @@ int trellis_tree_attention(const trellis_kv_cache* cache, const void* q, int64_t
   a.each = starts ? 0 : tokens / cache->rows;
   a.parents = parents;
   a.out = out;
-  a.scale = scale;
+  a.aim = p.aim;
+  a.items = static_cast<int>(p.items);
+  a.scale = scale * 1.44269504088896340736f;
+  a.part = reinterpret_cast<float*>(ws);
+  a.ml = reinterpret_cast<float*>(ws + p.off_ml);
   a.c = cache_of(cache);
-  const int64_t blocks = static_cast<int64_t>(tokens) * q_heads;
-  if (!grid_fits(blocks, 64)) return TRELLIS_ERR_BATCH;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(blocks)), block(64);
-  if (cache->dtype == TRELLIS_F16) hipLaunchKernelGGL(tree_kernel<_Float16>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(tree_kernel<bf16_t>, grid, block, 0, st, a);
+  // the chunks, then those that see to tokens of no row
+  const int64_t blocks = p.items + (starts ? (static_cast<int64_t>(tokens) + 63) / 64 : 0);
+  const int64_t joins = p.aim ? static_cast<int64_t>(tokens) * cache->heads : 0;
+  // (chunks count the units of all blocks in 32 bits)
+  if (!grid_fits(blocks, 256) || !grid_fits(joins, 256) ||
+      (p.aim && (p.items - p.aim) * tree_units(longest(cache)) >= (int64_t(1) << 31)))
+    return TRELLIS_ERR_BATCH;
+  l.exact = q_dtype != cache->dtype || out_dtype != cache->dtype;
+  l.waves = p.waves;
+  l.grid = static_cast<unsigned>(blocks);
+  l.stream = static_cast<hipStream_t>(stream);
+  if (cache->dtype == TRELLIS_F16) launch_tree_f16(l);
+  else launch_tree_bf16(l);
+  if (joins > 0) hipLaunchKernelGGL(tree_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(256), 0, l.stream, a, p.qr);
   return launched();
 }
 

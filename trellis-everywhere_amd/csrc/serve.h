@@ -10,6 +10,11 @@ typedef __bf16 bf16_t;
 
 enum : int { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };   // enum trellis_dtype
 
+// the attention's running maximum
+constexpr float ATT_LOW = -3.0e38f;                   // below every logit that counts
+constexpr float ATT_TOP = 11.f;                       // f16: log2 of the weight at the maximum when it is set
+constexpr float ATT_SLACK = 4.f;                      // how far (log2) a logit may pass it
+
 // Eight consecutive elements as fp32. VEC: the address is 16-byte aligned.
 template <class T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -133,6 +138,10 @@ __device__ __forceinline__ float group_sum(float v, int n, int lane) {
   if (n > 32) v += lane_xor<32>(v, lane);
   return v;
 }
+
+// A value that is the same in every lane, into a scalar register (a division leaves it in a vector register, and
+// addresses made from it in two a lane).
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A load of what no kernel of the call writes: where the address is the same in every lane, by the scalar unit (from
 // plain memory the compiler does that only if nothing the kernel stores could be there).
