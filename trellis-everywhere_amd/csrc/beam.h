@@ -4,128 +4,314 @@
 // lower beam, then the lower token. A candidate that is -inf or not a number is none.
 // Within a beam the order is that of its logits, so the sums meet only where beams do, in 64 bits there: candidates of two
 // beams may be nearer to each other than a rounding to 32 bits.
+//
+// beam_part_kernel: a wave takes a run of a beam's logits, R x 512 at a time, read once and held in registers: their
+// maximum, the sum of their exponentials, and their k best. Of the lanes' maxima, sorted across the wave, the k-th is a
+// bound that k of the logits reach: the few that do (k and a handful) are gathered through LDS and sorted by (logit, token)
+// into the wave's list of 64.
+// beam_join_kernel, a workgroup a batch element: per beam the runs' sums and lists, then the beams' lists.
 #pragma once
 
 #include "serve.h"
 
 namespace trellis {
 
-constexpr int BEAM_MOST = 64;   // beams, and candidates kept of each (TRELLIS_BEAM_MAX)
+constexpr int BEAM_MOST = 64;   // beams, candidates kept of each, runs of a beam (TRELLIS_BEAM_MAX)
 
 struct BeamArgs {
   const void* x;
   long long x_b, x_j;           // strides of batch and beam in elements
   int batch, beams, vocab, k, end_token;
+  int runs, per;                // waves a beam, and the pieces of 8 logits of each
   const float* scores;          // [batch][beams]
   const uint8_t* ended;         // [batch][beams] or null
   float* out_scores;            // [batch][k]
   int32_t* out_beams;
   int32_t* out_tokens;
-  double* lse;                  // workspace: [batch][beams]
-  uint2* best;                  // workspace: [batch][beams][k] (key, token)
+  double* sums;                 // workspace: [batch x beams][runs] (sum of exponentials against the maximum, maximum)
+  unsigned long long* best;     // workspace: [batch x beams][runs][k] keys in order
 };
 
-// Order-preserving, 0 for what is no candidate: -inf, not a number.
-__device__ __forceinline__ uint32_t beam_key(float x) {
-  if (!(x > -__builtin_inff())) return 0;
+typedef unsigned long long beam_t;   // a candidate: (order-preserving logit, ~token); 0: none
+
+__device__ __forceinline__ uint32_t beam_order(float x) {   // of a logit above -inf: above 0
   const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);   // -0 counts as 0
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float beam_value(uint32_t key) {
+__device__ __forceinline__ float beam_logit(beam_t c) {
+  const uint32_t key = c >> 32;
   return __builtin_bit_cast(float, (key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-// One workgroup a beam: maximum and sum, then k times the largest below the last.
-template <class T>
-__global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a) {
-  __shared__ float s_f[4];
-  __shared__ double s_d[4];
-  __shared__ unsigned long long s_u[4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int row = blockIdx.x, b = row / a.beams, j = row - b * a.beams;
+template <int H>
+__device__ __forceinline__ beam_t lane_xor64(beam_t v, int lane) {
+  const uint32_t lo = __builtin_bit_cast(uint32_t, lane_xor<H>(__builtin_bit_cast(float, static_cast<uint32_t>(v)), lane));
+  const uint32_t hi = __builtin_bit_cast(uint32_t, lane_xor<H>(__builtin_bit_cast(float, static_cast<uint32_t>(v >> 32)), lane));
+  return static_cast<beam_t>(hi) << 32 | lo;
+}
+template <int H> __device__ __forceinline__ float lane_xor_t(float v, int lane) { return lane_xor<H>(v, lane); }
+template <int H> __device__ __forceinline__ beam_t lane_xor_t(beam_t v, int lane) { return lane_xor64<H>(v, lane); }
+
+// One level of a sorting network over the wave: of lanes H apart the one that `up` names for the pair gets the larger.
+template <int H, class V>
+__device__ __forceinline__ V sort_level(V v, bool lower_larger, int lane) {
+  const V o = lane_xor_t<H>(v, lane);
+  const bool larger = lower_larger == ((lane & H) == 0);
+  return (o > v) == larger ? o : v;
+}
+template <int H, class V>
+__device__ __forceinline__ V sort_merge(V v, bool lower_larger, int lane) {   // of 2 H lanes that rise and fall
+  v = sort_level<H>(v, lower_larger, lane);
+  if constexpr (H > 1) v = sort_merge<H / 2>(v, lower_larger, lane);
+  return v;
+}
+// The wave's values in order, the largest first (or last).
+template <class V>
+__device__ __forceinline__ V wave_sort(V v, bool falling, int lane) {
+  v = sort_merge<1>(v, (lane & 2) == 0, lane);
+  v = sort_merge<2>(v, (lane & 4) == 0, lane);
+  v = sort_merge<4>(v, (lane & 8) == 0, lane);
+  v = sort_merge<8>(v, (lane & 16) == 0, lane);
+  v = sort_merge<16>(v, (lane & 32) == 0, lane);
+  return sort_merge<32>(v, falling, lane);
+}
+
+__device__ __forceinline__ beam_t readlane64(beam_t v, int l) {
+  return static_cast<beam_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
+}
+
+// The 64 largest of a list in order and of a wave's values in none.
+__device__ __forceinline__ beam_t beam_insert(beam_t best, beam_t c, int lane) {
+  c = wave_sort(c, false, lane);
+  return sort_merge<32>(best > c ? best : c, true, lane);
+}
+
+__device__ __forceinline__ double wave_sum64(double v, int lane) {
+  const auto add = [&](beam_t o) { v += __builtin_bit_cast(double, o); };
+  const auto bits = [&] { return __builtin_bit_cast(beam_t, v); };
+  add(lane_xor64<1>(bits(), lane));
+  add(lane_xor64<2>(bits(), lane));
+  add(lane_xor64<4>(bits(), lane));
+  add(lane_xor64<8>(bits(), lane));
+  add(lane_xor64<16>(bits(), lane));
+  add(lane_xor64<32>(bits(), lane));
+  return v;
+}
+
+// A beam that offers no token of its logits: their rows are not read.
+__device__ __forceinline__ bool beam_idle(const BeamArgs& a, long long row) {
+  return (a.ended && a.ended[row]) || !(a.scores[row] > -__builtin_inff());
+}
+
+// Eight logits as they lie in memory.
+template <class T> struct BeamPiece {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  vec8 v;
+  __device__ __forceinline__ float at(int e) const { return static_cast<float>(v[e]); }
+  // What follows converts anew: the 16-bit logits stay in half the registers of their fp32 values.
+  __device__ __forceinline__ void keep() {
+    if constexpr (sizeof(T) == 2) {
+      u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+      asm volatile("" : "+v"(w));
+      v = __builtin_bit_cast(vec8, w);
+    }
+  }
+};
+
+template <class T, int R>
+__global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
+  __shared__ beam_t s_few[4][64 + 512];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const unsigned id = blockIdx.x * 4 + wave;
+  const int row = uniform(id / a.runs), run = id - row * a.runs;
+  if (row >= a.batch * a.beams || beam_idle(a, row)) return;
+  const int b = uniform(row / a.beams), j = row - b * a.beams;
   const T* x = static_cast<const T*>(a.x) + b * a.x_b + j * a.x_j;
-  float top = -__builtin_inff();
-  for (int i = tid; i < a.vocab; i += 256) {
-    const float v = static_cast<float>(x[i]);
-    top = v > top ? v : top;
-  }
-  top = wave_max(top, lane);
-  if (lane == 0) s_f[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
-  double sum = 0.0;
-  for (int i = tid; i < a.vocab; i += 256) {
-    const float v = static_cast<float>(x[i]);
-    if (v > -__builtin_inff()) sum += expf(v - top);
-  }
-  for (int h = 32; h > 0; h >>= 1) sum += __shfl_xor(sum, h);
-  if (lane == 0) s_d[wave] = sum;
-  __syncthreads();
-  if (tid == 0) a.lse[row] = top + log((s_d[0] + s_d[1]) + (s_d[2] + s_d[3]));
-  unsigned long long last = ~0ull;
-  for (int n = 0; n < a.k; ++n) {
-    unsigned long long best = 0;
-    for (int i = tid; i < a.vocab; i += 256) {
-      const uint32_t key = beam_key(static_cast<float>(x[i]));
-      const unsigned long long c = key ? static_cast<unsigned long long>(key) << 32 | ~static_cast<uint32_t>(i) : 0;
-      if (c < last && c > best) best = c;
+  // (pieces of 8 count from the row's first logit, wherever that lies: equal rows have equal sums)
+  const int pieces = static_cast<int>((static_cast<long long>(a.vocab) + 7) / 8);
+  const int first = run * a.per, last = min(pieces, first + a.per);
+  beam_t* few = s_few[wave];
+  const float none = -__builtin_inff();
+
+  beam_t best = 0, least = 0;    // the list, and its k-th
+  float m = ATT_LOW;
+  double total = 0.0;
+  bool begun = false;
+  for (int p0 = first; p0 < last; p0 += 64 * R) {
+    BeamPiece<T> piece[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int p = p0 + 64 * r + lane;
+      const long long i0 = 8ll * p;
+      if (p < last && i0 + 8 <= a.vocab) {
+        __builtin_memcpy(&piece[r].v, x + i0, sizeof(piece[r].v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) piece[r].v[e] = p < last && i0 + e < a.vocab ? x[i0 + e] : static_cast<T>(none);
+      }
     }
-    for (int h = 32; h > 0; h >>= 1) {
-      const unsigned long long o = __shfl_xor(best, h);
-      best = o > best ? o : best;
+    // the maximum (of a NaN and a number fmaxf takes the number)
+    float tops[R], top = none;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      tops[r] = piece[r].at(0);
+#pragma unroll
+      for (int e = 1; e < 8; ++e) tops[r] = fmaxf(tops[r], piece[r].at(e));
+      top = fmaxf(top, tops[r]);
     }
-    __syncthreads();
-    if (lane == 0) s_u[wave] = best;
-    __syncthreads();
-    for (int w = 0; w < 4; ++w) best = s_u[w] > best ? s_u[w] : best;
-    last = best;
-    if (tid == 0) a.best[static_cast<long long>(row) * a.k + n] = make_uint2(best >> 32, ~static_cast<uint32_t>(best));
+    const float most = wave_max(top, lane);
+    if (most == none) continue;
+    const float to = fmaxf(m, most);
+    // the sum: up to 4 R additions in fp32, then in 64 bits
+    float sum[2] = {0.f, 0.f};
+    const auto add_all = [&](auto careful) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum[i] = 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        piece[r].keep();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = __builtin_amdgcn_exp2f((piece[r].at(e) - to) * 1.44269504088896340736f);
+          sum[e & 1] += !decltype(careful)::value || v == v ? v : 0.f;
+        }
+      }
+    };
+    add_all(std::false_type{});
+    if (__any(sum[0] + sum[1] != sum[0] + sum[1])) add_all(std::true_type{});   // not a number among them: those are none
+    total = total * static_cast<double>(__builtin_amdgcn_exp2f((m - to) * 1.44269504088896340736f)) +
+            wave_sum64(static_cast<double>(sum[0]) + static_cast<double>(sum[1]), lane);
+    m = to;
+    // what k of the logits reach
+    const float ranked = wave_sort(top == top ? top : none, true, lane);
+    float bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ranked), a.k - 1));
+    if (least) bound = fmaxf(bound, beam_logit(least));
+    unsigned with = 0;             // rounds that have some
+#pragma unroll
+    for (int r = 0; r < R; ++r) with |= (__any(tops[r] >= bound && tops[r] > none) ? 1u : 0u) << r;
+    int count = 0;
+    while (with || count) {
+      if (with) {
+        const int r = __builtin_ctz(with);
+        with &= with - 1;
+        BeamPiece<T> now = piece[0];
+#pragma unroll
+        for (int i = 1; i < R; ++i)
+          if (r == i) now = piece[i];
+        const uint32_t i0 = 8u * (p0 + 64 * r + lane);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = now.at(e);
+          const beam_t c = static_cast<beam_t>(beam_order(v)) << 32 | ~(i0 + e);
+          const bool is = v >= bound && v > none && c > least;
+          const unsigned long long who = __ballot(is);
+          if (is) few[count + __popcll(who & ((1ull << lane) - 1))] = c;
+          count += __popcll(who);
+        }
+      }
+      // into the list, 64 at a time, the last ones when there are no more
+      while (count >= 64 || (count && !with)) {
+        const int some = min(count, 64);
+        count -= some;
+        __builtin_amdgcn_wave_barrier();
+        const beam_t c = lane < some ? few[count + lane] : 0;
+        best = begun ? beam_insert(best, c, lane) : wave_sort(c, true, lane);
+        begun = true;
+        least = readlane64(best, a.k - 1);
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+  const long long at = static_cast<long long>(row) * a.runs + run;
+  if (lane < a.k) a.best[at * a.k + lane] = best;
+  if (lane == 0) {
+    a.sums[2 * at] = total;
+    a.sums[2 * at + 1] = m;
   }
 }
 
-// One wave a batch element: a beam a lane, its candidates in order; k times the largest of the lanes' first ones.
-__global__ __launch_bounds__(64) void beam_join_kernel(BeamArgs a) {
-  const int lane = threadIdx.x, b = blockIdx.x;
-  const long long row = static_cast<long long>(b) * a.beams + min(lane, a.beams - 1);
-  const double none = -static_cast<double>(__builtin_inff());
-  const bool ended = a.ended && a.ended[row];
-  const double score = a.scores[row], lse = ended ? 0.0 : a.lse[row];
-  int at = 0, token = a.end_token;
-  double value = none;
-  const auto next = [&]() {
-    value = none;
-    if (lane >= a.beams) return;
-    if (ended) {
-      if (at == 0) value = score;
-    } else if (at < a.k) {
-      const uint2 c = a.best[row * a.k + at];
-      token = c.y;
-      if (c.x) value = score + (static_cast<double>(beam_value(c.x)) - lse);
-    }
-    if (!(value > none)) value = none;
-    ++at;
-  };
-  next();
-  for (int n = 0; n < a.k; ++n) {
-    double best = value;
-    int from = lane;
-    for (int h = 1; h < 64; h <<= 1) {
-      const double o = __shfl_xor(best, h);
-      const int f = __shfl_xor(from, h);
-      if (o > best || (o == best && f < from)) {
-        best = o;
-        from = f;
+// Order-preserving bits of a double above -inf.
+__device__ __forceinline__ beam_t beam_order64(double v) {
+  const beam_t u = __builtin_bit_cast(beam_t, v + 0.0);
+  return (u >> 63) ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double beam_value64(beam_t key) {
+  return __builtin_bit_cast(double, (key >> 63) ? key ^ 1ull << 63 : ~key);
+}
+
+// A workgroup a batch element, a wave a beam at a time.
+__global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
+  __shared__ beam_t s_value[BEAM_MOST * BEAM_MOST];
+  __shared__ int32_t s_token[BEAM_MOST * BEAM_MOST];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const int b = blockIdx.x;
+  for (int j = wave; j < a.beams; j += waves) {
+    const long long row = static_cast<long long>(b) * a.beams + j;
+    const double score = a.scores[row];
+    double value = -__builtin_inf();
+    int token = a.end_token;
+    if (beam_idle(a, row)) {
+      if (lane == 0 && a.ended && a.ended[row]) value = score;
+    } else {
+      const bool is = lane < a.runs;
+      const beam_t* list = a.best + (row * a.runs + (is ? lane : 0)) * a.k;
+      beam_t ahead = is ? list[0] : 0;
+      const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0;
+      const float m = is ? static_cast<float>(a.sums[2 * (row * a.runs + lane) + 1]) : ATT_LOW;
+      const float most = wave_max(m, lane);
+      const double lse = static_cast<double>(most) + log(wave_sum64(sum * exp(static_cast<double>(m) - most), lane));
+      // the runs' lists are in order: their first ones, then their second ones ..., until none can pass the k-th
+      beam_t best = 0;
+      for (int i = 0; i < a.k; ++i) {
+        const beam_t c = ahead;
+        if (i + 1 < a.k && is) ahead = list[i + 1];
+        if (i == 0) best = wave_sort(c, true, lane);
+        else if (__any(c > readlane64(best, a.k - 1))) best = beam_insert(best, c, lane);
+        else break;
       }
+      token = static_cast<int>(~static_cast<uint32_t>(best));
+      if (best) value = score + (static_cast<double>(beam_logit(best)) - lse);
     }
-    const int picked = __shfl(token, from);
-    if (lane == 0) {
-      const long long o = static_cast<long long>(b) * a.k + n;
-      const bool is = best > none;
-      a.out_scores[o] = static_cast<float>(best);
-      a.out_beams[o] = is ? from : 0;
-      a.out_tokens[o] = is ? picked : a.end_token;
+    if (lane < a.k) {
+      const bool is = value > -__builtin_inf();
+      s_value[j * a.k + lane] = is ? beam_order64(value) : 0;
+      s_token[j * a.k + lane] = token;
     }
-    if (lane == from) next();
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  // the beams' lists, one a lane: k times the largest of their first ones, equal ones by the lower beam
+  int at = 0, from = 0, token = 0;
+  beam_t mine = 0;
+  const beam_t head = lane < a.beams ? s_value[lane * a.k] : 0;
+  beam_t now = head;
+  for (int n = 0; n < a.k; ++n) {
+    beam_t top = now;
+    const auto larger = [&](beam_t o) { top = o > top ? o : top; };
+    larger(lane_xor64<1>(top, lane));
+    larger(lane_xor64<2>(top, lane));
+    larger(lane_xor64<4>(top, lane));
+    larger(lane_xor64<8>(top, lane));
+    larger(lane_xor64<16>(top, lane));
+    larger(lane_xor64<32>(top, lane));
+    const int winner = top ? __builtin_ctzll(__ballot(now == top)) : 0;
+    const int place = __builtin_amdgcn_readlane(at, winner);
+    if (lane == n) {
+      mine = top;
+      from = winner;
+      token = winner * a.k + place;
+    }
+    if (lane == winner) {
+      ++at;
+      now = at < a.k && lane < a.beams ? s_value[lane * a.k + at] : 0;
+    }
+  }
+  if (lane < a.k) {
+    const long long o = static_cast<long long>(b) * a.k + lane;
+    a.out_scores[o] = mine ? static_cast<float>(beam_value64(mine)) : -__builtin_inff();
+    a.out_beams[o] = mine ? from : 0;
+    a.out_tokens[o] = mine ? s_token[token] : a.end_token;
   }
 }
 

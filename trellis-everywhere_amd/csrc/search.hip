@@ -49,15 +49,33 @@ int validate_beam(int batch, int beams, int vocab, int k) {
 }
 
 struct BeamPlan {
+  int rounds;         // of 512 logits a wave holds: 2, 4, 8 or 16
+  int runs, per;      // waves a beam, pieces of 8 logits of each
   size_t off_best, ws;
 };
 
-BeamPlan beam_plan(int batch, int beams, int k) {
-  const size_t rows = static_cast<size_t>(batch) * beams;
+// The longest runs that leave waves enough, 8 a CU, for the logits to be on their way; a beam has up to 64, each of
+// several rounds then.
+BeamPlan beam_plan(int batch, int beams, int vocab, int k) {
+  const int64_t rows = static_cast<int64_t>(batch) * beams, pieces = (static_cast<int64_t>(vocab) + 7) / 8;
+  const auto runs = [&](int rounds) { return (pieces + 64 * rounds - 1) / (64 * rounds); };
   BeamPlan p;
-  p.off_best = up256(rows * 8);
-  p.ws = p.off_best + up256(rows * k * 8);
+  p.rounds = 16;
+  while (p.rounds > 2 && rows * runs(p.rounds) < 8 * device_cus() && runs(p.rounds / 2) <= BEAM_MOST) p.rounds /= 2;
+  p.runs = static_cast<int>(runs(p.rounds) < BEAM_MOST ? runs(p.rounds) : BEAM_MOST);
+  p.per = static_cast<int>((pieces + p.runs - 1) / p.runs);
+  p.off_best = up256(static_cast<size_t>(rows) * p.runs * 16);
+  p.ws = p.off_best + up256(static_cast<size_t>(rows) * p.runs * k * 8);
   return p;
+}
+
+template <class T>
+void launch_beam_part(const BeamArgs& a, int rounds, unsigned grid, hipStream_t st) {
+  const dim3 block(256);
+  if (rounds == 2) hipLaunchKernelGGL((beam_part_kernel<T, 2>), dim3(grid), block, 0, st, a);
+  else if (rounds == 4) hipLaunchKernelGGL((beam_part_kernel<T, 4>), dim3(grid), block, 0, st, a);
+  else if (rounds == 8) hipLaunchKernelGGL((beam_part_kernel<T, 8>), dim3(grid), block, 0, st, a);
+  else hipLaunchKernelGGL((beam_part_kernel<T, 16>), dim3(grid), block, 0, st, a);
 }
 
 // ---------------------------------------------------------------- pages
@@ -158,7 +176,7 @@ int trellis_beam_workspace_bytes(int batch, int beams, int vocab, int k, size_t*
   if (!bytes) return TRELLIS_ERR_NULL;
   const int v = validate_beam(batch, beams, vocab, k);
   if (v) return v;
-  *bytes = beam_plan(batch, beams, k).ws;
+  *bytes = beam_plan(batch, beams, vocab, k).ws;
   return TRELLIS_OK;
 }
 
@@ -174,11 +192,11 @@ int trellis_beam_select(const void* logits, int64_t batch_stride, int64_t beam_s
   if (!aligned(logits, dtype_size(dtype)) || !aligned(scores, 4) || !aligned(new_scores, 4) || !aligned(new_beams, 4) ||
       !aligned(new_tokens, 4))
     return TRELLIS_ERR_ALIGN;
-  const BeamPlan p = beam_plan(batch, beams, k);
+  const BeamPlan p = beam_plan(batch, beams, vocab, k);
   if (!workspace || ws_bytes < p.ws) return TRELLIS_ERR_WORKSPACE;
   if (!aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
-  const int64_t rows = static_cast<int64_t>(batch) * beams;
-  if (!grid_fits(rows, 256)) return TRELLIS_ERR_BATCH;
+  const int64_t blocks = (static_cast<int64_t>(batch) * beams * p.runs + 3) / 4;
+  if (!grid_fits(blocks, 256) || static_cast<int64_t>(batch) * beams > INT32_MAX) return TRELLIS_ERR_BATCH;
   BeamArgs a;
   a.x = logits;
   a.x_b = batch_stride;
@@ -194,14 +212,16 @@ int trellis_beam_select(const void* logits, int64_t batch_stride, int64_t beam_s
   a.out_beams = new_beams;
   a.out_tokens = new_tokens;
   char* ws = static_cast<char*>(workspace);
-  a.lse = reinterpret_cast<double*>(ws);
-  a.best = reinterpret_cast<uint2*>(ws + p.off_best);
+  a.runs = p.runs;
+  a.per = p.per;
+  a.sums = reinterpret_cast<double*>(ws);
+  a.best = reinterpret_cast<unsigned long long*>(ws + p.off_best);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(rows)), block(256);
-  if (dtype == TRELLIS_F32) hipLaunchKernelGGL(beam_row_kernel<float>, grid, block, 0, st, a);
-  else if (dtype == TRELLIS_F16) hipLaunchKernelGGL(beam_row_kernel<_Float16>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(beam_row_kernel<bf16_t>, grid, block, 0, st, a);
-  hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(64), 0, st, a);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (dtype == TRELLIS_F32) launch_beam_part<float>(a, p.rounds, grid, st);
+  else if (dtype == TRELLIS_F16) launch_beam_part<_Float16>(a, p.rounds, grid, st);
+  else launch_beam_part<bf16_t>(a, p.rounds, grid, st);
+  hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(64 * (beams < 16 ? beams : 16)), 0, st, a);
   return launched();
 }
 
