@@ -25,18 +25,22 @@ int validate_tree(const trellis_kv_cache* c, int q_heads, int tokens, int q_dtyp
   return TRELLIS_OK;
 }
 
+// Types that take the exact form: q or out of another type than the cache's.
+bool tree_exact(const trellis_kv_cache* c, int q_dtype, int out_dtype) { return q_dtype != c->dtype || out_dtype != c->dtype; }
+
 struct TreePlan : TreeChunks {
   int qr;
-  size_t off_ml, ws;
+  size_t off_ml, off_done, ws;
 };
 
-TreePlan tree_plan(const trellis_kv_cache* c, int q_heads, int tokens) {
+TreePlan tree_plan(const trellis_kv_cache* c, int q_heads, int tokens, bool exact) {
   TreePlan p;
-  static_cast<TreeChunks&>(p) = tree_chunks(c->rows, c->heads, q_heads, c->head_dim, tokens, longest(c), device_cus());
-  p.qr = 32 * p.waves;
+  static_cast<TreeChunks&>(p) = tree_chunks(c->rows, c->heads, q_heads, c->head_dim, tokens, longest(c), exact, device_cus());
+  p.qr = 32 * tree_waves(exact);
   const size_t slots = p.aim ? static_cast<size_t>(p.items) * p.qr : 0;
   p.off_ml = up256(slots * c->head_dim * 4);
-  p.ws = p.off_ml + up256(slots * 8);
+  p.off_done = p.off_ml + up256(slots * 8);
+  p.ws = p.off_done + (p.aim ? up256((static_cast<size_t>(p.blocks) / c->heads + 1) * sizeof(TreeBlock)) : 0);
   return p;
 }
 
@@ -116,7 +120,7 @@ int trellis_tree_attention_workspace_bytes(const trellis_kv_cache* cache, int to
   if (!bytes) return TRELLIS_ERR_NULL;
   const int v = validate_tree(cache, q_heads, tokens, q_dtype, out_dtype);
   if (v) return v;
-  *bytes = tree_plan(cache, q_heads, tokens).ws;
+  *bytes = tree_plan(cache, q_heads, tokens, tree_exact(cache, q_dtype, out_dtype)).ws;
   return TRELLIS_OK;
 }
 
@@ -130,7 +134,8 @@ int trellis_tree_attention(const trellis_kv_cache* cache, const void* q, int64_t
   if (!q || !out) return TRELLIS_ERR_NULL;
   const int qs = dtype_size(q_dtype);
   if (!aligned(q, qs) || !aligned(out, 16)) return TRELLIS_ERR_ALIGN;
-  const TreePlan p = tree_plan(cache, q_heads, tokens);
+  const bool exact = tree_exact(cache, q_dtype, out_dtype);
+  const TreePlan p = tree_plan(cache, q_heads, tokens, exact);
   if (p.ws && (!workspace || ws_bytes < p.ws)) return TRELLIS_ERR_WORKSPACE;
   if (p.ws && !aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
   char* ws = static_cast<char*>(workspace);
@@ -154,21 +159,25 @@ int trellis_tree_attention(const trellis_kv_cache* cache, const void* q, int64_t
   a.scale = scale * 1.44269504088896340736f;
   a.part = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float*>(ws + p.off_ml);
+  a.done = reinterpret_cast<TreeBlock*>(ws + p.off_done);
   a.c = cache_of(cache);
   // the chunks, then those that see to tokens of no row
   const int64_t blocks = p.items + (starts ? (static_cast<int64_t>(tokens) + 63) / 64 : 0);
-  const int64_t joins = p.aim ? static_cast<int64_t>(tokens) * cache->heads : 0;
+  // (a block has about its share of the chunks)
+  const int64_t parts = p.aim ? p.items / p.blocks : 1;
+  const int shares = parts >= 16 && cache->head_dim <= 128 ? 4 : parts >= 8 ? 2 : 1;
+  const int rows = tree_join_rows(cache->head_dim, shares), subs = (p.qr + rows - 1) / rows;
+  const int64_t joins = p.aim ? p.blocks * subs : 0;
   // (chunks count the units of all blocks in 32 bits)
   if (!grid_fits(blocks, 256) || !grid_fits(joins, 256) ||
-      (p.aim && (p.items - p.aim) * tree_units(longest(cache)) >= (int64_t(1) << 31)))
+      (p.aim && p.blocks * tree_units(longest(cache)) >= (int64_t(1) << 31)))
     return TRELLIS_ERR_BATCH;
-  l.exact = q_dtype != cache->dtype || out_dtype != cache->dtype;
-  l.waves = p.waves;
+  l.exact = exact;
   l.grid = static_cast<unsigned>(blocks);
   l.stream = static_cast<hipStream_t>(stream);
   if (cache->dtype == TRELLIS_F16) launch_tree_f16(l);
   else launch_tree_bf16(l);
-  if (joins > 0) hipLaunchKernelGGL(tree_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(256), 0, l.stream, a, p.qr);
+  if (joins > 0) hipLaunchKernelGGL(tree_join_kernel, dim3(static_cast<unsigned>(joins)), dim3(256), 0, l.stream, a, p.qr, subs, shares);
   return launched();
 }
 

@@ -64,30 +64,31 @@ __device__ __forceinline__ void tree_none(const TreeArgs& a, int z, int lane) {
   }
 }
 
-// Workgroups that a CU's registers have to hold.
-constexpr int tree_residents(int dp, int wr, bool exact) { return wr == 4 && dp <= 128 && !exact ? 2 : 1; }
+// Blocks of 32 tokens a wave and step, and workgroups that a CU's registers (and LDS) have to hold.
+constexpr int tree_wide(int dp, bool exact) { return dp <= 128 && !exact ? 2 : 1; }
 
 // T: the cache's type. DP: head dims padded to 64, 128 or 256; FULL: d == DP. EXACT: q or out is of another type than the
-// cache's. WR: waves with queries of their own.
-template <class T, int DP, bool FULL, bool EXACT, int WR>
-__global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kernel(TreeArgs a) {
+// cache's.
+template <class T, int DP, bool FULL, bool EXACT>
+__global__ __launch_bounds__(256, tree_wide(DP, EXACT)) void tree_kernel(TreeArgs a) {
   typedef TreeType<T> AT;
   typedef typename AT::vec8 vec8;
   constexpr bool BF = !std::is_same<T, _Float16>::value;
   constexpr int NQ = EXACT ? (BF ? 3 : 2) : 1;            // terms of q
-  constexpr int NP = EXACT ? (BF ? 3 : 2) : WR == 4 ? 1 : 2;   // terms of the weights
+  constexpr int NP = EXACT ? (BF ? 3 : 2) : 1;            // terms of the weights
   constexpr int UP = BF ? 0 : 15;                         // log2 that q's largest element stays below
   constexpr float TOP = BF ? 0.f : ATT_TOP;
-  constexpr int WT = 4 / WR, QR = 32 * WR;
-  constexpr int NB = WR == 4 && DP <= 128 && !EXACT ? 2 : 1;   // times 32 tokens a wave and tile
-  constexpr int TT = 32 * WT * NB;                        // tokens of a tile
+  constexpr int WR = tree_waves(EXACT), WT = 4 / WR, QR = 32 * WR;
+  constexpr int NB = tree_wide(DP, EXACT);                // times 32 tokens a wave and step
+  constexpr int BT = 32 * WT * NB;                        // tokens of a step
   constexpr int KS = DP / 16, EB = DP / 32;               // k-steps of the first product, blocks of dims of the second
   constexpr int CH = DP / 8, ROW = 2 * DP;                // 16-byte pieces and bytes of a row
-  constexpr int PLANE = TT * ROW, STAGE = 2 * PLANE;
-  constexpr int UNITS = TT / 32;                          // loads of 16 rows of keys or values a wave and tile
+  constexpr int SLOT = BT * ROW;                          // bytes of a step's keys, and of its values: two slots of each
+  constexpr int PER = 64 / CH;                            // rows of one load of a wave
+  constexpr int OWN = BT / 4, GROUPS = OWN > 16 ? OWN / 16 : 1;   // rows that a wave loads a step, and their 16-row groups
   constexpr int OP = DP + 4;                              // floats of a row where waves meet
-  static_assert(WR == 4 || (WT - 1) * WR * 32 * (OP + 2) * 4 <= 2 * STAGE, "the waves' sums fit the tiles' memory");
-  __shared__ __align__(1024) char s_kv[2 * STAGE];
+  static_assert(WR == 4 || (WT - 1) * WR * 32 * (OP + 2) * 4 <= 4 * SLOT, "the waves' sums fit the slots' memory");
+  __shared__ __align__(1024) char s_kv[4 * SLOT];
   __shared__ __align__(8) uint8_t s_ok[2][8];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -98,14 +99,24 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
     return;
   }
   const int item = blockIdx.x, pos = uniform(item / a.c.heads), head = uniform(item - pos * a.c.heads);
-  const TreePlace at = tree_find(a, QR, pos, 0, lane);
+  const TreePlace at = tree_find(a, QR, pos, lane);
   const int b = uniform(at.b);
-  if (b < 0) return;
-  const TreeRow row = tree_row(a, b);
+  if (b < 0) {
+    if (a.aim && item == 0 && threadIdx.x == 0) a.done[0].live = 0;   // no row has a token
+    return;
+  }
+  const TreeRow read = tree_row(a, b), row = {uniform(read.first), uniform(read.n), uniform(read.base), uniform(read.len)};
   const int off = uniform(pos - at.before), chunk = uniform(off / at.blocks), block = uniform(at.blocks - 1 - (off - chunk * at.blocks));
   const int stop = uniform(tree_end(row, block, QR, a.group));
   const int size = a.aim ? at.units * TREE_UNIT : 0x7fffffff;
   const int begin = uniform(a.aim ? chunk * size : 0), end = uniform(min(stop, a.aim ? begin + size : stop));
+  if (a.aim && head == 0 && threadIdx.x == 0) {
+    if (chunk == 0) {
+      const int live = (stop + size - 1) / size;
+      a.done[1 + at.skipped + block] = {live, at.before + at.blocks - 1 - block, at.blocks, row.first, row.n * a.group, block};
+    }
+    if (item == 0) a.done[0].live = at.all;
+  }
   if (begin > 0 && begin >= stop) return;
   const bool whole = stop <= size;
   const int d = a.c.d, queries = row.n * a.group;
@@ -122,43 +133,55 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
   const int below = a.parents ? row.base : row.base + token + 1;   // slots that the lane's query sees all of
   int walk = a.parents && fine ? token : -1;              // the ancestor that comes next
 
-  // ---- tiles into LDS
+  // ---- keys and values into LDS, blocks going downwards, the next one's while one is used. A wave loads OWN rows of each, in 16-row groups that lie in one page each.
   const int sstr = static_cast<int>(a.c.slot_stride) * 2;   // bytes
   const unsigned lds = lds_addr(s_kv);
-  constexpr int PER = 64 / CH;                            // rows of one load of a wave
-  const int lr = lane / CH, lp = lane % CH;
   const auto piece_k = [](int r) { return CH == 8 ? (r >> 1) & 7 : r & 15; };
   const auto piece_v = [](int r) { return CH == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
-  const auto pages_of = [&](int t0, int (&pg)[UNITS]) {
+  constexpr int TIMES = (OWN < 16 ? OWN : 16) / PER;         // loads of a group
+  const int half = OWN < 16 ? wave * OWN & 15 : 0, group0 = wave * OWN & ~15;
+  unsigned koff[TIMES], voff[TIMES];                         // the lane's places within a group
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int j = t0 + 16 * ((wave * UNITS + u) >> 1);
-      pg[u] = load_const(a.c.table + b * a.c.table_stride + (min(j, row.len - 1) >> a.c.page_shift));
+  for (int t = 0; t < TIMES; ++t) {
+    const int r = half + t * PER + lane / CH, pk = lane % CH ^ piece_k(r), pv = lane % CH ^ piece_v(r);
+    koff[t] = FULL || 8 * pk < d ? r * sstr + 16 * pk : RSRC_PAST;
+    voff[t] = FULL || 8 * pv < d ? r * sstr + 16 * pv : RSRC_PAST;
+  }
+  const int steps = uniform(end > begin ? (end - begin + BT - 1) / BT : 0);
+  const auto block_at = [&](int i) { return begin + (steps - 1 - i) * BT; };
+  const auto flat = [](uintptr_t p) {   // into scalar registers
+    return static_cast<uintptr_t>(static_cast<unsigned>(uniform(static_cast<int>(p >> 32)))) << 32 |
+           static_cast<unsigned>(uniform(static_cast<int>(p)));
+  };
+  const uintptr_t k_base = flat(reinterpret_cast<uintptr_t>(a.c.k) + 2 * head * a.c.head_stride);
+  const uintptr_t v_base = flat(reinterpret_cast<uintptr_t>(a.c.v) + 2 * head * a.c.head_stride);
+  const int32_t* pages = a.c.table + b * a.c.table_stride;
+  int page[GROUPS];                     // of the next block to load
+  const auto pages_of = [&](int i) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+      page[g] = load_const(pages + (min(block_at(i) + group0 + 16 * g, row.len - 1) >> a.c.page_shift));
+  };
+  // block i, whose pages are known, into the slots `place`
+  const auto load_block = [&](int i, int place) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const int j = block_at(i) + group0 + 16 * g, id = uniform(page[g]);
+      const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(a.c.pages) && j < row.len;
+      const long long at = ok ? 2 * (id * a.c.page_stride + a.c.in_page(j) * static_cast<int>(a.c.slot_stride)) : 0;
+      // (past the row's end, and without a page, zeros)
+      const int bytes = uniform(ok ? min(16, row.len - j) * sstr : 0);
+      const rsrc_t k = make_rsrc(reinterpret_cast<const void*>(flat(k_base + at)), bytes);
+      const rsrc_t v = make_rsrc(reinterpret_cast<const void*>(flat(v_base + at)), bytes);
+      const unsigned to = lds + place * SLOT + (group0 + 16 * g + half) * ROW;
+#pragma unroll
+      for (int t = 0; t < TIMES; ++t) load_lds16<false>(k, uniform(to + t * 1024), koff[t]);
+#pragma unroll
+      for (int t = 0; t < TIMES; ++t) load_lds16<false>(v, uniform(to + 2 * SLOT + t * 1024), voff[t]);
+      if (lane == 0) s_ok[place][group0 / 16 + g] = ok;
     }
   };
-  const auto load_tile = [&](int t0, int buf, const int (&pg)[UNITS]) {
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int id = wave * UNITS + u, g16 = id >> 1, kv = id & 1, j = t0 + 16 * g16;
-      const int page = __builtin_amdgcn_readfirstlane(pg[u]);
-      const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.pages) && j < row.len;
-      const long long at16 = a.c.row_at(ok ? page : 0, head, j);
-      const rsrc_t r = make_rsrc(static_cast<const char*>(kv ? a.c.v : a.c.k) + 2 * at16, ok ? 16 * static_cast<unsigned>(sstr) : 0);
-      const unsigned to = lds + buf * STAGE + kv * PLANE + g16 * 16 * ROW;
-#pragma unroll
-      for (int m = 0; m < 16 / PER; ++m) {
-        const int rr = m * PER + lr, piece = lp ^ (kv ? piece_v(rr) : piece_k(rr));
-        unsigned voff = rr * sstr + 16 * piece;
-        if ((!FULL && 8 * piece >= d) || j + rr >= row.len) voff = RSRC_PAST;
-        load_lds16<false>(r, to + m * 1024, voff);
-      }
-      if (kv == 0 && lane == 0) s_ok[buf][g16] = ok;
-    }
-  };
-
-  const int tiles = end > begin ? (end - begin + TT - 1) / TT : 0;
-  int pg[UNITS];
-  if (tiles > 0) pages_of(begin + (tiles - 1) * TT, pg);
+  if (steps > 0) pages_of(0);
 
   // ---- q: lane (query c32, dims 16 j + 8 h ..), in NQ terms of T; zeros for queries and dims that are none
   vec8 q[NQ][KS];
@@ -225,30 +248,34 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
   const int l16 = lane & 15, vrow = (4 * h + (l16 >> 2)) * ROW;
   const int vx = piece_v(4 * h + (l16 >> 2)) * 16, vcol = 32 * ((lane >> 4) & 1) + 8 * (l16 & 3);
 
-  const auto use_tile = [&](int t0, int buf) {
-    const char* kp = s_kv + buf * STAGE + tw * NB * 32 * ROW;
-    const char* vp = kp + PLANE;
-    // S^T = K Q^T
-    float16_t s[NB];
+  struct Logits {
+    float16_t v[NB];
+  };
+  // (place: the block's slot)
+  // S^T = K Q^T of a block
+  const auto logits = [&](int place) {
+    const char* kp = s_kv + place * SLOT + tw * NB * 32 * ROW + krow;
+    Logits r;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = float16_t{};
+      r.v[nb] = float16_t{};
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        const vec8 k = *reinterpret_cast<const vec8*>(kp + nb * 32 * ROW + krow + ((32 * j) ^ kx));
+        const vec8 k = *reinterpret_cast<const vec8*>(kp + nb * 32 * ROW + ((32 * j) ^ kx));
 #pragma unroll
-        for (int t = 0; t < NQ; ++t) s[nb] = AT::mfma(k, q[t][j], s[nb]);
+        for (int t = 0; t < NQ; ++t) r.v[nb] = AT::mfma(k, q[t][j], r.v[nb]);
       }
     }
-    // what the queries see
-    const unsigned long long okay = *reinterpret_cast<const unsigned long long*>(s_ok[buf]);
-    const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(okay)), hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(okay >> 32));
-    const int j0 = t0 + tw * NB * 32;
-    if (j0 + 32 * NB > plain || (TT > 64 ? (lo & hi) : TT > 32 ? lo : (lo & 0xFFFFu) | 0x01010000u) != 0x01010101u) {
+    return r;
+  };
+  // what the queries see of it, and the maximum
+  const auto settle = [&](Logits& s, int i, int place) {
+    const unsigned flags = uniform(NB == 2 ? *reinterpret_cast<const int*>(s_ok[place] + 4 * tw) : *reinterpret_cast<const uint16_t*>(s_ok[place] + 2 * tw));
+    const int j0 = block_at(i) + 32 * NB * tw;
+    if (j0 + 32 * NB > plain || flags != (NB == 2 ? 0x01010101u : 0x0101u)) {
 #pragma unroll
       for (int nb = NB - 1; nb >= 0; --nb) {
-        const int j = j0 + 32 * nb, g16 = 2 * (tw * NB + nb);
-        const int k = below - j;
+        const int j = j0 + 32 * nb, k = below - j;
         unsigned sees = k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1;
         const int rel = j - row.base;
         while (walk >= 0 && walk >= rel) {
@@ -257,19 +284,18 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
           walk = p >= 0 && p < walk ? p : -1;
         }
         if (!fine) sees = 0;
-        const unsigned flags = (g16 < 4 ? lo : hi) >> (8 * (g16 & 3));
-        if (!(flags & 1)) sees &= 0xFFFF0000u;
-        if (!(flags & 0x100)) sees &= 0x0000FFFFu;
+        if (!(flags >> 16 * nb & 1)) sees &= 0xFFFF0000u;
+        if (!(flags >> 16 * nb & 0x100)) sees &= 0x0000FFFFu;
         sees >>= 4 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[nb][r] = (sees >> (8 * (r / 4) + r % 4)) & 1 ? s[nb][r] : -__builtin_inff();
+        for (int r = 0; r < 16; ++r) s.v[nb][r] = (sees >> (8 * (r / 4) + r % 4)) & 1 ? s.v[nb][r] : -__builtin_inff();
       }
     }
-    float top = s[0][0];
+    float top = s.v[0][0];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s.v[nb][r]);
     top *= fold;
     if (__any(top - m > TOP + ATT_SLACK)) {
       const float most = fmaxf(top, lane_xor<32>(top, lane));
@@ -282,28 +308,30 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
 #pragma unroll
       for (int e = 0; e < EB; ++e) o[e] *= by;
     }
-    // the weights, and out^T += V^T P^T
+  };
+  // the weights of a block, and out^T += V^T P^T
+  const auto accumulate = [&](const Logits& s, int place) {
+    const char* vp = s_kv + (2 + place) * SLOT + tw * NB * 32 * ROW + vrow + vcol;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         vec8 p[NP];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][8 * u + i], fold, -m));
+        for (int r = 0; r < 8; ++r) {
+          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s.v[nb][8 * u + r], fold, -m));
           l += x;
 #pragma unroll
           for (int t = 0; t < NP; ++t) {
             const T part = static_cast<T>(x);
-            p[t][i] = part;
+            p[t][r] = part;
             if (t + 1 < NP) x -= static_cast<float>(part);
           }
         }
-        const char* at16 = vp + (nb * 32 + 16 * u) * ROW + vrow + vcol;
 #pragma unroll
         for (int e = 0; e < EB; ++e) {
           typedef __attribute__((address_space(3))) short4_t* lds4_t;
-          const char* v4 = at16 + ((64 * e) ^ vx);
+          const char* v4 = vp + (nb * 32 + 16 * u) * ROW + ((64 * e) ^ vx);
           const short4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(v4));
           const short4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(v4 + 8 * ROW));
           const vec8 v = __builtin_bit_cast(vec8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -313,17 +341,27 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
       }
   };
 
-  // (the barrier: the tile has arrived for every wave, and none still reads the one whose place the next one takes)
-  const auto arrive = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  if (tiles > 0) {
-    int t = tiles - 1, buf = 0;
-    load_tile(begin + t * TT, 0, pg);
-    if (t > 0) pages_of(begin + (t - 1) * TT, pg);
-    for (; t >= 0; --t, buf ^= 1) {
-      arrive();
-      if (t > 0) load_tile(begin + (t - 1) * TT, buf ^ 1, pg);
-      if (t > 1) pages_of(begin + (t - 2) * TT, pg);
-      if (active) use_tile(begin + t * TT, buf);
+  if (steps > 0) {
+    load_block(0, 0);
+    if (steps > 1) pages_of(1);
+    int i = 0;
+    while (true) {
+#pragma unroll
+      for (int place = 0; place < 2; ++place) {
+        if (i >= steps) break;
+        // the block has arrived, for every wave, and none still reads the one whose place the next one takes
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (i + 1 < steps) load_block(i + 1, 1 - place);
+        if (i + 2 < steps) pages_of(i + 2);
+        if (active) {
+          Logits s = logits(place);
+          settle(s, i, place);
+          accumulate(s, place);
+        }
+        ++i;
+      }
+      if (i >= steps) break;
     }
   }
   l += lane_xor<32>(l, lane);
@@ -402,7 +440,6 @@ __global__ __launch_bounds__(256, tree_residents(DP, WR, EXACT)) void tree_kerne
 struct TreeLaunch {
   TreeArgs a;
   bool exact;
-  int waves;
   unsigned grid;
   hipStream_t stream;
 };
@@ -411,20 +448,18 @@ void launch_tree_f16(const TreeLaunch& l);
 void launch_tree_bf16(const TreeLaunch& l);
 
 template <class T, int DP, bool FULL, bool EXACT>
-void launch_tree_waves(const TreeLaunch& l) {
-  if (l.waves == 4) hipLaunchKernelGGL((tree_kernel<T, DP, FULL, EXACT, 4>), dim3(l.grid), dim3(256), 0, l.stream, l.a);
-  else if (l.waves == 2) hipLaunchKernelGGL((tree_kernel<T, DP, FULL, EXACT, 2>), dim3(l.grid), dim3(256), 0, l.stream, l.a);
-  else if constexpr (DP < 256) hipLaunchKernelGGL((tree_kernel<T, DP, FULL, EXACT, 1>), dim3(l.grid), dim3(256), 0, l.stream, l.a);
+void launch_tree_as(const TreeLaunch& l) {
+  hipLaunchKernelGGL((tree_kernel<T, DP, FULL, EXACT>), dim3(l.grid), dim3(256), 0, l.stream, l.a);
 }
 
 template <class T, int DP>
 void launch_tree_dp(const TreeLaunch& l) {
   if (l.a.c.d == DP) {
-    if (l.exact) launch_tree_waves<T, DP, true, true>(l);
-    else launch_tree_waves<T, DP, true, false>(l);
+    if (l.exact) launch_tree_as<T, DP, true, true>(l);
+    else launch_tree_as<T, DP, true, false>(l);
   } else {
-    if (l.exact) launch_tree_waves<T, DP, false, true>(l);
-    else launch_tree_waves<T, DP, false, false>(l);
+    if (l.exact) launch_tree_as<T, DP, false, true>(l);
+    else launch_tree_as<T, DP, false, false>(l);
   }
 }
 

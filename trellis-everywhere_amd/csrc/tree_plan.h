@@ -15,34 +15,47 @@ constexpr int tree_units(int n) { return (n + TREE_UNIT - 1) / TREE_UNIT; }
 // A row's queries of one key-value head, token by token, are cut into blocks of `qr` = 32 x waves.
 constexpr int tree_blocks(int64_t queries, int qr) { return static_cast<int>((queries + qr - 1) / qr); }
 
-// Units of a chunk.
-constexpr int tree_chunk_units(int units, int aim) {
-  const int even = (units + aim - 1) / aim;
-  return even > TREE_LEAST ? even : TREE_LEAST;
+// The most units of a chunk: an even share of the work (`units` of `blocks` blocks, the longest `most`) for each of `aim`
+// workgroups, two thirds of one where rows are uneven, so that they end together (32 rows of up to 8192 tokens 133 -> 110 us;
+// rows of one length 32.9 -> 37.4).
+constexpr int tree_chunk_units(int units, int blocks, int most, int heads, int aim) {
+  const int64_t work = static_cast<int64_t>(units) * heads;
+  const int shares = 2 * static_cast<int64_t>(most) * blocks > 3 * static_cast<int64_t>(units) ? aim + aim / 2 : aim;
+  const int64_t even = (work + shares - 1) / shares;
+  return static_cast<int>(even > TREE_LEAST ? even : TREE_LEAST);
 }
 
+// Waves of a workgroup's four that have queries of their own; the others share a wave's queries and take other keys. All four
+// for 16-bit types; two where q's and the weights' terms make the products two to six times as many (fp32 queries: 32 rows
+// of 8192 tokens, 1 / 16 / 32 new ones each, two waves 209 / 241 / 419 us, four 332 / 361 / 390, one 205 / 312 / 538).
+constexpr int tree_waves(bool exact) { return exact ? 2 : 4; }
+
 struct TreeChunks {
-  int waves;       // of 32 queries each in a block: 1, 2 or 4 (of a workgroup's four; the others share their keys)
   int aim;         // chunks wanted of the whole work; 0: a block's keys are one chunk
+  int64_t blocks;  // the most blocks of all rows and heads
   int64_t items;   // the most chunks that can be made
 };
 
 // `tokens` new tokens of `rows` rows up to n long, some `tokens` / rows each.
-constexpr TreeChunks tree_chunks(int rows, int heads, int q_heads, int head_dim, int tokens, int n, int cus) {
-  const int group = q_heads / heads;
-  TreeChunks p = {4, 0, 0};
+constexpr TreeChunks tree_chunks(int rows, int heads, int q_heads, int head_dim, int tokens, int n, bool exact, int cus) {
+  const int group = q_heads / heads, qr = 32 * tree_waves(exact);
+  TreeChunks p = {0, 0, 0};
   if (rows < 1) return p;
-  const int64_t queries = static_cast<int64_t>(tokens) * group, each = (queries + rows - 1) / rows;
-  p.waves = each <= 32 && head_dim <= 128 ? 1 : each <= 64 ? 2 : 4;
-  const int qr = 32 * p.waves;
   // every row has one block that is not full, and (where a block holds a token's queries) no more blocks than tokens
+  const int64_t queries = static_cast<int64_t>(tokens) * group;
   int64_t blocks = queries / qr + rows;
   if (group <= qr && blocks > tokens) blocks = tokens;
-  p.items = blocks * heads;
-  const int64_t want = static_cast<int64_t>(cus) * (p.waves == 4 && head_dim <= 128 ? 2 : 1);
-  if (n <= TREE_LEAST * TREE_UNIT || rows > TREE_ROWS || p.items >= want) return p;
+  p.blocks = p.items = blocks * heads;
+  // A share for each CU; two where the products bound the call and a CU's registers hold two workgroups (one or two shares:
+  // a row of 9216 tokens, 1024 new 211 / 180 us, 64 new of 32768 65.1 / 67.6, 24 new 40.7 / 46.0; 8 rows of 4096, 24 new
+  // 39.7 / 42.0, 48 new 62.6 / 54.2; 32 rows of 1024, 8 new 32.9 / 37.4).
+  const bool twice = !exact && head_dim <= 128 && queries > static_cast<int64_t>(rows) * qr;
+  const int64_t want = static_cast<int64_t>(cus) * (twice ? 2 : 1);
+  if (n <= TREE_LEAST * TREE_UNIT || rows > TREE_ROWS || p.items >= 2 * static_cast<int64_t>(cus)) return p;
   p.aim = static_cast<int>(want);
-  p.items += p.aim;
+  // (those that the work is cut into, and every block one that is not full)
+  const int64_t most = p.blocks * tree_units(n) / TREE_LEAST;
+  p.items += most < want + want / 2 ? most : want + want / 2;
   return p;
 }
 

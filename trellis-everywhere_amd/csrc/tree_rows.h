@@ -19,6 +19,7 @@ struct TreeArgs {
   float scale;               // times log2(e)
   float* part;               // [items][queries of a block][d] unnormalised sums of blocks of several chunks
   float* ml;                 // [items][queries of a block][2] their maximum and sum
+  struct TreeBlock* done;    // [blocks of one head + 1] what the join needs of each, their number first
   Cache c;
 };
 
@@ -43,49 +44,71 @@ __device__ __forceinline__ TreeRow tree_row(const TreeArgs& a, int row) {
   return r;
 }
 
+// A block of queries of several chunks, as the join finds it.
+struct __attribute__((aligned(32))) TreeBlock {
+  int live;                  // its chunks
+  int first, step;           // the first one's place in one head's line, and from one to the next
+  int token, queries, block; // the row's first token and its queries, and which of the row's blocks it is
+};
+
 // A row's place in the line of chunks: rows slowest, then its chunks, then its blocks from the last to the first, then
 // heads.
 struct TreePlace {
-  int b, blocks, chunks, before;   // b < 0: no such row
-  int units;                       // of a chunk
+  int b, blocks, chunks;   // b < 0: no such row
+  int before, skipped;     // chunks and blocks of one head of the rows below
+  int all;                 // blocks of all rows (where they are cut into chunks)
+  int units;               // of a chunk of the row
 };
 
-// The row with chunk `pos` of one head's line, or (pos < 0) with token `t`. By a whole wave.
-__device__ __forceinline__ TreePlace tree_find(const TreeArgs& a, int qr, int pos, int t, int lane) {
+// The row of chunk `pos` of one head's line. By a whole wave.
+__device__ __forceinline__ TreePlace tree_find(const TreeArgs& a, int qr, int pos, int lane) {
   constexpr int AHEAD = TREE_ROWS / 64;
-  int units = 0, before = 0;
+  int units = 0, before = 0, skipped = 0, all = 0;
   for (int s = 0; s < a.c.rows; s += TREE_ROWS) {
-    int first[AHEAD], n[AHEAD], blocks[AHEAD], own[AHEAD];
+    int blocks[AHEAD], own[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      first[i] = n[i] = blocks[i] = own[i] = 0;
+      blocks[i] = own[i] = 0;
       if (s + 64 * i >= a.c.rows) continue;
       const TreeRow r = tree_row(a, s + 64 * i + lane);
-      first[i] = r.first;
-      n[i] = r.n;
       blocks[i] = tree_blocks(static_cast<int64_t>(r.n) * a.group, qr);
       own[i] = max(1, tree_units(r.len));
     }
     if (a.aim) {   // (then there are no more rows than these)
-      int all = 0;
+      int work = 0, count = 0, most = 0;
+      bool falls = false;      // starts in no order: no row then, as their tokens could be more than there are
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) all += blocks[i] * own[i];
-      units = tree_chunk_units(__builtin_amdgcn_readlane(wave_scan(all), 63) * a.c.heads, a.aim);
+      for (int i = 0; i < AHEAD; ++i) {
+        if (a.starts && s + 64 * i + lane < a.c.rows)
+          falls = falls || a.starts[s + 64 * i + lane + 1] < a.starts[s + 64 * i + lane];
+        work += blocks[i] * own[i];
+        count += blocks[i];
+        most = max(most, blocks[i] ? own[i] : 0);
+      }
+      work = __builtin_amdgcn_readlane(wave_scan(work), 63);
+      all = __builtin_amdgcn_readlane(wave_scan(count), 63);
+      most = uniform(static_cast<int>(wave_max(static_cast<float>(most), lane)));   // (units: below 2^24)
+      units = tree_chunk_units(work, all, most, a.c.heads, a.aim);
+      if (__any(falls)) break;
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (s + 64 * i >= a.c.rows) continue;
       const int chunks = a.aim ? (own[i] + units - 1) / units : 1, mine = blocks[i] * chunks, scan = wave_scan(mine);
-      const unsigned long long hit = pos < 0 ? __ballot(t >= first[i] && t - first[i] < n[i]) : __ballot(before + scan > pos);
+      const int scan_b = a.aim ? wave_scan(blocks[i]) : scan;
+      const unsigned long long hit = __ballot(before + scan > pos);
       if (hit) {
         const int l = __builtin_ctzll(hit);
-        return {s + 64 * i + l, __builtin_amdgcn_readlane(blocks[i], l), __builtin_amdgcn_readlane(chunks, l),
-                before + __builtin_amdgcn_readlane(scan - mine, l), units};
+        return {s + 64 * i + l, __builtin_amdgcn_readlane(blocks[i], l),
+                __builtin_amdgcn_readlane(chunks, l), before + __builtin_amdgcn_readlane(scan - mine, l),
+                skipped + __builtin_amdgcn_readlane(scan_b - blocks[i], l), all,
+                __builtin_amdgcn_readlane((own[i] + chunks - 1) / chunks, l)};   // (its chunks alike)
       }
       before += __builtin_amdgcn_readlane(scan, 63);
+      skipped += __builtin_amdgcn_readlane(scan_b, 63);
     }
   }
-  return {-1, 0, 0, 0, 0};
+  return {-1, 0, 0, 0, 0, 0, 0};
 }
 
 // The end of the keys that a block of queries can see.
