@@ -16,6 +16,7 @@
 
 namespace trellis {
 
+constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int BEAM_MOST = 64;   // beams, candidates kept of each, runs of a beam (TRELLIS_BEAM_MAX)
 
 struct BeamArgs {
@@ -28,7 +29,7 @@ struct BeamArgs {
   float* out_scores;            // [batch][k]
   int32_t* out_beams;
   int32_t* out_tokens;
-  double* sums;                 // workspace: [batch x beams][runs] (sum of exponentials against the maximum, maximum)
+  double* sums;                 // workspace: [batch x beams][runs] (sum of exponentials, and against which power of e)
   unsigned long long* best;     // workspace: [batch x beams][runs][k] keys in order
 };
 
@@ -76,6 +77,27 @@ __device__ __forceinline__ V wave_sort(V v, bool falling, int lane) {
   return sort_merge<32>(v, falling, lane);
 }
 
+// The same for (value, where it is from): of equal values the lower place counts as larger.
+template <int H>
+__device__ __forceinline__ void pair_merge(beam_t& v, uint32_t& from, bool lower_larger, int lane) {
+  const beam_t o = lane_xor64<H>(v, lane);
+  const uint32_t f = __builtin_bit_cast(uint32_t, lane_xor<H>(__builtin_bit_cast(float, from), lane));
+  const bool larger = lower_larger == ((lane & H) == 0), above = o > v || (o == v && f < from);
+  if (above == larger) {
+    v = o;
+    from = f;
+  }
+  if constexpr (H > 1) pair_merge<H / 2>(v, from, lower_larger, lane);
+}
+__device__ __forceinline__ void pair_sort(beam_t& v, uint32_t& from, bool falling, int lane) {
+  pair_merge<1>(v, from, (lane & 2) == 0, lane);
+  pair_merge<2>(v, from, (lane & 4) == 0, lane);
+  pair_merge<4>(v, from, (lane & 8) == 0, lane);
+  pair_merge<8>(v, from, (lane & 16) == 0, lane);
+  pair_merge<16>(v, from, (lane & 32) == 0, lane);
+  pair_merge<32>(v, from, falling, lane);
+}
+
 __device__ __forceinline__ beam_t readlane64(beam_t v, int l) {
   return static_cast<beam_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l))) << 32 |
          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
@@ -85,6 +107,18 @@ __device__ __forceinline__ beam_t readlane64(beam_t v, int l) {
 __device__ __forceinline__ beam_t beam_insert(beam_t best, beam_t c, int lane) {
   c = wave_sort(c, false, lane);
   return sort_merge<32>(best > c ? best : c, true, lane);
+}
+
+// The largest of the wave's values, in every lane.
+__device__ __forceinline__ beam_t wave_top(beam_t v, int lane) {
+  const auto larger = [&](beam_t o) { v = o > v ? o : v; };
+  larger(lane_xor64<1>(v, lane));
+  larger(lane_xor64<2>(v, lane));
+  larger(lane_xor64<4>(v, lane));
+  larger(lane_xor64<8>(v, lane));
+  larger(lane_xor64<16>(v, lane));
+  larger(lane_xor64<32>(v, lane));
+  return v;
 }
 
 __device__ __forceinline__ double wave_sum64(double v, int lane) {
@@ -136,7 +170,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
 
   beam_t best = 0, least = 0;    // the list, and its k-th
   float m = ATT_LOW;
-  double total = 0.0;
+  double total = 0.0, base = ATT_LOW;    // the sum against exp(base)
   bool begun = false;
   for (int p0 = first; p0 < last; p0 += 64 * R) {
     BeamPiece<T> piece[R];
@@ -163,29 +197,47 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
     const float most = wave_max(top, lane);
     if (most == none) continue;
     const float to = fmaxf(m, most);
-    // the sum: up to 4 R additions in fp32, then in 64 bits
+    // The sum, of 2^(x log2(e) - top log2(e)) with the second product rounded once and kept as it is (its error is no term's
+    // own): up to 4 R additions in fp32, then in 64 bits.
+    const float shift = to * LOG2E;
     float sum[2] = {0.f, 0.f};
     const auto add_all = [&](auto careful) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) sum[i] = 0.f;
+      sum[0] = sum[1] = 0.f;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         piece[r].keep();
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float v = __builtin_amdgcn_exp2f((piece[r].at(e) - to) * 1.44269504088896340736f);
-          sum[e & 1] += !decltype(careful)::value || v == v ? v : 0.f;
+          const float x1 = piece[r].at(e);
+          if constexpr (decltype(careful)::value) {
+            const float v = __builtin_amdgcn_exp2f((x1 - to) * LOG2E);
+            sum[e & 1] += v == v ? v : 0.f;
+          } else {
+            sum[e & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x1, LOG2E, -shift));
+          }
         }
       }
     };
     add_all(std::false_type{});
-    if (__any(sum[0] + sum[1] != sum[0] + sum[1])) add_all(std::true_type{});   // not a number among them: those are none
-    total = total * static_cast<double>(__builtin_amdgcn_exp2f((m - to) * 1.44269504088896340736f)) +
-            wave_sum64(static_cast<double>(sum[0]) + static_cast<double>(sum[1]), lane);
+    double against = static_cast<double>(shift) / static_cast<double>(LOG2E);
+    // (beyond 2^20 half a step of the product is no small power of 2)
+    const bool far = fabsf(to) > 1048576.f;
+    if (!far) add_all(std::false_type{});
+    if (far || __any(sum[0] + sum[1] != sum[0] + sum[1])) {   // not a number among them: those are none
+      add_all(std::true_type{});
+      against = to;
+    }
+    const double mine = static_cast<double>(sum[0]) + static_cast<double>(sum[1]);
+    total = total * static_cast<double>(__builtin_amdgcn_exp2f(static_cast<float>((base - against) * static_cast<double>(LOG2E)))) +
+            wave_sum64(mine, lane);
     m = to;
+    base = against;
     // what k of the logits reach
-    const float ranked = wave_sort(top == top ? top : none, true, lane);
-    float bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ranked), a.k - 1));
+    float bound = most;
+    if (a.k > 1) {
+      const float ranked = wave_sort(top == top ? top : none, true, lane);
+      bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ranked), a.k - 1));
+    }
     if (least) bound = fmaxf(bound, beam_logit(least));
     unsigned with = 0;             // rounds that have some
 #pragma unroll
@@ -199,12 +251,19 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
 #pragma unroll
         for (int i = 1; i < R; ++i)
           if (r == i) now = piece[i];
+        now.keep();
         const uint32_t i0 = 8u * (p0 + 64 * r + lane);
+        unsigned have = 0;         // the lane's logits that reach the bound: mostly one of a few lanes
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = now.at(e);
+        for (int e = 0; e < 8; ++e) have |= (now.at(e) >= bound && now.at(e) > none ? 1u : 0u) << e;
+        while (__any(have != 0)) {
+          const int e = have ? __builtin_ctz(have) : 0;
+          float v = now.at(0);
+#pragma unroll
+          for (int i = 1; i < 8; ++i) v = e == i ? now.at(i) : v;
           const beam_t c = static_cast<beam_t>(beam_order(v)) << 32 | ~(i0 + e);
-          const bool is = v >= bound && v > none && c > least;
+          const bool is = have && c > least;
+          have &= have - 1;
           const unsigned long long who = __ballot(is);
           if (is) few[count + __popcll(who & ((1ull << lane) - 1))] = c;
           count += __popcll(who);
@@ -216,7 +275,8 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
         count -= some;
         __builtin_amdgcn_wave_barrier();
         const beam_t c = lane < some ? few[count + lane] : 0;
-        best = begun ? beam_insert(best, c, lane) : wave_sort(c, true, lane);
+        if (a.k == 1) best = wave_top(c > best ? c : best, lane);
+        else best = begun ? beam_insert(best, c, lane) : wave_sort(c, true, lane);
         begun = true;
         least = readlane64(best, a.k - 1);
         __builtin_amdgcn_wave_barrier();
@@ -227,7 +287,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   if (lane < a.k) a.best[at * a.k + lane] = best;
   if (lane == 0) {
     a.sums[2 * at] = total;
-    a.sums[2 * at + 1] = m;
+    a.sums[2 * at + 1] = base;
   }
 }
 
@@ -256,20 +316,27 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
     } else {
       const bool is = lane < a.runs;
       const beam_t* list = a.best + (row * a.runs + (is ? lane : 0)) * a.k;
-      beam_t ahead = is ? list[0] : 0;
-      const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0;
-      const float m = is ? static_cast<float>(a.sums[2 * (row * a.runs + lane) + 1]) : ATT_LOW;
-      const float most = wave_max(m, lane);
-      const double lse = static_cast<double>(most) + log(wave_sum64(sum * exp(static_cast<double>(m) - most), lane));
-      // the runs' lists are in order: their first ones, then their second ones ..., until none can pass the k-th
-      beam_t best = 0;
-      for (int i = 0; i < a.k; ++i) {
-        const beam_t c = ahead;
-        if (i + 1 < a.k && is) ahead = list[i + 1];
-        if (i == 0) best = wave_sort(c, true, lane);
-        else if (__any(c > readlane64(best, a.k - 1))) best = beam_insert(best, c, lane);
-        else break;
-      }
+      // the lists' first ones at once: seldom more of a list are looked at
+      constexpr int AHEAD = 4;
+      beam_t head[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) head[i] = is && i < a.k ? list[i] : 0;
+      const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0, base = is ? a.sums[2 * (row * a.runs + lane) + 1] : ATT_LOW;
+      const float most = wave_max(static_cast<float>(base), lane);
+      // (one lane's, for all: each one's first addition takes its own product unrounded)
+      const double each = static_cast<double>(most) + log(wave_sum64(sum * exp(base - static_cast<double>(most)), lane));
+      const double lse = __builtin_bit_cast(double, readlane64(__builtin_bit_cast(beam_t, each), 0));
+      // the lists are in order: their first ones, then their second ones ..., until none can pass the k-th
+      beam_t best = a.k == 1 ? wave_top(head[0], lane) : wave_sort(head[0], true, lane);
+      const auto more = [&](beam_t c) {
+        if (!__any(c > readlane64(best, a.k - 1))) return false;
+        best = beam_insert(best, c, lane);
+        return true;
+      };
+      bool go = a.k > 1;
+#pragma unroll
+      for (int i = 1; i < AHEAD; ++i) go = go && more(head[i]);
+      for (int i = AHEAD; go && i < a.k; ++i) go = more(is ? list[i] : 0);
       token = static_cast<int>(~static_cast<uint32_t>(best));
       if (best) value = score + (static_cast<double>(beam_logit(best)) - lse);
     }
@@ -281,37 +348,37 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
   }
   __syncthreads();
   if (wave > 0) return;
-  // the beams' lists, one a lane: k times the largest of their first ones, equal ones by the lower beam
-  int at = 0, from = 0, token = 0;
-  beam_t mine = 0;
-  const beam_t head = lane < a.beams ? s_value[lane * a.k] : 0;
-  beam_t now = head;
-  for (int n = 0; n < a.k; ++n) {
-    beam_t top = now;
-    const auto larger = [&](beam_t o) { top = o > top ? o : top; };
-    larger(lane_xor64<1>(top, lane));
-    larger(lane_xor64<2>(top, lane));
-    larger(lane_xor64<4>(top, lane));
-    larger(lane_xor64<8>(top, lane));
-    larger(lane_xor64<16>(top, lane));
-    larger(lane_xor64<32>(top, lane));
-    const int winner = top ? __builtin_ctzll(__ballot(now == top)) : 0;
-    const int place = __builtin_amdgcn_readlane(at, winner);
-    if (lane == n) {
-      mine = top;
-      from = winner;
-      token = winner * a.k + place;
-    }
-    if (lane == winner) {
-      ++at;
-      now = at < a.k && lane < a.beams ? s_value[lane * a.k + at] : 0;
+  // the beams' lists together, by the value and then the beam: their first 64 / beams candidates, then the next, until none
+  // can pass the k-th
+  const int per = 64 / a.beams, mine = lane / per, nth = lane - mine * per;
+  beam_t best = 0;
+  uint32_t from = ~0u;       // beam x k + place
+  for (int i0 = 0; i0 < a.k; i0 += per) {
+    const int at = mine * a.k + i0 + nth;
+    const bool is = mine < a.beams && i0 + nth < a.k;
+    beam_t c = is ? s_value[at] : 0;
+    uint32_t f = is && c ? at : ~0u;
+    if (i0 > 0) {
+      // (an equal one passes only if its beam is lower)
+      const beam_t last = readlane64(best, a.k - 1);
+      const uint32_t last_from = __builtin_amdgcn_readlane(from, a.k - 1);
+      if (!__any(c > last || (c == last && f < last_from))) break;
+      pair_sort(c, f, false, lane);
+      const bool lower = c > best || (c == best && f < from);
+      best = lower ? c : best;
+      from = lower ? f : from;
+      pair_merge<32>(best, from, true, lane);
+    } else {
+      pair_sort(c, f, true, lane);
+      best = c;
+      from = f;
     }
   }
   if (lane < a.k) {
     const long long o = static_cast<long long>(b) * a.k + lane;
-    a.out_scores[o] = mine ? static_cast<float>(beam_value64(mine)) : -__builtin_inff();
-    a.out_beams[o] = mine ? from : 0;
-    a.out_tokens[o] = mine ? s_token[token] : a.end_token;
+    a.out_scores[o] = best ? static_cast<float>(beam_value64(best)) : -__builtin_inff();
+    a.out_beams[o] = best ? from / a.k : 0;
+    a.out_tokens[o] = best ? s_token[from] : a.end_token;
   }
 }
 
