@@ -6,9 +6,9 @@
 // beams may be nearer to each other than a rounding to 32 bits.
 //
 // beam_part_kernel: a wave takes a run of a beam's logits, R x 512 at a time, read once and held in registers: their
-// maximum, the sum of their exponentials, and their k best. Of the lanes' maxima, sorted across the wave, the k-th is a
-// bound that k of the logits reach: the few that do (k and a handful) are gathered through LDS and sorted by (logit, token)
-// into the wave's list of 64.
+// maximum, the sum of their exponentials, and their k best. Of the maxima of the 256 lanes of four waves side by side, sorted
+// across each wave and merged, the k-th is a bound that k of their logits reach: the few that do (k and a handful) are
+// gathered through LDS and sorted by (logit, token) into each wave's list of 64.
 // beam_join_kernel, a workgroup a batch element: per beam the runs' sums and lists, then the beams' lists.
 #pragma once
 
@@ -156,10 +156,11 @@ template <class T> struct BeamPiece {
 template <class T, int R>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   __shared__ beam_t s_few[4][64 + 512];
+  __shared__ float s_top[4][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const unsigned id = blockIdx.x * 4 + wave;
-  const int row = uniform(id / a.runs), run = id - row * a.runs;
-  if (row >= a.batch * a.beams || beam_idle(a, row)) return;
+  // a workgroup's four waves take runs of one beam
+  const int quads = a.runs / 4, row = uniform(blockIdx.x / quads), run = (blockIdx.x - row * quads) * 4 + wave;
+  if (beam_idle(a, row)) return;
   const int b = uniform(row / a.beams), j = row - b * a.beams;
   const T* x = static_cast<const T*>(a.x) + b * a.x_b + j * a.x_j;
   // (pieces of 8 count from the row's first logit, wherever that lies: equal rows have equal sums)
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   float m = ATT_LOW;
   double total = 0.0, base = ATT_LOW;    // the sum against exp(base)
   bool begun = false;
-  for (int p0 = first; p0 < last; p0 += 64 * R) {
+  for (int p0 = first; p0 < first + a.per; p0 += 64 * R) {
     BeamPiece<T> piece[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -195,6 +196,18 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
       top = fmaxf(top, tops[r]);
     }
     const float most = wave_max(top, lane);
+    // what k of the workgroup's logits reach
+    float bound = a.k > 1 ? wave_sort(top == top ? top : none, true, lane) : most;
+    __syncthreads();
+    s_top[wave][lane] = bound;
+    __syncthreads();
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      if (a.k > 1) bound = sort_merge<32>(fmaxf(bound, s_top[wave ^ w][63 - lane]), true, lane);
+      else bound = fmaxf(bound, s_top[wave ^ w][lane]);
+    }
+    bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bound), a.k > 1 ? a.k - 1 : 0));
+    bound = fmaxf(bound, least ? beam_logit(least) : -__FLT_MAX__);
     if (most == none) continue;
     const float to = fmaxf(m, most);
     // The sum, of 2^(x log2(e) - top log2(e)) with the second product rounded once and kept as it is (its error is no term's
@@ -232,16 +245,9 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
             wave_sum64(mine, lane);
     m = to;
     base = against;
-    // what k of the logits reach
-    float bound = most;
-    if (a.k > 1) {
-      const float ranked = wave_sort(top == top ? top : none, true, lane);
-      bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ranked), a.k - 1));
-    }
-    if (least) bound = fmaxf(bound, beam_logit(least));
     unsigned with = 0;             // rounds that have some
 #pragma unroll
-    for (int r = 0; r < R; ++r) with |= (__any(tops[r] >= bound && tops[r] > none) ? 1u : 0u) << r;
+    for (int r = 0; r < R; ++r) with |= (__any(tops[r] >= bound) ? 1u : 0u) << r;
     int count = 0;
     while (with || count) {
       if (with) {
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
         const uint32_t i0 = 8u * (p0 + 64 * r + lane);
         unsigned have = 0;         // the lane's logits that reach the bound: mostly one of a few lanes
 #pragma unroll
-        for (int e = 0; e < 8; ++e) have |= (now.at(e) >= bound && now.at(e) > none ? 1u : 0u) << e;
+        for (int e = 0; e < 8; ++e) have |= (now.at(e) >= bound ? 1u : 0u) << e;
         while (__any(have != 0)) {
           const int e = have ? __builtin_ctz(have) : 0;
           float v = now.at(0);

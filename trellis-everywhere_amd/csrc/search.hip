@@ -62,7 +62,8 @@ struct BeamPlan {
 // several rounds then.
 BeamPlan beam_plan(int batch, int beams, int vocab, int k) {
   const int64_t rows = static_cast<int64_t>(batch) * beams, pieces = (static_cast<int64_t>(vocab) + 7) / 8;
-  const auto runs = [&](int rounds) { return (pieces + 64 * rounds - 1) / (64 * rounds); };
+  // (a workgroup's four waves share a beam)
+  const auto runs = [&](int rounds) { return (pieces + 256 * rounds - 1) / (256 * rounds) * 4; };
   BeamPlan p;
   p.rounds = 16;
   while (p.rounds > 2 && rows * runs(p.rounds) < 8 * device_cus() && runs(p.rounds / 2) <= BEAM_MOST) p.rounds /= 2;
@@ -204,7 +205,7 @@ int trellis_beam_select(const void* logits, int64_t batch_stride, int64_t beam_s
   const BeamPlan p = beam_plan(batch, beams, vocab, k);
   if (!workspace || ws_bytes < p.ws) return TRELLIS_ERR_WORKSPACE;
   if (!aligned(workspace, 256)) return TRELLIS_ERR_ALIGN;
-  const int64_t blocks = (static_cast<int64_t>(batch) * beams * p.runs + 3) / 4;
+  const int64_t blocks = static_cast<int64_t>(batch) * beams * (p.runs / 4);
   if (!grid_fits(blocks, 256) || static_cast<int64_t>(batch) * beams > INT32_MAX) return TRELLIS_ERR_BATCH;
   BeamArgs a;
   a.x = logits;
