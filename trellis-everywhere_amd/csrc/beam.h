@@ -30,7 +30,7 @@ struct BeamArgs {
   int32_t* out_beams;
   int32_t* out_tokens;
   double* sums;                 // workspace: [batch x beams][runs] (sum of exponentials, and against which power of e)
-  unsigned long long* best;     // workspace: [batch x beams][runs][k] keys in order
+  unsigned long long* best;     // workspace: [batch x beams][runs / 4][k] keys in order
 };
 
 typedef unsigned long long beam_t;   // a candidate: (order-preserving logit, ~token); 0: none
@@ -289,12 +289,23 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
       }
     }
   }
-  const long long at = static_cast<long long>(row) * a.runs + run;
-  if (lane < a.k) a.best[at * a.k + lane] = best;
   if (lane == 0) {
+    const long long at = static_cast<long long>(row) * a.runs + run;
     a.sums[2 * at] = total;
     a.sums[2 * at + 1] = base;
   }
+  // the four lists as one
+  __syncthreads();
+  few[lane] = best;
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    const beam_t c = s_few[w][63 - lane];
+    best = best > c ? best : c;
+    if (a.k > 1) best = sort_merge<32>(best, true, lane);
+  }
+  if (lane < a.k) a.best[static_cast<long long>(blockIdx.x) * a.k + lane] = best;
 }
 
 // Order-preserving bits of a double above -inf.
@@ -321,28 +332,23 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
       if (lane == 0 && a.ended && a.ended[row]) value = score;
     } else {
       const bool is = lane < a.runs;
-      const beam_t* list = a.best + (row * a.runs + (is ? lane : 0)) * a.k;
-      // the lists' first ones at once: seldom more of a list are looked at
-      constexpr int AHEAD = 4;
-      beam_t head[AHEAD];
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) head[i] = is && i < a.k ? list[i] : 0;
+      // the lists, as many of each one's first entries at once as lanes hold
+      const int lists = a.runs / 4, per = 64 / lists, of = lane / per, nth = lane - of * per;
+      const beam_t* list = a.best + (row * lists + min(of, lists - 1)) * a.k;
+      const auto entry = [&](int i) { return of < lists && i + nth < a.k ? list[i + nth] : 0; };
+      const beam_t first = entry(0), second = entry(per);
       const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0, base = is ? a.sums[2 * (row * a.runs + lane) + 1] : ATT_LOW;
       const float most = wave_max(static_cast<float>(base), lane);
       // (one lane's, for all: each one's first addition takes its own product unrounded)
       const double each = static_cast<double>(most) + log(wave_sum64(sum * exp(base - static_cast<double>(most)), lane));
       const double lse = __builtin_bit_cast(double, readlane64(__builtin_bit_cast(beam_t, each), 0));
-      // the lists are in order: their first ones, then their second ones ..., until none can pass the k-th
-      beam_t best = a.k == 1 ? wave_top(head[0], lane) : wave_sort(head[0], true, lane);
-      const auto more = [&](beam_t c) {
-        if (!__any(c > readlane64(best, a.k - 1))) return false;
+      // they are in order: no further ones when none of these can pass the k-th
+      beam_t best = a.k == 1 ? wave_top(first, lane) : wave_sort(first, true, lane);
+      for (int i = per; i < a.k; i += per) {
+        const beam_t c = i == per ? second : entry(i);
+        if (!__any(c > readlane64(best, a.k - 1))) break;
         best = beam_insert(best, c, lane);
-        return true;
-      };
-      bool go = a.k > 1;
-#pragma unroll
-      for (int i = 1; i < AHEAD; ++i) go = go && more(head[i]);
-      for (int i = AHEAD; go && i < a.k; ++i) go = more(is ? list[i] : 0);
+      }
       token = static_cast<int>(~static_cast<uint32_t>(best));
       if (best) value = score + (static_cast<double>(beam_logit(best)) - lse);
     }

@@ -70,7 +70,7 @@ BeamPlan beam_plan(int batch, int beams, int vocab, int k) {
   p.runs = static_cast<int>(runs(p.rounds) < BEAM_MOST ? runs(p.rounds) : BEAM_MOST);
   p.per = static_cast<int>((pieces + p.runs - 1) / p.runs);
   p.off_best = up256(static_cast<size_t>(rows) * p.runs * 16);
-  p.ws = p.off_best + up256(static_cast<size_t>(rows) * p.runs * k * 8);
+  p.ws = p.off_best + up256(static_cast<size_t>(rows) * (p.runs / 4) * k * 8);
   return p;
 }
 
