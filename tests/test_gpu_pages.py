@@ -64,6 +64,31 @@ def test_copies_of_one_layer_and_without_planes(te, gpu_device):
     same(scores, P.scores), same(pos, ref.copy_pages([P.pos], [0, 1], [5, 6])[0])
 
 
+def test_layers_in_one_tensor(te, gpu_device):
+    """Stacked layers, contiguous or a slice of a larger stack, give what a list of them gives."""
+    P = Pages([60, 33], 2, 16, 64, F16, 9, idle=None, spare=6)
+    host, _ = _layers(P, 5, gpu_device)
+    stack = [torch.stack(t).to(gpu_device) for t in host]
+    every = [torch.cat([t, t])[::2] for t in stack]      # layers 0, 2, 4, 1, 3, two strides apart
+    ints = lambda t: torch.tensor(t, dtype=torch.int32, device=gpu_device)
+    src, dst, starts, path = ints([0, 1]), ints([3, 2]), ints([0, 10, 20]), ints([[0, 3, 8, -1], [1, 2, 5, 9]])
+    for k, v, s, z in (stack, every):
+        lists = [[u.clone() for u in t] for t in (k, v, s, z)]
+        te.copy_pages(k, v, src, dst, scores=s, pos=z)
+        te.copy_pages(lists[0], lists[1], src, dst, scores=lists[2], pos=lists[3])
+        table, lens = P.table.to(gpu_device), P.lens.to(gpu_device)
+        a = te.keep_kv(k, v, table, lens, starts, path, scores=s, pos=z)
+        assert torch.equal(a, te.keep_kv(lists[0], lists[1], table, lens, starts, path, scores=lists[2], pos=lists[3]))
+        for got, want in zip((k, v, s, z), lists):
+            assert torch.equal(got.nan_to_num(0), torch.stack(want).nan_to_num(0))
+    k, v, s, z = stack
+    for bad in (lambda: te.copy_pages(k, v[:4], src, dst), lambda: te.copy_pages(k, list(v), src, dst), lambda: te.copy_pages(list(k), v, src, dst),
+                lambda: te.copy_pages(k, v, src, dst, scores=s[0]), lambda: te.copy_pages(k, v, src, dst, pos=list(z)), lambda: te.copy_pages(k[:0], v[:0], src, dst),
+                lambda: te.copy_pages(k[0], v, src, dst), lambda: te.copy_pages(list(k), list(v), src, dst, scores=s)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bad()
+
+
 def test_copies_of_pages_that_are_none(te, gpu_device):
     """Ids outside the pool, and a page onto itself, copy nothing; no pages at all are no error."""
     P = Pages([100], 2, 16, 64, F16, 2, idle=None)

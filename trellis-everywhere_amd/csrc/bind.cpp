@@ -254,14 +254,10 @@ struct CacheView {
   int device;
 };
 
-// k_pages, v_pages, scores, pos, table, lens of a call (table and lens None: one that takes none); max_len None: all that
-// the table can hold.
-CacheView cache_view(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject* pos_o, PyObject* table_o, PyObject* lens_o,
-                     PyObject* max_len) {
-  const at::Tensor &k = tensor(k_o, "k_pages"), &v = tensor(v_o, "v_pages");
-  const bool rows = table_o != Py_None || lens_o != Py_None;
-  const at::Tensor *table = rows ? &tensor(table_o, "table") : nullptr, *lens = rows ? &tensor(lens_o, "lens") : nullptr;
-  const at::Tensor *scores = optional_tensor(scores_o, "scores"), *pos = optional_tensor(pos_o, "pos");
+// A call's cache (no table and lens: one that takes none); max_len None: all that the table can hold.
+CacheView view_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor* scores, const at::Tensor* pos,
+                  const at::Tensor* table, const at::Tensor* lens, PyObject* max_len) {
+  const bool rows = table != nullptr;
   if (!on_gpu(k)) refuse("the cache lives on a GPU");
   const int device = index_of(k);
   if (k.dim() != 4 || v.sizes() != k.sizes() || v.strides() != k.strides() || v.scalar_type() != k.scalar_type())
@@ -288,6 +284,14 @@ CacheView cache_view(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject*
          static_cast<int32_t>(height), static_cast<int32_t>(width),
          max_len == Py_None ? static_cast<int32_t>(std::min<int64_t>(width * k.size(2), 1 << 30)) : whole(max_len, "max_len")};
   return w;
+}
+
+// k_pages, v_pages, scores, pos, table, lens of a call.
+CacheView cache_view(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject* pos_o, PyObject* table_o, PyObject* lens_o,
+                     PyObject* max_len) {
+  const at::Tensor &k = tensor(k_o, "k_pages"), &v = tensor(v_o, "v_pages"), &table = tensor(table_o, "table"),
+                   &lens = tensor(lens_o, "lens");
+  return view_of(k, v, optional_tensor(scores_o, "scores"), optional_tensor(pos_o, "pos"), &table, &lens, max_len);
 }
 
 // Scratch of a call: the caller's, or a block of torch's allocator, which hands it on in stream order.
@@ -496,47 +500,79 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// The tensors of a model's layers: one tensor, or a list or tuple with one for each layer. None: no layer has one.
-struct PerLayer {
-  PyObject* const* items;
-  Py_ssize_t n;
-  PyObject* alone;
-  PerLayer(PyObject* o, const char* name) : alone(o) {
-    if (PyList_Check(o) || PyTuple_Check(o)) {
-      items = PySequence_Fast_ITEMS(o);
-      n = PySequence_Fast_GET_SIZE(o);
-      if (n == 0) refuse("%s holds no layer", name);
-    } else {
-      items = nullptr;
-      n = o == Py_None ? 0 : 1;
-    }
-  }
-  PyObject* operator[](Py_ssize_t i) const { return n == 0 ? Py_None : items ? items[i] : alone; }
-  void all_written() const {
-    for (Py_ssize_t i = 0; i < n; ++i) written((*this)[i]);
-  }
-};
-
-// One cache a layer; table and lens None: a call that takes none.
+// One cache a layer, of k_pages, v_pages, scores and pos (or None) as one layer's tensor, a list or tuple with one for each
+// layer (None for a layer without scores or pos), or one tensor with the layers as its first dim. table and lens None: a
+// call that takes none.
 struct LayerViews {
-  PerLayer k, v, scores, pos;
   std::vector<trellis_kv_cache> c;
-  int device;
-  LayerViews(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject* pos_o, PyObject* table, PyObject* lens)
-      : k(k_o, "k_pages"), v(v_o, "v_pages"), scores(scores_o, "scores"), pos(pos_o, "pos") {
-    if (v.n != k.n || (scores.n && scores.n != k.n) || (pos.n && pos.n != k.n))
-      refuse("k_pages, v_pages, scores and pos must have as many layers");
-    if (k.n > INT16_MAX) refuse("too many layers");
-    c.reserve(k.n);
-    for (Py_ssize_t i = 0; i < k.n; ++i) {
-      const CacheView w = cache_view(k[i], v[i], scores[i], pos[i], table, lens, Py_None);
-      if (i && w.device != device) refuse("the layers must be on one device");
-      device = w.device;
-      c.push_back(w.c);
+  std::vector<PyObject*> into;    // the tensors that the call writes into
+  c10::Device where{c10::kCPU};
+  int device = -1;
+
+  LayerViews(PyObject* k, PyObject* v, PyObject* scores, PyObject* pos, PyObject* table_o, PyObject* lens_o) {
+    const bool rows = table_o != Py_None || lens_o != Py_None;
+    const at::Tensor *table = rows ? &tensor(table_o, "table") : nullptr, *lens = rows ? &tensor(lens_o, "lens") : nullptr;
+    const bool listed = PyList_Check(k) || PyTuple_Check(k);
+    if (!listed && tensor(k, "k_pages").dim() == 5) stacked(k, v, scores, pos, table, lens);
+    else each(k, v, scores, pos, listed, table, lens);
+  }
+
+  void each(PyObject* k, PyObject* v, PyObject* scores, PyObject* pos, bool listed, const at::Tensor* table, const at::Tensor* lens) {
+    PyObject* from[4] = {k, v, scores, pos};
+    const char* names[4] = {"k_pages", "v_pages", "scores", "pos"};
+    const Py_ssize_t layers = listed ? PySequence_Fast_GET_SIZE(k) : 1;
+    if (layers < 1 || layers > INT16_MAX) refuse("k_pages must hold 1 to %d layers", INT16_MAX);
+    for (int i = 1; i < 4; ++i) {
+      const bool list = PyList_Check(from[i]) || PyTuple_Check(from[i]);
+      if (from[i] != Py_None && (list ? PySequence_Fast_GET_SIZE(from[i]) != layers : layers != 1))
+        refuse("%s must have as many layers as k_pages: %d", names[i], static_cast<int>(layers));
+    }
+    c.reserve(layers);
+    into.reserve(4 * layers);
+    for (Py_ssize_t l = 0; l < layers; ++l) {
+      const at::Tensor* t[4];
+      for (int i = 0; i < 4; ++i) {
+        PyObject* o = PyList_Check(from[i]) || PyTuple_Check(from[i]) ? PySequence_Fast_GET_ITEM(from[i], l) : from[i];
+        t[i] = i < 2 ? &tensor(o, names[i]) : optional_tensor(o, names[i]);
+        if (t[i]) into.push_back(o);
+      }
+      take(view_of(*t[0], *t[1], t[2], t[3], table, lens, Py_None), *t[0]);
     }
   }
+
+  void stacked(PyObject* k_o, PyObject* v_o, PyObject* scores_o, PyObject* pos_o, const at::Tensor* table, const at::Tensor* lens) {
+    const at::Tensor &k = tensor(k_o, "k_pages"), &v = tensor(v_o, "v_pages");
+    const at::Tensor *scores = optional_tensor(scores_o, "scores"), *pos = optional_tensor(pos_o, "pos");
+    const int64_t layers = k.size(0);
+    if (layers < 1 || layers > INT16_MAX) refuse("k_pages must hold 1 to %d layers", INT16_MAX);
+    for (const at::Tensor* t : {&v, scores, pos})
+      if (t && (t->dim() != (t == &v ? 5 : 4) || t->size(0) != layers))
+        refuse("v_pages, scores and pos must hold the layers as k_pages does: %lld first", static_cast<long long>(layers));
+    const auto first = [](const at::Tensor* t) { return t ? t->select(0, 0) : at::Tensor(); };
+    const at::Tensor k0 = first(&k), v0 = first(&v), s0 = first(scores), p0 = first(pos);
+    take(view_of(k0, v0, scores ? &s0 : nullptr, pos ? &p0 : nullptr, table, lens, Py_None), k0);
+    c.reserve(layers);
+    for (int64_t l = 1; l < layers; ++l) {
+      trellis_kv_cache one = c[0];
+      one.k = static_cast<char*>(one.k) + l * k.stride(0) * 2;
+      one.v = static_cast<char*>(one.v) + l * v.stride(0) * 2;
+      if (scores) one.scores += l * scores->stride(0);
+      if (pos) one.pos += l * pos->stride(0);
+      c.push_back(one);
+    }
+    for (PyObject* o : {k_o, v_o, scores_o, pos_o})
+      if (o != Py_None) into.push_back(o);
+  }
+
+  void take(const CacheView& w, const at::Tensor& k) {
+    if (!c.empty() && w.device != device) refuse("the layers must be on one device");
+    device = w.device;
+    where = k.device();
+    c.push_back(w.c);
+  }
+
   void all_written() const {
-    for (const PerLayer* p : {&k, &v, &scores, &pos}) p->all_written();
+    for (PyObject* o : into) written(o);
   }
 };
 
@@ -545,8 +581,8 @@ PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     count(n, 7, "copy_pages");
     const LayerViews w(a[0], a[1], a[5], a[6], Py_None, Py_None);
-    const at::Tensor &src = tensor(a[2], "src"), &first = THPVariable_Unpack(w.k[0]);
-    const c10::DeviceGuard guard(first.device());
+    const at::Tensor& src = tensor(a[2], "src");
+    const c10::DeviceGuard guard(w.where);
     if (src.dim() != 1 || src.size(0) > INT32_MAX) refuse("src must be int32 [n]");
     const int64_t pages = src.size(0);
     tensor(a[3], "dst");
@@ -564,7 +600,7 @@ PyObject* keep_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count(n, 8, "keep_kv");
     tensor(a[2], "table");
     const LayerViews w(a[0], a[1], a[6], a[7], a[2], a[3]);
-    const c10::DeviceGuard guard(THPVariable_Unpack(w.k[0]).device());
+    const c10::DeviceGuard guard(w.where);
     const at::Tensor &path = tensor(a[5], "path"), &lens = THPVariable_Unpack(a[3]);
     const int rows = w.c[0].rows;
     tensor(a[4], "starts");

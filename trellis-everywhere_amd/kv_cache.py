@@ -85,7 +85,8 @@ def tree_attention(q, k_pages, v_pages, table, lens, *, starts=None, parents=Non
 
 def copy_pages(k_pages, v_pages, src, dst, *, counts=None, scores=None, pos=None) -> None:
     """Page dst[i] becomes page src[i], its first counts[i] tokens if given (int32 [n] each), in one launch for up to 32
-    layers: k_pages and v_pages (scores, pos) are one layer's tensor, or a list with one for each layer.
+    layers: k_pages and v_pages (scores, pos) are one layer's tensor, a list with one for each layer, or one tensor with the
+    layers as its first dim.
     No page may be in dst twice, or in src and dst; src[i] == dst[i], and ids outside the pool, copy nothing."""
     return _result(_capi.serve().copy_pages(k_pages, v_pages, src, dst, counts, scores, pos))
 
@@ -93,7 +94,7 @@ def copy_pages(k_pages, v_pages, src, dst, *, counts=None, scores=None, pos=None
 def keep_kv(k_pages, v_pages, table, lens, starts, path, *, scores=None, pos=None):
     """After a check of drafted tokens: of each row's n = starts[b+1] - starts[b] newest tokens those on its path stay.
     Token path[b, i] moves to slot lens[b] - n + i, in place, key, value, score and position together, in one launch for
-    up to 32 layers (lists as for copy_pages).
+    up to 32 layers (given as for copy_pages).
 
     path: int32 [rows, width], ascending numbers below n; it ends at the first entry that is not one (-1)
     Returns the new lengths lens - n + the paths' as a new tensor. No page that holds new tokens may be in two rows'
