@@ -339,8 +339,7 @@ def _run_beam(s):
 
 def _run_copy(s):
     if own:
-        planes = {n: None if s[n] is None else list(s[n]) for n in ("scores", "pos")}
-        _te().copy_pages(list(s["k"]), list(s["v"]), s["src"], s["dst"], counts=s["counts"], **planes)
+        _te().copy_pages(s["k"], s["v"], s["src"], s["dst"], counts=s["counts"], scores=s["scores"], pos=s["pos"])
     else:
         src, dst = s["src"].long(), s["dst"].long()
         page = s["case"]["page"]
@@ -354,8 +353,7 @@ def _run_copy(s):
 
 def _run_keep(s):
     if own:
-        planes = {n: None if s[n] is None else list(s[n]) for n in ("scores", "pos")}
-        lens = _te().keep_kv(list(s["k"]), list(s["v"]), s["table"], s["lens"], s["starts"], s["path"], **planes)
+        lens = _te().keep_kv(s["k"], s["v"], s["table"], s["lens"], s["starts"], s["path"], scores=s["scores"], pos=s["pos"])
     else:
         page, table = s["case"]["page"], s["table"].long()
         base = s["lens"].long() - s["starts"].long().diff()
