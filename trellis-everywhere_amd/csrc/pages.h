@@ -24,14 +24,24 @@ __device__ __forceinline__ RowPair load_rows(const Layers& l, int layer, long lo
   return {*reinterpret_cast<const u32x4_t*>(static_cast<const char*>(l.k[layer]) + 2 * at + 16 * sub),
           *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(l.v[layer]) + 2 * at + 16 * sub)};
 }
+// NT: nontemporal stores.
+template <bool NT = false>
 __device__ __forceinline__ void store_rows(const Layers& l, int layer, long long at, int sub, RowPair r) {
-  *reinterpret_cast<u32x4_t*>(static_cast<char*>(l.k[layer]) + 2 * at + 16 * sub) = r.k;
-  *reinterpret_cast<u32x4_t*>(static_cast<char*>(l.v[layer]) + 2 * at + 16 * sub) = r.v;
+  u32x4_t* k = reinterpret_cast<u32x4_t*>(static_cast<char*>(l.k[layer]) + 2 * at + 16 * sub);
+  u32x4_t* v = reinterpret_cast<u32x4_t*>(static_cast<char*>(l.v[layer]) + 2 * at + 16 * sub);
+  if constexpr (NT) {
+    __builtin_nontemporal_store(r.k, k);
+    __builtin_nontemporal_store(r.v, v);
+  } else {
+    *k = r.k;
+    *v = r.v;
+  }
 }
 
 // Page dst[i] takes the first counts[i] tokens of page src[i] (all without counts); a page outside the pool, or onto
 // itself: nothing. A workgroup takes PAGE_AHEAD rows a lane group of one (layer, copy, head): `parts` of them a page.
-// Bound: memory.
+// Bound: memory (12 layers x 40 pages of 64 tokens of 8 heads of 128 with scores and positions, 256 MB moved: 41.8 us, 6.1 TB/s;
+// 54.6 with plain stores, 42.2 with nontemporal loads alone, 47.0 with both).
 struct CopyArgs {
   Cache c;
   Layers l;
@@ -41,6 +51,7 @@ struct CopyArgs {
   int n;
 };
 
+template <bool NT>
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a, int lpr, int parts) {
   const int part = blockIdx.x % parts;
   const unsigned rest = blockIdx.x / parts;
@@ -64,7 +75,7 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a, int lpr, in
 #pragma unroll
   for (int u = 0; u < PAGE_AHEAD; ++u) {
     const int slot = first + u * groups + group;
-    if (own && slot < count) store_rows(a.l, layer, a.c.row_at(dst, head, slot), sub, r[u]);
+    if (own && slot < count) store_rows<NT>(a.l, layer, a.c.row_at(dst, head, slot), sub, r[u]);
   }
   for (int slot = first + threadIdx.x; slot < min(count, first + groups * PAGE_AHEAD); slot += 256) {
     const long long s = a.c.slot_at(src, head, slot), t = a.c.slot_at(dst, head, slot);

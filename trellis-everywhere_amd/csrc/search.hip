@@ -252,11 +252,15 @@ int trellis_kv_copy_pages(const trellis_kv_cache* layers, int n_layers, const in
   const int64_t one = static_cast<int64_t>(n) * layers->heads * parts;
   const int most = n_layers < PAGE_LAYERS ? n_layers : PAGE_LAYERS;
   if (one > INT32_MAX || !grid_fits(one * most, 256)) return TRELLIS_ERR_BATCH;
+  // copies of 16 MB and more: what is written is not read again from the caches soon
+  const bool nt = static_cast<int64_t>(n) * n_layers * layers->heads * layers->page_size * layers->head_dim * 4 >= 16000000;
   hipStream_t st = static_cast<hipStream_t>(stream);
   for (int at = 0; at < n_layers; at += PAGE_LAYERS) {
     const int some = n_layers - at < PAGE_LAYERS ? n_layers - at : PAGE_LAYERS;
     a.l = layers_of(layers + at, some);
-    hipLaunchKernelGGL(copy_pages_kernel, dim3(static_cast<unsigned>(one * some)), dim3(256), 0, st, a, lpr, parts);
+    const dim3 grid(static_cast<unsigned>(one * some));
+    if (nt) hipLaunchKernelGGL(copy_pages_kernel<true>, grid, dim3(256), 0, st, a, lpr, parts);
+    else hipLaunchKernelGGL(copy_pages_kernel<false>, grid, dim3(256), 0, st, a, lpr, parts);
   }
   return launched();
 }
