@@ -4,8 +4,7 @@ and a paged key-value cache with its attention and eviction.
     python examples/decode_block.py                      # a small model, checked against plain torch
     python examples/decode_block.py --blocks 4 --hidden 4096 --ffn 12288 --heads 32 --kv-heads 8 --tokens 64
 
-The weights are random packed words (what an encoder's output looks like); prompts are fed a token at a
-time. The blocks are pre-norm with per-head norms of q and k and rotary positions:
+The weights are random packed words (what an encoder's output looks like). The blocks are pre-norm with per-head norms of q and k and rotary positions:
 
     y = norm(h);  q, k, v = linear(y);  h += o(attention(rot(norm(q)), cache))
     y = norm(h);  gate, up = linear(y); h += down(silu(gate) * up)
@@ -61,17 +60,23 @@ class Decoder:
         self.cache = te.PagedKVCache(blocks, kv_heads, head_dim, rows=rows, max_len=budget + 1 if budget else max_len,
                                      page_size=page_size, device=device, evictable=budget is not None)
 
-    @torch.no_grad()
     def step(self, h):
         """One token's hidden states h [rows, hidden] (f32) through the blocks; the normed output [rows, hidden]."""
-        rows, cache = h.shape[0], self.cache
-        cache.grow(1)
+        return self.forward(h, 1)
+
+    @torch.no_grad()
+    def forward(self, h, counts, depths=None, parents=None):
+        """Hidden states of counts[b] new tokens for each row b (an int: for every row), row by row, h [tokens, hidden]
+        (f32): prompts, or (depths, parents: PagedKVCache.grow and attend_new) drafted tokens in a tree."""
+        cache, n = self.cache, h.shape[0]
+        cache.grow(counts, depths)
+        several = not isinstance(counts, int) or counts > 1 or depths is not None
         first = self.blocks[0]
         y = te.rms_norm(h, first.attn_norm, out_dtype=torch.float16)
         for i, b in enumerate(self.blocks):
-            q, k, v = (t.view(rows, -1, b.head_dim) for t in b.qkv([y, y, y], out_dtype=torch.float16))
+            q, k, v = (t.view(n, -1, b.head_dim) for t in b.qkv([y, y, y], out_dtype=torch.float16))
             q = cache.append(i, q, k, v, q_norm=b.q_norm, k_norm=b.k_norm, cos=self.cos, sin=self.sin)
-            x = cache.attend(i, q).view(rows, -1)
+            x = (cache.attend_new(i, q, parents=parents) if several else cache.attend(i, q)).view(n, -1)
             y, h = te.residual_norm(b.linears["o"](x), h, b.ffn_norm, out_dtype=torch.float16)
             gate, up = b.gate_up([y, y])
             x = b.linears["down"]((torch.nn.functional.silu(gate) * up).half())

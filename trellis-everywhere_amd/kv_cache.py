@@ -1,9 +1,12 @@
 """A paged key-value cache and the attention that decodes from it (trellis_kv_append,
 trellis_paged_attention, trellis_kv_evict): what a decoder block runs between its q/k/v and its o linear
 (the reference's QKNORM, ROPE, cache copy and ATTN dispatches over one contiguous sequence,
-within web/model.js:77-102). For serving: forward only. Arguments are checked in csrc/bind.cpp.
+within web/model.js:77-102); and beyond the reference, several new tokens a row (prompts, drafted tokens in a
+tree: trellis_tree_attention, trellis_kv_keep) and sequences that fork (trellis_kv_copy_pages). For serving:
+forward only. Arguments are checked in csrc/bind.cpp.
 
-append_kv, paged_attention and evict_kv work on tensors that the caller owns; PagedKVCache owns them.
+append_kv, paged_attention, tree_attention, evict_kv, copy_pages and keep_kv work on tensors that the caller owns;
+PagedKVCache owns them.
 
   k_pages, v_pages: [pages, heads, page_size, head_dim] float16 or bfloat16; alike in strides, unit last
   table: int32 [rows, width], row b's token j in slot j % page_size of page table[b, j // page_size]; an
@@ -127,11 +130,13 @@ class PagedKVCache:
     """The key-value cache of a model's layers for up to `rows` sequences of up to `max_len` cached tokens,
     in pages that the rows take from one pool as they grow.
 
-    A step calls grow() once, then append() and attend() for each layer; evict() once after a step keeps
-    the rows within a budget. The page tables, lengths and positions are shared by the layers. Calls are
-    ordered on the current stream; use the cache on one stream at a time. A grow(), evict() or release() that
-    changes a row's pages sends the table anew and waits for the stream (a budget that is a multiple of
-    page_size takes and frees a page each step)."""
+    A step calls grow() once, then append() and attend() for each layer (attend_new() where it gave rows several
+    tokens: prompts, drafts); evict() once after a step keeps the rows within a budget, keep() the drafted tokens
+    that a check has accepted; reorder() lets rows go on from others' sequences, as beams do. The page tables,
+    lengths and positions are shared by the layers, full pages by rows that have forked (but for an evictable
+    cache, whose rows change all of theirs). Calls are ordered on the current stream; use the cache on one stream
+    at a time. A grow(), evict(), keep(), reorder() or release() that changes a row's pages sends the table anew and
+    waits for the stream (a budget that is a multiple of page_size takes and frees a page each step)."""
 
     def __init__(self, layers: int, heads: int, head_dim: int, *, rows: int, max_len: int, pages: int | None = None,
                  page_size: int = 64, dtype: torch.dtype = torch.float16, device="cuda", evictable: bool = False):
@@ -152,7 +157,9 @@ class PagedKVCache:
         self.lengths, self.seen = [0] * rows, [0] * rows     # the host's copies of lens and next_pos
         self._free = list(range(pages - 1, -1, -1))
         self._owned: list[list[int]] = [[] for _ in range(rows)]
+        self._refs = [0] * pages     # rows that have the page
         self._starts = self._positions = None
+        self._drafts: tuple[list[int], list[int]] | None = None     # the last grow()'s counts, and seen before it
         # rows that the last grow() gave tokens, on the device (None: all); lens of these and of the others
         self._fed: torch.Tensor | None = None
         self._lens_of: tuple[torch.Tensor, torch.Tensor] | None = None
@@ -164,13 +171,29 @@ class PagedKVCache:
         width = self.table.shape[1]
         self._upload(self.table, [own + [-1] * (width - len(own)) for own in self._owned])
 
-    def grow(self, counts) -> None:
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._refs[page] = 1
+        return page
+
+    def _drop(self, page: int) -> None:
+        self._refs[page] -= 1
+        if self._refs[page] == 0:
+            self._free.append(page)
+
+    def grow(self, counts, depths=None) -> None:
         """Room for counts[b] new tokens in each row b (an int: in every row); the next append() calls fill it.
+        depths: for drafted tokens in a tree, each token's depth below its row's sequence (0: next after it), row by
+            row; its position is that far on. None: the tokens follow each other.
         Raises ValueError, and changes nothing, where a row would pass max_len or the pool has too few pages."""
         rows = len(self.lengths)
         counts = [counts] * rows if isinstance(counts, int) else list(counts)
         if len(counts) != rows or min(counts) < 0:
             raise ValueError(f"counts must be {rows} numbers >= 0")
+        if depths is not None:
+            depths = list(depths)
+            if len(depths) != sum(counts) or min(depths, default=0) < 0:
+                raise ValueError(f"depths must be {sum(counts)} numbers >= 0")
         lengths = [n + c for n, c in zip(self.lengths, counts)]
         if max(lengths) > self.max_len:
             raise ValueError(f"a row of {max(lengths)} tokens passes max_len={self.max_len}")
@@ -178,15 +201,21 @@ class PagedKVCache:
         if sum(need) > len(self._free):
             raise ValueError(f"{sum(need)} pages needed, {len(self._free)} free")
         for own, k in zip(self._owned, need):
-            own.extend(self._free.pop() for _ in range(k))
+            own.extend(self._take() for _ in range(k))
         if any(need):
             self._upload_table()
         self.lengths = lengths
-        self.seen = [p + c for p, c in zip(self.seen, counts)]
+        before, at = self.seen, 0
+        self._drafts = counts, before
+        steps = []          # positions that each row advances by
+        for c in counts:
+            steps.append(c if depths is None else max(depths[at:at + c], default=-1) + 1)
+            at += c
+        self.seen = [p + c for p, c in zip(before, steps)]
         self._fed, self._lens_of = None, None
         if self.scores[0] is not None and not all(counts):
             self._fed = torch.tensor([c > 0 for c in counts]).to(self.device)
-        if all(c == 1 for c in counts):
+        if depths is None and all(c == 1 for c in counts):
             # a decode step: but for the table, where a row takes a page, nothing comes from the host
             self.lens += 1
             self._starts, self._positions = None, self.next_pos.clone()
@@ -197,7 +226,10 @@ class PagedKVCache:
             starts = [0]
             for c in counts:
                 starts.append(starts[-1] + c)
-            where = [i for p, c in zip(self.seen, counts) for i in range(p - c, p)]
+            if depths is None:
+                where = [p + i for p, c in zip(before, counts) for i in range(c)]
+            else:
+                where = [p + d for p, d in zip([p for p, c in zip(before, counts) for _ in range(c)], depths)]
             self._starts = torch.tensor(starts, dtype=torch.int32).to(self.device)
             self._positions = torch.tensor(where, dtype=torch.int32).to(self.device)
 
@@ -223,6 +255,82 @@ class PagedKVCache:
         fed, waiting = self._lens_of
         return ask(fed, self.scores[layer]).add_(ask(waiting, None))     # each row is empty in one of them
 
+    def attend_new(self, layer: int, q, *, parents=None, scale: float | None = None, out_dtype=None):
+        """tree_attention of the tokens that grow() made room for, row by row: q has a query for each. parents: int32 on
+        the device, the number within its row of the token that each one continues (-1: the row's sequence); None: each
+        continues the one before it. An evictable cache's scores stay as they are."""
+        if self._positions is None:
+            raise ValueError("grow() first")
+        return tree_attention(q, self.k[layer], self.v[layer], self.table, self.lens, starts=self._starts, parents=parents,
+                              scale=scale, max_len=max(self.lengths), out_dtype=out_dtype)
+
+    def keep(self, paths) -> None:
+        """keep_kv in every layer: of the tokens that the last grow() gave row b those numbered paths[b] stay (ascending, a
+        line of the tree from its root), closed up; the pages that the rows no longer fill go back to the pool. The rows'
+        sequences have then grown by their paths. Raises ValueError, and changes nothing, where a path does not fit."""
+        if self._drafts is None:
+            raise ValueError("grow() first")
+        counts, before = self._drafts
+        paths = [list(p) for p in paths]
+        if len(paths) != len(counts) or any(p != sorted(set(p)) or (p and not 0 <= p[0] <= p[-1] < c) for p, c in zip(paths, counts)):
+            raise ValueError("each row's path must be ascending numbers below its count of new tokens")
+        starts = [0]
+        for c in counts:
+            starts.append(starts[-1] + c)
+        starts = self._starts if self._starts is not None else torch.tensor(starts, dtype=torch.int32).to(self.device)
+        width = max(len(p) for p in paths)
+        path = torch.tensor([p + [-1] * (width - len(p)) for p in paths], dtype=torch.int32).view(len(paths), width).to(self.device)
+        self.lens.copy_(keep_kv(self.k, self.v, self.table, self.lens, starts, path, scores=self.scores, pos=self.pos))
+        self.seen = [p + len(k) for p, k in zip(before, paths)]
+        self._upload(self.next_pos, self.seen)
+        self._set_lengths([n - c + len(p) for n, c, p in zip(self.lengths, counts, paths)])
+
+    def reorder(self, parents) -> None:
+        """Row b goes on from what row parents[b] holds (several rows may from one; what no row goes on from is dropped): the
+        rows share the pages that are full and copy the one that they will fill further (an evictable cache's rows copy
+        all). Raises ValueError, and changes nothing, where the pool has too few pages."""
+        rows = len(self.lengths)
+        parents = [int(p) for p in parents]
+        if len(parents) != rows or min(parents) < 0 or max(parents) >= rows:
+            raise ValueError(f"parents must be {rows} numbers in 0 .. {rows - 1}")
+        share = self.scores[0] is None
+        # of the rows that go on from one, the row itself keeps its pages as they are, or else the first
+        heir = {p: p if parents[p] == p else parents.index(p) for p in parents}
+        full = [n // self.page_size if share else 0 for n in self.lengths]
+        want = sum(len(self._owned[p]) - full[p] for b, p in enumerate(parents) if heir[p] != b)
+        gone = [page for p in range(rows) if p not in heir for page in self._owned[p]]
+        back = sum(self._refs[page] == gone.count(page) for page in set(gone))
+        if want > len(self._free) + back:
+            raise ValueError(f"{want} pages needed, {len(self._free) + back} free")
+        old = self._owned
+        for page in gone:
+            self._drop(page)
+        src, dst, counts = [], [], []
+        self._owned = []
+        for b, p in enumerate(parents):
+            own = list(old[p])
+            if heir[p] != b:
+                for i, page in enumerate(own):
+                    if i < full[p]:
+                        self._refs[page] += 1
+                    else:
+                        own[i] = self._take()
+                        src.append(page)
+                        dst.append(own[i])
+                        counts.append(min(self.page_size, self.lengths[p] - i * self.page_size))
+            self._owned.append(own)
+        if src:
+            ints = [torch.tensor(t, dtype=torch.int32).to(self.device) for t in (src, dst, counts)]
+            copy_pages(self.k, self.v, ints[0], ints[1], counts=ints[2], scores=self.scores, pos=self.pos)
+        if parents != list(range(rows)):
+            self._upload_table()
+            if self._fed is not None:
+                self._fed = self._fed[torch.tensor(parents, device=self.device)]
+        self.seen = [self.seen[p] for p in parents]
+        self._upload(self.next_pos, self.seen)
+        self._set_lengths([self.lengths[p] for p in parents])
+        self._upload(self.lens, self.lengths)
+
     def evict(self, keep: int, recent: int) -> None:
         """evict_kv of every layer, in place; the pages that the rows no longer fill go back to the pool."""
         if self.scores[0] is None:
@@ -244,11 +352,11 @@ class PagedKVCache:
         self._upload(self.lens, self.lengths)
 
     def _set_lengths(self, lengths) -> None:
-        self._starts = self._positions = self._lens_of = None
+        self._starts = self._positions = self._lens_of = self._drafts = None
         self.lengths, freed = lengths, False
         for own, n in zip(self._owned, lengths):
             while len(own) > -(-n // self.page_size):
-                self._free.append(own.pop())
+                self._drop(own.pop())
                 freed = True
         if freed:
             self._upload_table()
