@@ -64,13 +64,15 @@ __device__ __forceinline__ void tree_none(const TreeArgs& a, int z, int lane) {
   }
 }
 
-// Blocks of 32 tokens a wave and step, and workgroups that a CU's registers (and LDS) have to hold.
-constexpr int tree_wide(int dp, bool exact) { return dp <= 128 && !exact ? 2 : 1; }
+// Blocks of 32 tokens a wave and step (two slots of their keys and values have to fit LDS), and workgroups that a CU's
+// registers hold.
+constexpr int tree_wide(int dp, bool exact) { return dp > 128 && exact ? 1 : 2; }
+constexpr int tree_residents(int dp, bool exact) { return dp > 128 || exact ? 1 : 2; }
 
 // T: the cache's type. DP: head dims padded to 64, 128 or 256; FULL: d == DP. EXACT: q or out is of another type than the
 // cache's.
 template <class T, int DP, bool FULL, bool EXACT>
-__global__ __launch_bounds__(256, tree_wide(DP, EXACT)) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256, tree_residents(DP, EXACT)) void tree_kernel(TreeArgs a) {
   typedef TreeType<T> AT;
   typedef typename AT::vec8 vec8;
   constexpr bool BF = !std::is_same<T, _Float16>::value;
