@@ -7,7 +7,8 @@
 namespace trellis {
 
 constexpr int TREE_UNIT = 128;                        // tokens that chunks are counted in
-constexpr int TREE_LEAST = 2;                         // units of the shortest chunk
+constexpr int TREE_LEAST = 1;                         // units of the shortest chunk
+constexpr int TREE_WHOLE = 256;                       // tokens up to which a row is not cut
 constexpr int TREE_ROWS = 512;                        // the most rows that are cut into chunks
 
 constexpr int tree_units(int n) { return (n + TREE_UNIT - 1) / TREE_UNIT; }
@@ -51,7 +52,7 @@ constexpr TreeChunks tree_chunks(int rows, int heads, int q_heads, int head_dim,
   // 39.7 / 42.0, 48 new 62.6 / 54.2; 32 rows of 1024, 8 new 32.9 / 37.4).
   const bool twice = !exact && head_dim <= 128 && queries > static_cast<int64_t>(rows) * qr;
   const int64_t want = static_cast<int64_t>(cus) * (twice ? 2 : 1);
-  if (n <= TREE_LEAST * TREE_UNIT || rows > TREE_ROWS || p.items >= 2 * static_cast<int64_t>(cus)) return p;
+  if (n <= TREE_WHOLE || rows > TREE_ROWS || p.items >= 2 * static_cast<int64_t>(cus)) return p;
   p.aim = static_cast<int>(want);
   // (those that the work is cut into, and every block one that is not full)
   const int64_t most = p.blocks * tree_units(n) / TREE_LEAST;
