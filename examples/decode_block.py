@@ -4,7 +4,8 @@ and a paged key-value cache with its attention and eviction.
     python examples/decode_block.py                      # a small model, checked against plain torch
     python examples/decode_block.py --blocks 4 --hidden 4096 --ffn 12288 --heads 32 --kv-heads 8 --tokens 64
 
-The weights are random packed words (what an encoder's output looks like). The blocks are pre-norm with per-head norms of q and k and rotary positions:
+The weights are random packed words (what an encoder's output looks like). The blocks are pre-norm with
+per-head norms of q and k and rotary positions:
 
     y = norm(h);  q, k, v = linear(y);  h += o(attention(rot(norm(q)), cache))
     y = norm(h);  gate, up = linear(y); h += down(silu(gate) * up)

@@ -231,7 +231,6 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
         }
       }
     };
-    add_all(std::false_type{});
     double against = static_cast<double>(shift) / static_cast<double>(LOG2E);
     // (beyond 2^20 half a step of the product is no small power of 2)
     const bool far = fabsf(to) > 1048576.f;
