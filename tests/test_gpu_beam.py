@@ -184,6 +184,26 @@ def test_workspace_of_the_caller(te, gpu_device):
     assert e.value.status == 10
 
 
+def test_writes_count(te, gpu_device):
+    own = {"x": torch.zeros((1, 2, 50), device=gpu_device), "s": torch.zeros((1, 2), device=gpu_device),
+           "e": torch.zeros((1, 2), dtype=torch.bool, device=gpu_device), "ws": torch.zeros(1 << 16, dtype=torch.uint8, device=gpu_device)}
+    before = {n: t._version for n, t in own.items()}
+    te.beam_select(own["x"], own["s"], 3, ended=own["e"], workspace=own["ws"])
+    assert {n for n, t in own.items() if t._version != before[n]} == {"ws"}
+
+
+def test_infinite_and_missing_scores(te, gpu_device):
+    """A score that is not a number is no candidate; a logit of +inf, which is not allowed, ends the call all the same."""
+    x, _ = _random(2, 5, 300, F32, 12)
+    s = torch.tensor([[math.nan, -math.inf, 1e5, -1e5, 0.0], [math.nan] * 5])
+    got = te.beam_select(x.to(gpu_device), s.to(gpu_device), 7)
+    want = ref.beams(x, s.nan_to_num(nan=-math.inf), 7)
+    assert torch.equal(got[1].cpu(), want[1]) and got[0][1].tolist() == [-math.inf] * 7 and got[1][1].tolist() == [0] * 7
+    x[0, 2, 7] = math.inf
+    te.beam_select(x.to(gpu_device), s.to(gpu_device), 7)
+    torch.cuda.synchronize()
+
+
 def test_refusals(te, gpu_device):
     dev = gpu_device
     x, s = torch.zeros((2, 3, 50), device=dev), torch.zeros((2, 3), device=dev)

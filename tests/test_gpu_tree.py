@@ -287,6 +287,83 @@ def test_workspace_of_the_caller(te, gpu_device):
     assert got is out and torch.equal(out, te.tree_attention(q, k, v, table, lens, out_dtype=F32))
 
 
+def test_workspaces_that_do_not_do(te, gpu_device):
+    P = Pages([3000], 1, 16, 64, F16, 3)
+    q = torch.zeros((4, 4, 64), dtype=F16, device=gpu_device)
+    k, v, table, lens, _, _ = P.to(gpu_device)
+    for ws, status in ((torch.empty(64, dtype=torch.uint8, device=gpu_device), 10), (torch.empty((1 << 24) + 8, dtype=torch.uint8, device=gpu_device)[8:], 8)):
+        with pytest.raises(te.TrellisError) as e:
+            te.tree_attention(q, k, v, table, lens, workspace=ws)
+        assert e.value.status == status
+
+
+@pytest.mark.parametrize("group", [129, 300])
+@pytest.mark.parametrize("x,cache,y", TYPES[:3])
+def test_groups_of_more_heads_than_a_block_holds(te, gpu_device, group, x, cache, y):
+    _tree(te, gpu_device, [40, 3, 700], [3, 1, 5], 1, group, 32, 16, x, cache, y, seed=group)
+    _tree(te, gpu_device, [40, 9], [7, 9], 1, group, 64, 16, x, cache, y, seed=group, parents=None)
+
+
+@pytest.mark.parametrize("y", [F16, F32])
+def test_starts_in_no_order_of_long_rows(te, gpu_device, y):
+    """Rows that are cut into chunks: nothing outside out is touched, and the next call is right."""
+    P = Pages([900, 20, 1300], 2, 16, 64, F16, 5, idle=0.0)
+    q = torch.randn((12, 4, 64), generator=P.g).half()
+    k, v, table, lens, _, _ = P.to(gpu_device)
+    for s in ([0, 12, 0, 12], [12, 0, 12, 0], [0, 4, 2, 12], [-5, 4, 8, 12], [0, 4, 8, 99], [2 ** 31 - 1, 0, 0, 0], [5, 5, 5, 5]):
+        wide = torch.full((12 + 128, 4, 64), 7.0, dtype=y, device=gpu_device)
+        te.tree_attention(q.to(gpu_device), k, v, table, lens, starts=torch.tensor(s, dtype=torch.int32, device=gpu_device), out=wide[64:76])
+        torch.cuda.synchronize()
+        assert (wide[:64] == 7).all() and (wide[76:] == 7).all() and wide.isfinite().all(), s
+    assert (wide[64:76] == 0).all()     # no row has a token
+    s = torch.tensor([0, 4, 5, 12], dtype=torch.int32)
+    got = te.tree_attention(q.to(gpu_device), k, v, table, lens, starts=s.to(gpu_device), out_dtype=y)
+    close(got, ref.tree(q, P, s), y, 3e-3)
+
+
+@pytest.mark.parametrize("y", [F16, F32])
+def test_graphs_and_streams(te, gpu_device, y):
+    """Two calls at once on two streams, and replays of a captured call whose rows and chunks change between them, with
+    eager calls in between, give what one eager call gives."""
+    P = Pages([2000, 700, 64], 2, 16, 64, F16, 8, idle=None)
+    k, v, table, lens, _, _ = P.to(gpu_device)
+    ints = lambda t: torch.tensor(t, dtype=torch.int32, device=gpu_device)
+    starts, parents = ints([0, 20, 25, 40]), _parents([20, 5, 15], P.g).to(gpu_device)
+    qs = [torch.randn((40, 8, 64), generator=P.g).half().to(gpu_device) for _ in range(2)]
+    call = lambda q, starts=starts, lens=lens: te.tree_attention(q, k, v, table, lens, starts=starts, parents=parents, out_dtype=y)
+    eager = [call(q) for q in qs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            a = call(qs[0])
+        b = call(qs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(a, eager[0]) and torch.equal(b, eager[1])
+    q = qs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(q)
+    for i, (s, n) in enumerate((([0, 20, 25, 40], [2000, 700, 64]), ([0, 1, 40, 40], [40, 700, 0]), ([0, 0, 0, 0], [9, 9, 9]), ([3, 8, 30, 33], [5, 650, 3]))):
+        q.copy_(qs[i % 2])
+        starts.copy_(ints(s))
+        lens.copy_(ints(n))
+        graph.replay()
+        want = call(qs[i % 2], ints(s), ints(n))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+
+
+def test_writes_count(te, gpu_device):
+    P = Pages([40], 2, 16, 64, F16, 7, idle=None)
+    k, v, table, lens, _, _ = P.to(gpu_device)
+    q, ws = torch.zeros((4, 4, 64), dtype=F16, device=gpu_device), torch.zeros(1 << 20, dtype=torch.uint8, device=gpu_device)
+    own = {"q": q, "k": k, "v": v, "table": table, "lens": lens, "out": torch.zeros_like(q), "ws": ws}
+    before = {n: t._version for n, t in own.items()}
+    te.tree_attention(q, k, v, table, lens, out=own["out"], workspace=ws)
+    assert {n for n, t in own.items() if t._version != before[n]} == {"out", "ws"}
+
+
 def test_refusals(te, gpu_device):
     dev = gpu_device
     P = Pages([20, 3], 2, 16, 64, F16, 0, idle=None)
