@@ -249,26 +249,21 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
     for (int r = 0; r < R; ++r) with |= (__any(tops[r] >= bound) ? 1u : 0u) << r;
     int count = 0;
     while (with || count) {
-      if (with) {
-        const int r = __builtin_ctz(with);
-        with &= with - 1;
-        BeamPiece<T> now = piece[0];
+      // (every round in its own place: to bring the round's piece into one costs more than all else here)
 #pragma unroll
-        for (int i = 1; i < R; ++i)
-          if (r == i) now = piece[i];
+      for (int r = 0; r < R; ++r) {
+        if (!(with >> r & 1) || count >= 64) continue;
+        with &= ~(1u << r);
+        BeamPiece<T> now = piece[r];
         now.keep();
-        const uint32_t i0 = 8u * (p0 + 64 * r + lane);
-        unsigned have = 0;         // the lane's logits that reach the bound: mostly one of a few lanes
+        uint32_t own = lane;
+        asm volatile("" : "+v"(own));   // (or every place in the run is formed beforehand and kept)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) have |= (now.at(e) >= bound ? 1u : 0u) << e;
-        while (__any(have != 0)) {
-          const int e = have ? __builtin_ctz(have) : 0;
-          float v = now.at(0);
-#pragma unroll
-          for (int i = 1; i < 8; ++i) v = e == i ? now.at(i) : v;
-          const beam_t c = static_cast<beam_t>(beam_order(v)) << 32 | ~(i0 + e);
-          const bool is = have && c > least;
-          have &= have - 1;
+        for (int e = 0; e < 8; ++e) {
+          const float v = now.at(e);
+          if (!__any(v >= bound)) continue;       // mostly one logit of one lane does
+          const beam_t c = static_cast<beam_t>(beam_order(v)) << 32 | ~(8u * (p0 + 64 * r + own) + e);
+          const bool is = v >= bound && c > least;
           const unsigned long long who = __ballot(is);
           if (is) few[count + __popcll(who & ((1ull << lane) - 1))] = c;
           count += __popcll(who);
