@@ -304,7 +304,8 @@ int trellis_kv_evict(const trellis_kv_cache *cache, int keep, int recent, const 
  * counterpart: it decodes one sequence a token at a time, web/model.js:77-102). */
 
 /* Attention of several new tokens per row. Row b's n = starts[b+1] - starts[b] tokens (starts:
- * [rows + 1]; NULL: tokens / rows each) are the newest of its lens[b], in its last n slots. The i-th
+ * [rows + 1], none below the one before it, or the call's results mean nothing, though nothing outside
+ * out is touched; NULL: tokens / rows each) are the newest of its lens[b], in its last n slots. The i-th
  * sees the slots below lens[b] - n, itself and its ancestors:
  *   out = sum_j p_j v_j, p = softmax over the tokens j it sees of scale * q . k_j
  *   parents: [tokens], the number within the row of the token that each one continues; one that is

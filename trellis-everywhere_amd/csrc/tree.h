@@ -18,8 +18,17 @@
 // Tiles go downwards, so that a lane walks its query's ancestors once, from itself to the first, a word of 32 tokens at a
 // time; only tiles with a new token, a missing page or the row's end are masked.
 // The chunks' results (maximum, sum, unnormalised out) meet in tree_join_kernel, in a fixed order.
-// Precision: the sums are fp32. The weights enter their product as in attend.h, but once rounded to the cache's type (half
-// a step of it, as out's own rounding) where the products bound the call: blocks of 128 queries of 16-bit types.
+// Precision: the sums are fp32. Where q, cache and out are of one 16-bit type (not EXACT) the weights are rounded once to
+// it, half a step, as out is itself: the error against float64 is 1.2 times that of fp32 products, and the terms that
+// attend.h takes would be two or three times the second product's instructions. Other types take those terms, of q too.
+// Bound: new tokens of few queries a key (32 rows of up to 8192 tokens, up to 26 new each, 32 heads over 8 of 128) by
+// memory: 107-112 us, 4.9 TB/s and 13 MiB of partial sums. Many by the loop's own latencies: 1024 tokens behind 8192
+// 160-177 us, 870 TFLOP/s, the matrix cores busy 48 % of the time and the vector units 44 %; LDS has no conflicts. The waves
+// of a SIMD, two, are all that fills one's waits: taken out one by one (of 185 us) the exponentials are worth 17, the second
+// product 38, the loads into LDS 36, the maximum 4. Small calls by the chain plan, length, page, keys, weights, values: 7 tokens
+// behind 149 9.8 us.
+// 32 queries a wave: of 16 (16x16x32) each key read from LDS would serve half as many, and LDS would bound the loop. 64
+// tokens a step: with 32 and three workgroups a CU 1024 tokens behind 8192 took 192-201 us instead of 177.
 #pragma once
 
 #include "tree_rows.h"
@@ -135,7 +144,8 @@ __global__ __launch_bounds__(256, tree_residents(DP, EXACT)) void tree_kernel(Tr
   const int below = a.parents ? row.base : row.base + token + 1;   // slots that the lane's query sees all of
   int walk = a.parents && fine ? token : -1;              // the ancestor that comes next
 
-  // ---- keys and values into LDS, blocks going downwards, the next one's while one is used. A wave loads OWN rows of each, in 16-row groups that lie in one page each.
+  // ---- keys and values into LDS, blocks going downwards, the next one's while one is used. A wave loads OWN rows of each, in
+  // 16-row groups that lie in one page each.
   const int sstr = static_cast<int>(a.c.slot_stride) * 2;   // bytes
   const unsigned lds = lds_addr(s_kv);
   const auto piece_k = [](int r) { return CH == 8 ? (r >> 1) & 7 : r & 15; };
@@ -359,8 +369,8 @@ __global__ __launch_bounds__(256, tree_residents(DP, EXACT)) void tree_kernel(Tr
         if (active) {
           Logits s = logits(place);
           settle(s, i, place);
-          // (the waves of a SIMD drift apart then, so that one's exponentials meet another's products: a prompt's part of
-          // 2048 tokens 182 -> 166 us, 50 prompts of 6000 117 -> 109; around the logits too: 175 and 110)
+          // (the waves of a SIMD drift apart then, so that one's exponentials meet another's products: a call of 1024 tokens
+          // behind 8192 172.7 -> 163.1 us, of five prompts of 6007 tokens in all 105.9 -> 102.1; less with the logits too)
           __builtin_amdgcn_s_setprio(1);
           accumulate(s, place);
           __builtin_amdgcn_s_setprio(0);

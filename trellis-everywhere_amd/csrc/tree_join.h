@@ -7,7 +7,8 @@ namespace trellis {
 
 // out = sum_i f_i part_i / sum_i f_i sum_i over a block's chunks i, f_i = 2^(m_i - max). A workgroup's threads are (share of
 // the chunks, query, 4 dims): `subs` workgroups a block. The maximum runs along with the sums, so that no load waits for
-// another one.
+// another one. Bound: the partial sums' bytes (one row of 32717 tokens, 63 new: 33.5 MB in 8.8 us), and a launch behind the
+// chunks' (1.5 to 2 us).
 constexpr int tree_join_rows(int d, int shares) { return 256 / (d / 4) / shares; }
 
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int qr, int subs, int shares) {

@@ -74,7 +74,7 @@ def tree_attention(q, k_pages, v_pages, table, lens, *, starts=None, parents=Non
     sees the tokens before them, itself and its ancestors: softmax(scale * q.k) v over these, scale d**-0.5 if None.
 
     q: [tokens, q_heads, d], any token and head strides; query head i over key-value head i // (q_heads // heads)
-    starts: int32 [rows + 1], row by row as for append_kv; None: the same number of tokens for each row
+    starts: int32 [rows + 1], ascending, row by row as for append_kv; None: the same number of tokens for each row
     parents: int32 [tokens], the number within its row of the token that each one continues; one that is not below the
         token's own (-1) is none: it continues the cached tokens. None: each continues the one before it, so that it
         sees them all (a prompt, or part of one).
