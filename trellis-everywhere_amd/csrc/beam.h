@@ -6,15 +6,15 @@
 // beams may be nearer to each other than a rounding to 32 bits.
 //
 // beam_part_kernel: a wave takes a run of a beam's logits, R x 512 at a time, read once and held in registers: their
-// maximum, the sum of their exponentials, and their k best. Of the maxima of the 256 lanes of four waves side by side, sorted
-// across each wave and merged, the k-th is a bound that k of their logits reach: the few that do (k and a handful) are
+// maximum, the sum of their exponentials, and their k best. Of the maxima of the 256 lanes of four waves side by side (or of
+// every four of them), sorted, the k-th is a bound that k of their logits reach: the few that do (k and a handful) are
 // gathered through LDS and sorted by (logit, token) into each wave's list of 64.
 // beam_join_kernel, a workgroup a batch element: per beam the runs' sums and lists, then the beams' lists.
-// Bound: the vector units, busy 76 % of the time: a logit of 16 bits is some 10 instructions (unpacked twice, maximum, fma,
-// exponential at a quarter rate, sum, compare), a wave's sorting and gathering as much as half of them again. 64 x 8 beams
-// of 151936 bf16 logits, a fifth of the beams ended: part 41.7 us (3.0 TB/s), join 7.0; 16 x 4 of f16: 12.6 + 4.5; one beam
-// of 49152 fp32 logits: 4.5 + 3.7, two chains of loads and cross-lane steps. With a bound of each wave's own logits the
-// first call took 69 us instead of 57; with the candidates' pieces brought into one loop body 54 instead of 47.
+// Bound: the vector units, busy 71 % of the time: 13 instructions a logit of 16 bits, some 6 of them its own (unpacked
+// twice, maximum, fma, exponential at a quarter rate, sum), the rest a wave's bounds, loads, sorting and gathering. 64 x 8
+// beams of 151936 bf16 logits, a fifth of the beams ended: part 39.1 us (3.2 TB/s), join 7.0; 16 x 4 of f16: 12.1 + 4.4;
+// one beam of 49152 fp32 logits: 4.5 + 3.8, two chains of loads and cross-lane steps. With a bound of each wave's own
+// logits the first call took 69 us instead of 57; with the candidates' pieces brought into one loop body 54 instead of 47.
 #pragma once
 
 #include "serve.h"
@@ -23,6 +23,11 @@ namespace trellis {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int BEAM_MOST = 64;   // beams, candidates kept of each, runs of a beam (TRELLIS_BEAM_MAX)
+
+// Up to this k the bound is the k-th of 64 maxima of four lanes each: one sort instead of a sort and three merges (64 x 8
+// beams, k = 16: 41.7 -> 39.1 us, the short sort of a list's first 16 included). Beyond, of the 256 lanes' own: the 64th of 64
+// would let some 300 of a run's logits pass (a call with k = 32 / 33: 53.2 / 53.9 us).
+constexpr int BEAM_QUADS = 32;
 
 struct BeamArgs {
   const void* x;
@@ -80,6 +85,15 @@ __device__ __forceinline__ V wave_sort(V v, bool falling, int lane) {
   v = sort_merge<8>(v, (lane & 16) == 0, lane);
   v = sort_merge<16>(v, (lane & 32) == 0, lane);
   return sort_merge<32>(v, falling, lane);
+}
+
+// The same of each 16 lanes.
+template <class V>
+__device__ __forceinline__ V row_sort(V v, bool falling, int lane) {
+  v = sort_merge<1>(v, (lane & 2) == 0, lane);
+  v = sort_merge<2>(v, (lane & 4) == 0, lane);
+  v = sort_merge<4>(v, (lane & 8) == 0, lane);
+  return sort_merge<8>(v, falling, lane);
 }
 
 // The same for (value, where it is from): of equal values the lower place counts as larger.
@@ -200,16 +214,29 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
       for (int e = 1; e < 8; ++e) tops[r] = fmaxf(tops[r], piece[r].at(e));
       top = fmaxf(top, tops[r]);
     }
+    top = top == top ? top : none;
     const float most = wave_max(top, lane);
     // what k of the workgroup's logits reach
-    float bound = a.k > 1 ? wave_sort(top == top ? top : none, true, lane) : most;
+    float bound = most;
+    const bool quads_do = a.k > 1 && a.k <= BEAM_QUADS;
+    if (quads_do) {
+      bound = fmaxf(top, lane_xor<1>(top, lane));
+      bound = fmaxf(bound, lane_xor<2>(bound, lane));
+    } else if (a.k > 1) {
+      bound = wave_sort(top, true, lane);
+    }
     __syncthreads();
-    s_top[wave][lane] = bound;
+    if (!quads_do) s_top[wave][lane] = bound;
+    else if ((lane & 3) == 0) s_top[wave][lane >> 2] = bound;
     __syncthreads();
+    if (quads_do) {
+      bound = wave_sort(s_top[lane >> 4][lane & 15], true, lane);
+    } else {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      if (a.k > 1) bound = sort_merge<32>(fmaxf(bound, s_top[wave ^ w][63 - lane]), true, lane);
-      else bound = fmaxf(bound, s_top[wave ^ w][lane]);
+      for (int w = 1; w < 4; ++w) {
+        if (a.k > 1) bound = sort_merge<32>(fmaxf(bound, s_top[wave ^ w][63 - lane]), true, lane);
+        else bound = fmaxf(bound, s_top[wave ^ w][lane]);
+      }
     }
     bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bound), a.k > 1 ? a.k - 1 : 0));
     bound = fmaxf(bound, least ? beam_logit(least) : -__FLT_MAX__);
@@ -281,7 +308,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
         __builtin_amdgcn_wave_barrier();
         const beam_t c = lane < some ? few[count + lane] : 0;
         if (a.k == 1) best = wave_top(c > best ? c : best, lane);
-        else best = begun ? beam_insert(best, c, lane) : wave_sort(c, true, lane);
+        else best = begun ? beam_insert(best, c, lane) : some <= 16 ? row_sort(c, true, lane) : wave_sort(c, true, lane);
         begun = true;
         least = readlane64(best, a.k - 1);
         __builtin_amdgcn_wave_barrier();
