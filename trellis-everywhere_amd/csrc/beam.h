@@ -365,9 +365,10 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
       const beam_t first = entry(0), second = entry(per);
       const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0, base = is ? a.sums[2 * (row * a.runs + lane) + 1] : ATT_LOW;
       const float most = wave_max(static_cast<float>(base), lane);
-      // (one lane's, for all: each one's first addition takes its own product unrounded)
-      const double each = static_cast<double>(most) + log(wave_sum64(sum * exp(base - static_cast<double>(most)), lane));
-      const double lse = __builtin_bit_cast(double, readlane64(__builtin_bit_cast(beam_t, each), 0));
+      // lse = most + rest, never added: from 1e16 on the logarithm would be lost beside the maximum. (One lane's, for all: each
+      // one's first addition takes its own product unrounded.)
+      const double each = log(wave_sum64(sum * exp(base - static_cast<double>(most)), lane));
+      const double rest = __builtin_bit_cast(double, readlane64(__builtin_bit_cast(beam_t, each), 0));
       // they are in order: no further ones when none of these can pass the k-th
       beam_t best = a.k == 1 ? wave_top(first, lane) : wave_sort(first, true, lane);
       for (int i = per; i < a.k; i += per) {
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
         best = beam_insert(best, c, lane);
       }
       token = static_cast<int>(~static_cast<uint32_t>(best));
-      if (best) value = score + (static_cast<double>(beam_logit(best)) - lse);
+      if (best) value = score + (static_cast<double>(beam_logit(best)) - static_cast<double>(most) - rest);
     }
     if (lane < a.k) {
       const bool is = value > -__builtin_inf();
