@@ -61,3 +61,28 @@ def test_equal_logits_of_any_size(te, gpu_device, dtype, sizes, vocab, k):
     # beams of different sizes
     x = torch.stack([torch.full((vocab,), float(s)) for s in (sizes[-1], -sizes[-1], 0.0, sizes[0])])[None]
     _select(te, gpu_device, x.to(dtype), torch.tensor([[-4.0, -1.0, -3.5, -0.75]]), k)
+
+
+@pytest.mark.parametrize("k", [1, 5, 64])
+@pytest.mark.parametrize("vocab", [1, 50, 3001, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_beams_of_the_lowest_value(te, gpu_device, dtype, vocab, k):
+    """A mask of the type's lowest value: on a whole beam beside an ordinary one, ahead of it and behind it; on all beams; mixed
+    with -inf; in all of a row but one token, far from it."""
+    low = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(vocab + k)
+    scores = torch.tensor([[-20.0, -0.25, -30.0], [-1.0, -2.0, -25.0]])
+    x = torch.randn((2, 3, vocab), generator=g) * 3
+    x = x.to(dtype)
+    x[0, 1] = low
+    x[1, 2] = low
+    _select(te, gpu_device, x, scores, k)
+    _select(te, gpu_device, torch.full_like(x, low), scores, k)
+    _select(te, gpu_device, torch.full_like(x, low), torch.zeros((2, 3)), k)
+    x = torch.full_like(x, low)
+    x[0, :, ::2] = -INF
+    x[1, 0], x[1, 1, vocab // 2:], x[1, 2, : vocab // 2] = -INF, -INF, -INF
+    _select(te, gpu_device, x, scores, k)
+    x = torch.full_like(x, low)
+    x[0, 0, vocab - 1], x[0, 1, vocab // 2], x[1, 1, 0], x[1, 2, -1] = 0.0, low / 2, torch.finfo(dtype).max, -1.5
+    _select(te, gpu_device, x, scores, k)

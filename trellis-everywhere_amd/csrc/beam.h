@@ -23,6 +23,7 @@ namespace trellis {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int BEAM_MOST = 64;   // beams, candidates kept of each, runs of a beam (TRELLIS_BEAM_MAX)
+constexpr float BEAM_LOW = -__FLT_MAX__;   // no finite logit lies below it: what the sums are taken against begins here
 
 // Up to this k the bound is the k-th of 64 maxima of four lanes each: one sort instead of a sort and three merges (64 x 8
 // beams, k = 16: 41.7 -> 39.1 us, the short sort of a list's first 16 included). Beyond, of the 256 lanes' own: the 64th of 64
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   const float none = -__builtin_inff();
 
   beam_t best = 0, least = 0;    // the list, and its k-th
-  float m = ATT_LOW;
-  double total = 0.0, base = ATT_LOW;    // the sum against exp(base)
+  float m = BEAM_LOW;
+  double total = 0.0, base = BEAM_LOW;   // the sum against exp(base)
   bool begun = false;
   for (int p0 = first; p0 < first + a.per; p0 += 64 * R) {
     BeamPiece<T> piece[R];
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
       }
     }
     bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bound), a.k > 1 ? a.k - 1 : 0));
-    bound = fmaxf(bound, least ? beam_logit(least) : -__FLT_MAX__);
+    bound = fmaxf(bound, least ? beam_logit(least) : BEAM_LOW);
     if (most == none) continue;
     const float to = fmaxf(m, most);
     // The sum, of 2^(x log2(e) - top log2(e)) with the second product rounded once and kept as it is (its error is no term's
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamArgs a) {
       const beam_t* list = a.best + (row * lists + min(of, lists - 1)) * a.k;
       const auto entry = [&](int i) { return of < lists && i + nth < a.k ? list[i + nth] : 0; };
       const beam_t first = entry(0), second = entry(per);
-      const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0, base = is ? a.sums[2 * (row * a.runs + lane) + 1] : ATT_LOW;
+      const double sum = is ? a.sums[2 * (row * a.runs + lane)] : 0.0, base = is ? a.sums[2 * (row * a.runs + lane) + 1] : BEAM_LOW;
       const float most = wave_max(static_cast<float>(base), lane);
       // lse = most + rest, never added: from 1e16 on the logarithm would be lost beside the maximum. (One lane's, for all: each
       // one's first addition takes its own product unrounded.)
