@@ -261,6 +261,9 @@ class PagedKVCache:
         continues the one before it. An evictable cache's scores stay as they are."""
         if self._positions is None:
             raise ValueError("grow() first")
+        new = self._positions.shape[0]
+        if q.dim() != 3 or q.shape[0] != new:
+            raise ValueError(f"q must be [{new}, q_heads, head_dim], a query for each token that grow() made room for")
         return tree_attention(q, self.k[layer], self.v[layer], self.table, self.lens, starts=self._starts, parents=parents,
                               scale=scale, max_len=max(self.lengths), out_dtype=out_dtype)
 
