@@ -17,6 +17,8 @@ PagedKVCache owns them.
 """
 from __future__ import annotations
 
+from collections import Counter
+
 import torch
 
 from . import _capi
@@ -298,11 +300,14 @@ class PagedKVCache:
             raise ValueError(f"parents must be {rows} numbers in 0 .. {rows - 1}")
         share = self.scores[0] is None
         # of the rows that go on from one, the row itself keeps its pages as they are, or else the first
-        heir = {p: p if parents[p] == p else parents.index(p) for p in parents}
+        heir: dict[int, int] = {}
+        for b, p in enumerate(parents):
+            if p == b or p not in heir:
+                heir[p] = b
         full = [n // self.page_size if share else 0 for n in self.lengths]
         want = sum(len(self._owned[p]) - full[p] for b, p in enumerate(parents) if heir[p] != b)
         gone = [page for p in range(rows) if p not in heir for page in self._owned[p]]
-        back = sum(self._refs[page] == gone.count(page) for page in set(gone))
+        back = sum(self._refs[page] == n for page, n in Counter(gone).items())
         if want > len(self._free) + back:
             raise ValueError(f"{want} pages needed, {len(self._free) + back} free")
         old = self._owned
