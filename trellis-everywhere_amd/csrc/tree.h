@@ -96,8 +96,9 @@ __global__ __launch_bounds__(256, tree_residents(DP, EXACT)) void tree_kernel(Tr
   constexpr int CH = DP / 8, ROW = 2 * DP;                // 16-byte pieces and bytes of a row
   constexpr int SLOT = BT * ROW;                          // bytes of a step's keys, and of its values: two slots of each
   constexpr int PER = 64 / CH;                            // rows of one load of a wave
-  constexpr int OWN = BT / 4, GROUPS = OWN > 16 ? OWN / 16 : 1;   // rows that a wave loads a step, and their 16-row groups
+  constexpr int OWN = BT / 4, GROUPS = OWN / 16;          // rows that a wave loads a step, and their 16-row groups
   constexpr int OP = DP + 4;                              // floats of a row where waves meet
+  static_assert(OWN % 16 == 0, "a wave loads whole groups: a group's flag has one writer");
   static_assert(WR == 4 || (WT - 1) * WR * 32 * (OP + 2) * 4 <= 4 * SLOT, "the waves' sums fit the slots' memory");
   __shared__ __align__(1024) char s_kv[4 * SLOT];
   __shared__ __align__(8) uint8_t s_ok[2][8];
@@ -150,12 +151,12 @@ __global__ __launch_bounds__(256, tree_residents(DP, EXACT)) void tree_kernel(Tr
   const unsigned lds = lds_addr(s_kv);
   const auto piece_k = [](int r) { return CH == 8 ? (r >> 1) & 7 : r & 15; };
   const auto piece_v = [](int r) { return CH == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
-  constexpr int TIMES = (OWN < 16 ? OWN : 16) / PER;         // loads of a group
-  const int half = OWN < 16 ? wave * OWN & 15 : 0, group0 = wave * OWN & ~15;
+  constexpr int TIMES = 16 / PER;                            // loads of a group
+  const int group0 = wave * OWN;
   unsigned koff[TIMES], voff[TIMES];                         // the lane's places within a group
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    const int r = half + t * PER + lane / CH, pk = lane % CH ^ piece_k(r), pv = lane % CH ^ piece_v(r);
+    const int r = t * PER + lane / CH, pk = lane % CH ^ piece_k(r), pv = lane % CH ^ piece_v(r);
     koff[t] = FULL || 8 * pk < d ? r * sstr + 16 * pk : RSRC_PAST;
     voff[t] = FULL || 8 * pv < d ? r * sstr + 16 * pv : RSRC_PAST;
   }
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(256, tree_residents(DP, EXACT)) void tree_kernel(Tr
       const int bytes = uniform(ok ? min(16, row.len - j) * sstr : 0);
       const rsrc_t k = make_rsrc(reinterpret_cast<const void*>(flat(k_base + at)), bytes);
       const rsrc_t v = make_rsrc(reinterpret_cast<const void*>(flat(v_base + at)), bytes);
-      const unsigned to = lds + place * SLOT + (group0 + 16 * g + half) * ROW;
+      const unsigned to = lds + place * SLOT + (group0 + 16 * g) * ROW;
 #pragma unroll
       for (int t = 0; t < TIMES; ++t) load_lds16<false>(k, uniform(to + t * 1024), koff[t]);
 #pragma unroll
