@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int qr, int 
   const int tid = threadIdx.x, d = a.c.d, quads = d / 4;
   const unsigned unit = uniform(blockIdx.x / subs);
   const int sub = blockIdx.x - unit * subs, pos = uniform(unit / a.c.heads), head = unit - pos * a.c.heads;
-  const int all = load_const(&a.done->live);
+  const int all = a.done->live;          // (written by the chunks' kernel: no load_const)
   const TreeBlock block = a.done[1 + pos];
   if (pos >= all || block.live < 2) return;
   const int rows = tree_join_rows(d, shares), slot = tid / quads, quad = tid - slot * quads, share = slot / rows;
