@@ -331,8 +331,10 @@ int trellis_tree_attention(const trellis_kv_cache *cache, const void *q, int64_t
  *   logits: [batch][beams][vocab] of `dtype`, batch and beam strides in elements, below +inf
  *   scores: f32 [batch][beams]; ended: [batch][beams], 0 or not, or NULL
  *   new_scores f32, new_beams, new_tokens int32: [batch][k]
- * Beams are compared in 64 bits; new_scores are rounded once. The workspace
- * (trellis_beam_workspace_bytes, 256-byte aligned) needs no initialisation. */
+ * Candidates are formed in 64 bits on sums of fp32 exponentials: within 5e-6 (two beams' candidates
+ * nearer than twice that may change places; a beam's own keep the order of their logits), then rounded
+ * once to new_scores (below fp32's lowest value to -inf). The workspace (trellis_beam_workspace_bytes,
+ * 256-byte aligned) needs no initialisation. */
 #define TRELLIS_BEAM_MAX 64
 int trellis_beam_workspace_bytes(int batch, int beams, int vocab, int k, size_t *bytes);
 int trellis_beam_select(const void *logits, int64_t batch_stride, int64_t beam_stride, int dtype,
@@ -342,7 +344,8 @@ int trellis_beam_select(const void *logits, int64_t batch_stride, int64_t beam_s
 
 /* Pages copied in all layers: the first counts[i] tokens (counts NULL: all) of page dst[i] become those
  * of page src[i], keys, values and (where a layer has them) scores and positions.
- *   layers: n_layers caches, alike but for their pointers; table, lens and max_len are not looked at
+ *   layers: n_layers caches, alike but for their pointers; table and lens are not read (NULL where rows
+ *   is 0), but rows, width and max_len have to be those of a cache all the same (0, 1 and 0 will do)
  *   src, dst, counts: int32 [n]; no page may be in dst twice, or in dst and src (but src[i] == dst[i],
  *   and ids outside the pool, copy nothing) */
 int trellis_kv_copy_pages(const trellis_kv_cache *layers, int n_layers, const int32_t *src,

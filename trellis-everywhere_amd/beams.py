@@ -21,8 +21,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, *, ended: to
 
     logits: [batch, beams, vocab] float32, float16 or bfloat16, any batch and beam strides, below +inf
     scores: float32 [batch, beams]; ended: bool [batch, beams]; beams and k up to 64
-    Returns (scores float32, beams int32, tokens int32), each [batch, k]. Beams are compared in 64 bits, the scores
-    rounded once. k = 1 of one beam is the likeliest token and its log-probability.
+    Returns (scores float32, beams int32, tokens int32), each [batch, k]. The scores are formed in 64 bits on fp32
+    exponentials' sums (within 5e-6, mostly some 1e-7: two beams' candidates nearer than twice that may change places; a
+    beam's own keep the order of their logits) and rounded once (below float32's lowest value to -inf). k = 1 of one beam is
+    the likeliest token and its log-probability.
     workspace: scratch for a caller that keeps its own, as for paged_attention."""
     r = _capi.serve().beam_select(logits, scores, k, ended, end_token, workspace)
     if r.__class__ is int:

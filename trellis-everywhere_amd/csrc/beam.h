@@ -2,18 +2,22 @@
 //   c(j, v) = score_j + x_jv - lse_j,  lse_j = log sum_v exp(x_jv)
 // of beam j's logits x_j (an ended beam offers (j, end token) alone, at score_j), the k largest, equal ones by the
 // lower beam, then the lower token. A candidate that is -inf or not a number is none.
-// Within a beam the order is that of its logits, so the sums meet only where beams do, in 64 bits there: candidates of two
-// beams may be nearer to each other than a rounding to 32 bits.
+// Within a beam the order is that of its logits, exactly. Beams meet in 64 bits, so that a score's size costs nothing, but on
+// sums of fp32 exponentials, up to 64 of them added in fp32: log sum exp is off by less than 5e-6 (some 1e-7 for a model's
+// logits), and candidates of two beams within twice that of each other may change places. Equal rows have equal sums.
 //
 // beam_part_kernel: a wave takes a run of a beam's logits, R x 512 at a time, read once and held in registers: their
 // maximum, the sum of their exponentials, and their k best. Of the maxima of the 256 lanes of four waves side by side (or of
 // every four of them), sorted, the k-th is a bound that k of their logits reach: the few that do (k and a handful) are
 // gathered through LDS and sorted by (logit, token) into each wave's list of 64.
 // beam_join_kernel, a workgroup a batch element: per beam the runs' sums and lists, then the beams' lists.
-// Bound: the vector units, busy 71 % of the time: 13 instructions a logit of 16 bits, some 6 of them its own (unpacked
-// twice, maximum, fma, exponential at a quarter rate, sum), the rest a wave's bounds, loads, sorting and gathering. 64 x 8
-// beams of 151936 bf16 logits, a fifth of the beams ended: part 39.1 us (3.2 TB/s), join 7.0; 16 x 4 of f16: 12.1 + 4.4;
-// one beam of 49152 fp32 logits: 4.5 + 3.8, two chains of loads and cross-lane steps. With a bound of each wave's own
+// Bound: of large calls the vector units, busy 71 % of the time: 13 instructions a logit of 16 bits, some 6 of them its own
+// (unpacked twice, maximum, fma, exponential at a quarter rate, sum), the rest a wave's bounds, loads, sorting and gathering.
+// 64 x 8 beams of 151936 bf16 logits, a fifth of the beams ended: part 39.1 us (3.2 TB/s), join 7.0. Smaller ones by the chain
+// load, maximum, sort, sum, gather, sort, which a wave runs once with nothing of another run under way: 16 x 4 of f16 12.1 +
+// 4.4 (vector units busy 41 %), one beam of 49152 fp32 logits 4.5 + 3.8. Many beams or a large k by the join, whose last merge
+// is one wave that sorts 64 / beams entries of a beam at a time: 4 x 16 beams with k = 32 / 64 28 / 40 us the call, 64 beams of
+// 49152 with k = 64 59. With a bound of each wave's own
 // logits the first call took 69 us instead of 57; with the candidates' pieces brought into one loop body 54 instead of 47.
 #pragma once
 

@@ -52,6 +52,9 @@ constexpr TreeChunks tree_chunks(int rows, int heads, int q_heads, int head_dim,
   // 39.7 / 42.0, 48 new 62.6 / 54.2; 32 rows of 1024, 8 new 32.9 / 37.4).
   const bool twice = !exact && head_dim <= 128 && queries > static_cast<int64_t>(rows) * qr;
   const int64_t want = static_cast<int64_t>(cus) * (twice ? 2 : 1);
+  // Two blocks a CU and more stay whole, whatever their lengths (whole / cut: 64 rows of 8 heads, 26 new, uneven up to 8192
+  // 221 / 221 us, 96 345 / 359; 64 rows of 4096, 8 new, 186 / 194, of 1024 54.9 / 62.1; 200 uneven up to 2048 180 / 194; a
+  // prompt's parts, 16 of 8192 tokens in all, 116 / 129): workgroups that wait leave memory to the others.
   if (n <= TREE_WHOLE || rows > TREE_ROWS || p.items >= 2 * static_cast<int64_t>(cus)) return p;
   p.aim = static_cast<int>(want);
   // (those that the work is cut into, and every block one that is not full)

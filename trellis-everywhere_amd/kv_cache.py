@@ -133,12 +133,14 @@ class PagedKVCache:
     in pages that the rows take from one pool as they grow.
 
     A step calls grow() once, then append() and attend() for each layer (attend_new() where it gave rows several
-    tokens: prompts, drafts); evict() once after a step keeps the rows within a budget, keep() the drafted tokens
-    that a check has accepted; reorder() lets rows go on from others' sequences, as beams do. The page tables,
-    lengths and positions are shared by the layers, full pages by rows that have forked (but for an evictable
-    cache, whose rows change all of theirs). Calls are ordered on the current stream; use the cache on one stream
-    at a time. A grow(), evict(), keep(), reorder() or release() that changes a row's pages sends the table anew and
-    waits for the stream (a budget that is a multiple of page_size takes and frees a page each step)."""
+    tokens: prompts, drafts); evict() once after a step keeps the rows within a budget, by the weights that attend()
+    has added up (attend_new() adds none: of a prompt that came in one pass, all of score 0 until later tokens' attend()
+    weighs it, evict() keeps the last positions and the lowest slots; one fed a token at a time through attend() has its
+    scores); keep() the drafted tokens that a check has accepted; reorder() lets rows go on from others' sequences, as
+    beams do. The page tables, lengths and positions are shared by the layers, full pages by rows that have forked (but
+    for an evictable cache, whose rows change all of theirs). Calls are ordered on the current stream; use the cache on
+    one stream at a time. A grow(), evict(), keep(), reorder() or release() that changes a row's pages sends the table
+    anew and waits for the stream (a budget that is a multiple of page_size takes and frees a page each step)."""
 
     def __init__(self, layers: int, heads: int, head_dim: int, *, rows: int, max_len: int, pages: int | None = None,
                  page_size: int = 64, dtype: torch.dtype = torch.float16, device="cuda", evictable: bool = False):
@@ -260,7 +262,8 @@ class PagedKVCache:
     def attend_new(self, layer: int, q, *, parents=None, scale: float | None = None, out_dtype=None):
         """tree_attention of the tokens that grow() made room for, row by row: q has a query for each. parents: int32 on
         the device, the number within its row of the token that each one continues (-1: the row's sequence); None: each
-        continues the one before it. An evictable cache's scores stay as they are."""
+        continues the one before it. An evictable cache's scores stay as they are: a later evict() knows nothing of these
+        tokens' attention."""
         if self._positions is None:
             raise ValueError("grow() first")
         new = self._positions.shape[0]
