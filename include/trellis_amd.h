@@ -315,7 +315,8 @@ int trellis_kv_evict(const trellis_kv_cache *cache, int keep, int recent, const 
  *   out: [tokens][q_heads][head_dim] contiguous of out_dtype, 16-byte aligned
  * A token of no row, one whose slot the table (or max_len) does not hold, and one all of whose tokens
  * lie on pages that do not exist give 0. Keys and values of a row's tokens are finite, those of tokens
- * that another one does not see included. Workspace as for trellis_paged_attention. */
+ * that another one does not see included (bf16 values up to 2^124 / the row's tokens in size, so that
+ * the fp32 sums of up to 16 times them are). Workspace as for trellis_paged_attention. */
 int trellis_tree_attention_workspace_bytes(const trellis_kv_cache *cache, int tokens, int q_heads,
                                            int q_dtype, int out_dtype, size_t *bytes);
 int trellis_tree_attention(const trellis_kv_cache *cache, const void *q, int64_t q_token_stride,

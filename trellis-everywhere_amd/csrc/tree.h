@@ -23,7 +23,8 @@
 // it, half a step, as out is itself: the error against float64 (rms) is 1.1 (rows of thousands of tokens in f16) to 1.3 times
 // (bf16, 1024 tokens behind 8192) that of a result rounded once, and the terms that attend.h takes would be two or three times
 // the second product's instructions. Other types take those terms, of q too: 1024 fp32 queries behind 8192 f16 tokens 366 us,
-// bf16 ones 457, for the 170 of 16-bit types.
+// bf16 ones 457, for the 170 of 16-bit types. The sums are of weights up to 2^15 (f16) or 2^4 (bf16): bf16 values of 2^124 /
+// tokens and more in size can overflow them.
 // Bound: new tokens of few queries a key (32 rows of up to 8192 tokens, up to 26 new each, 32 heads over 8 of 128) by
 // memory: 107-112 us, 4.9 TB/s and 13 MiB of partial sums. Many by the loop's own latencies: 1024 tokens behind 8192
 // 160-177 us, 870 TFLOP/s, the matrix cores busy 48 % of the time and the vector units 44 %; LDS has no conflicts (heads of 64

@@ -8,7 +8,8 @@ forward only. Arguments are checked in csrc/bind.cpp.
 append_kv, paged_attention, tree_attention, evict_kv, copy_pages and keep_kv work on tensors that the caller owns;
 PagedKVCache owns them.
 
-  k_pages, v_pages: [pages, heads, page_size, head_dim] float16 or bfloat16; alike in strides, unit last
+  k_pages, v_pages: [pages, heads, page_size, head_dim] float16 or bfloat16; alike in strides, unit last; bfloat16
+         values up to 2^124 / (a row's tokens) in size (the attention's sums of up to 16 times them are fp32)
   table: int32 [rows, width], row b's token j in slot j % page_size of page table[b, j // page_size]; an
          id outside the pool is no page (nothing is written, its tokens count as absent)
   lens:  int32 [rows], tokens per row
